@@ -288,6 +288,104 @@ cudaError_t mkb_ipc_close(void* device_ptr);
 int mkb_engine_grid(mkb_engine* e);
 void mkb_engine_destroy(mkb_engine* e);
 
+/* ---- batched serving: packed prompts and a paged cache --------------------------
+ * Operators for many requests at once (no counterpart in the reference, which
+ * decodes one stream over a contiguous cache). `batch` requests bring their new
+ * tokens packed one after another: request b's are rows cu_q[b] .. cu_q[b+1] - 1
+ * (device int[batch + 1], ascending, first 0, last `tokens`); cu_q NULL means
+ * q_len tokens each (tokens == batch * q_len). Query head h reads KV head
+ * h / (heads / kv_heads). Strides are in elements; the last dimension (head_dim,
+ * 64 or 128) is contiguous; every base is 16-byte aligned and every other stride
+ * a multiple of 8 elements.
+ *
+ * The paged cache is two pools of pages, addressed as page * stride[0] + KV head *
+ * stride[1] + slot * stride[2]. Key j of request b lies in page block_table[b,
+ * j / page_size], slot j % page_size; kv_lens[b] counts its keys, this call's new
+ * tokens included, so token i of the request's n new ones is at position
+ * kv_lens[b] - n + i. Table entries past a request's last key are not read.
+ *
+ * A token sees the keys at its own position and before it. One that sees none (a
+ * negative position) gets zeros. What lies in the cache past a request's last key
+ * (uninitialised memory, NaN) reaches no output.
+ *
+ * Lengths live on the device, so they are checked there: a page outside the pool,
+ * more keys than the table has room for, or a position past the RoPE tables makes
+ * the rows that need it NaN, touches no memory out of range, and is recorded in
+ * *status (0 = ok; first code kept). */
+enum { MKB_BF16 = 0, MKB_FP16 = 1, MKB_FP32 = 2 };
+enum {
+  MKB_SERVE_BAD_PAGE = 1,      /* block_table names a page outside the pool */
+  MKB_SERVE_BAD_LENGTH = 2,    /* kv_lens[b] exceeds the table's width in keys */
+  MKB_SERVE_BAD_POSITION = 3,  /* a position past the RoPE tables (append) */
+  MKB_SERVE_TIMEOUT = 4        /* a bounded wait inside the kernel expired */
+};
+
+typedef struct mkb_attn_args {
+  int dtype;                   /* MKB_BF16 or MKB_FP16: q, k, v and out */
+  int heads, kv_heads, head_dim;
+  int tokens, batch, q_len;
+  const int* cu_q;             /* device int[batch + 1] or NULL */
+  const void* q;               /* [tokens, heads, head_dim] */
+  int64_t q_stride[2];         /* token, head */
+  void* out;                   /* [tokens, heads, head_dim] */
+  int64_t out_stride[2];
+  const void* k;               /* prompt: [tokens, kv_heads, head_dim]; paged: the pool */
+  const void* v;
+  int64_t k_stride[3];         /* prompt: token, head, unused; paged: page, head, slot */
+  int64_t v_stride[3];
+  const int* kv_lens;          /* paged: device int[batch] */
+  const int* block_table;      /* paged: device int[batch, table_width], rows table_stride apart */
+  int64_t table_stride;
+  int table_width, pages, page_size; /* page_size a power of two, 16 or more */
+  float scale;                 /* scores are scale * q.k */
+  void* workspace;             /* device, mkb_attn_workspace_bytes(); zeroed once with
+                                  mkb_attn_workspace_reset and left zeroed by every call.
+                                  Calls that share one must not overlap in time. */
+  uint32_t* status;            /* device uint32 or NULL */
+} mkb_attn_args;
+
+typedef struct mkb_append_args {
+  int dtype, source_dtype;     /* caches, q and k_out; qkv (MKB_BF16, MKB_FP16 or MKB_FP32) */
+  int heads, kv_heads, head_dim;
+  int tokens, batch, q_len;
+  const int* cu_q;
+  const void* qkv;             /* [tokens, heads + 2 kv_heads, head_dim]: q, k, v heads */
+  int64_t qkv_stride[2];       /* token, head */
+  const void* q_norm;          /* [head_dim] of the cache's type, or NULL: no norm */
+  const void* k_norm;
+  float eps;
+  const void* cos_table;       /* [table_rows, head_dim] contiguous, FP32 or the cache's type */
+  const void* sin_table;
+  int rope_fp32, rope_rows;
+  void* q_out;                 /* [tokens, heads, head_dim] contiguous */
+  void* k_out;                 /* [tokens, kv_heads, head_dim] contiguous, or NULL */
+  void* k_cache;
+  void* v_cache;
+  int64_t k_stride[3];         /* page, head, slot */
+  int64_t v_stride[3];
+  const int* kv_lens;
+  const int* block_table;
+  int64_t table_stride;
+  int table_width, pages, page_size;
+  uint32_t* status;
+} mkb_append_args;
+
+/* Causal attention of whole prompts packed one after another: a token sees the
+ * tokens of its own prompt up to itself. k and v are packed like q; kv_lens, the
+ * table and the paging fields are not used. Asynchronous. */
+cudaError_t mkb_prompt_attention(const mkb_attn_args* a, cudaStream_t stream);
+/* Attention of every request's new tokens (one each when decoding, a chunk of a
+ * prompt, or a mix) over its keys in the paged cache. Asynchronous. */
+cudaError_t mkb_paged_attention(const mkb_attn_args* a, cudaStream_t stream);
+/* Before them: RMSNorm of every q and k head (where its weight is given),
+ * rotate-half RoPE at the token's position, q to q_out, k and v to the cache (k
+ * also to k_out, packed). Two tokens at the same page and slot race. Asynchronous. */
+cudaError_t mkb_paged_append(const mkb_append_args* a, cudaStream_t stream);
+/* Bytes of workspace an attention call with these arguments needs (tokens, batch,
+ * heads, kv_heads, head_dim and q_len / cu_q are read). */
+size_t mkb_attn_workspace_bytes(const mkb_attn_args* a);
+cudaError_t mkb_attn_workspace_reset(void* workspace, size_t bytes, cudaStream_t stream);
+
 /* ---- schedule introspection (host only, no GPU needed) ------------------------ */
 /* out[0..13] = qa, qb, in_bc, h, c, oa, ob, ja, jb, da, db, va, vb, group_size. */
 int mkb_plan_query(int grid, int cta, int32_t out[16]);

@@ -8,7 +8,10 @@ Drop-in for the reference's decode path (tejeshbhalla/mega-kernel):
 * :func:`extension` -- the PyTorch extension ``megakernel_extension`` with the
   reference's ``decode(...)`` call (pytorch_binding.cu:36-48);
 * :class:`DecodeEngine` -- the resident engine (weights table, transposed down
-  weights, workspace and CUDA graph kept across tokens).
+  weights, workspace and CUDA graph kept across tokens);
+* :mod:`megakernel_b200.serving` -- the attention steps of many requests at once
+  over a paged cache (:func:`paged_append`, :func:`prompt_attention`,
+  :func:`paged_attention`).
 
 There is no CPU or PyTorch fallback: without the built library every entry
 point raises.
@@ -18,6 +21,7 @@ from __future__ import annotations
 from . import _lib
 from .engine import DecodeEngine, check_model, decode_call
 from .rope import rope_tables
+from .serving import paged_append, paged_attention, prompt_attention, serving_status
 
 _ext = None
 
@@ -36,4 +40,5 @@ def decode(*args, **kwargs):
     return extension().decode(*args, **kwargs)
 
 
-__all__ = ["DecodeEngine", "decode", "decode_call", "extension", "rope_tables", "check_model", "_lib"]
+__all__ = ["DecodeEngine", "decode", "decode_call", "extension", "rope_tables", "check_model", "_lib",
+           "paged_append", "paged_attention", "prompt_attention", "serving_status"]

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import (POINTER, Structure, c_float, c_int, c_int32, c_size_t, c_uint32,
+from ctypes import (POINTER, Structure, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32,
                     c_ulonglong, c_void_p, c_char_p)
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -99,6 +99,46 @@ class Model(Structure):
     ]
 
 
+class AttnArgs(Structure):
+    """Mirror of ``mkb_attn_args``."""
+
+    _fields_ = [
+        ("dtype", c_int), ("heads", c_int), ("kv_heads", c_int), ("head_dim", c_int),
+        ("tokens", c_int), ("batch", c_int), ("q_len", c_int),
+        ("cu_q", c_void_p),
+        ("q", c_void_p), ("q_stride", c_int64 * 2),
+        ("out", c_void_p), ("out_stride", c_int64 * 2),
+        ("k", c_void_p), ("v", c_void_p),
+        ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3),
+        ("kv_lens", c_void_p), ("block_table", c_void_p), ("table_stride", c_int64),
+        ("table_width", c_int), ("pages", c_int), ("page_size", c_int),
+        ("scale", c_float),
+        ("workspace", c_void_p),
+        ("status", c_void_p),
+    ]
+
+
+class AppendArgs(Structure):
+    """Mirror of ``mkb_append_args``."""
+
+    _fields_ = [
+        ("dtype", c_int), ("source_dtype", c_int),
+        ("heads", c_int), ("kv_heads", c_int), ("head_dim", c_int),
+        ("tokens", c_int), ("batch", c_int), ("q_len", c_int),
+        ("cu_q", c_void_p),
+        ("qkv", c_void_p), ("qkv_stride", c_int64 * 2),
+        ("q_norm", c_void_p), ("k_norm", c_void_p), ("eps", c_float),
+        ("cos_table", c_void_p), ("sin_table", c_void_p),
+        ("rope_fp32", c_int), ("rope_rows", c_int),
+        ("q_out", c_void_p), ("k_out", c_void_p),
+        ("k_cache", c_void_p), ("v_cache", c_void_p),
+        ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3),
+        ("kv_lens", c_void_p), ("block_table", c_void_p), ("table_stride", c_int64),
+        ("table_width", c_int), ("pages", c_int), ("page_size", c_int),
+        ("status", c_void_p),
+    ]
+
+
 # (name, restype, argtypes) for every symbol declared in include/mkb200.h
 SIGNATURES = [
     ("launch_decode_kernel", c_int,
@@ -137,6 +177,11 @@ SIGNATURES = [
     ("mkb_ipc_close", c_int, [c_void_p]),
     ("mkb_engine_grid", c_int, [c_void_p]),
     ("mkb_engine_destroy", None, [c_void_p]),
+    ("mkb_prompt_attention", c_int, [POINTER(AttnArgs), c_void_p]),
+    ("mkb_paged_attention", c_int, [POINTER(AttnArgs), c_void_p]),
+    ("mkb_paged_append", c_int, [POINTER(AppendArgs), c_void_p]),
+    ("mkb_attn_workspace_bytes", c_size_t, [POINTER(AttnArgs)]),
+    ("mkb_attn_workspace_reset", c_int, [c_void_p, c_size_t, c_void_p]),
     ("mkb_plan_query", c_int, [c_int, c_int, POINTER(c_int32)]),
     ("mkb_plan_query_tp", c_int, [c_int, c_int, c_int, c_int, POINTER(c_int32)]),
     ("mkb_qkv_global_row", c_int, [c_int, c_int, c_int]),

@@ -21,7 +21,8 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(HERE, "libmkb200.so")
 EXT_DIR = os.path.join(HERE, "_build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-KERNEL_SOURCES = ["mkb_decode.cu", "mkb_host.cu", "mkb_noalloc.cu", "mkb_prefill.cu"]
+KERNEL_SOURCES = ["mkb_decode.cu", "mkb_host.cu", "mkb_noalloc.cu", "mkb_prefill.cu", "mkb_append.cu", "mkb_attn.cu"]
+EXT_SOURCES = ["binding.cpp", "binding_serving.cpp"]
 
 
 def nvcc() -> str:
@@ -42,13 +43,35 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
     deps.append(os.path.join(INCLUDE, "mkb200.h"))
     if not force and not _stale(LIB, deps):
         return LIB
-    cmd = [nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xptxas", "-v", "-shared",
-           "-Xcompiler", "-fPIC", "-Xlinker", "-soname=libmkb200.so", "-o", LIB, *srcs]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    # one object per source, compiled side by side; an object newer than its source and every header stays
+    heads = [d for d in deps if not d.endswith(".cu")]
+    obj_dir = os.path.join(EXT_DIR, "obj")
+    os.makedirs(obj_dir, exist_ok=True)
+    objs, running = [], []
+    for s in srcs:
+        o = os.path.join(obj_dir, os.path.basename(s) + ".o")
+        objs.append(o)
+        if force or _stale(o, [s, *heads]):
+            part = f"{o}.{os.getpid()}"
+            cmd = [nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xptxas", "-v", "-Xcompiler", "-fPIC",
+                   "-c", "-o", part, s]
+            running.append((o, part, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    failed = False
+    for o, part, p in running:
+        text = p.communicate()[0]
+        if verbose or p.returncode != 0:
+            sys.stderr.write(text)
+        failed |= p.returncode != 0
+        if p.returncode == 0:
+            os.replace(part, o)
+    if failed:
+        raise RuntimeError("nvcc failed building libmkb200.so")
+    r = subprocess.run([nvcc(), *ARCH, "-shared", "-Xlinker", "-soname=libmkb200.so", "-o", LIB, *objs],
+                       capture_output=True, text=True)
     if verbose or r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
     if r.returncode != 0:
-        raise RuntimeError("nvcc failed building libmkb200.so")
+        raise RuntimeError("nvcc failed linking libmkb200.so")
     return LIB
 
 
@@ -64,7 +87,7 @@ def build_extension(verbose: bool = False):
     ctypes.CDLL(LIB, mode=ctypes.RTLD_GLOBAL)
     os.makedirs(EXT_DIR, exist_ok=True)
     prebuilt = os.path.join(EXT_DIR, "megakernel_extension.so")
-    deps = [os.path.join(CSRC, "binding.cpp"), os.path.join(INCLUDE, "mkb200.h")]
+    deps = [os.path.join(CSRC, f) for f in EXT_SOURCES] + [os.path.join(INCLUDE, "mkb200.h")]
     if not _stale(prebuilt, deps):
         import importlib.machinery
         import importlib.util
@@ -75,7 +98,7 @@ def build_extension(verbose: bool = False):
         return mod
     return load(
         name="megakernel_extension",
-        sources=[os.path.join(CSRC, "binding.cpp")],
+        sources=[os.path.join(CSRC, f) for f in EXT_SOURCES],
         extra_include_paths=[INCLUDE],
         extra_cflags=["-O3", "-std=c++17"],
         extra_ldflags=[f"-L{HERE}", "-lmkb200"],

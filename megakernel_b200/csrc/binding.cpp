@@ -152,7 +152,10 @@ std::vector<int64_t> status(int64_t device) {
   return std::vector<int64_t>(out, out + 8);
 }
 
+void register_serving(pybind11::module_& module);  // binding_serving.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, module) {
   module.def("decode", &decode, "Qwen3 single-token decode (B200 engine)");
   module.def("status", &status, "in-kernel status of the decode workspace on a device");
+  register_serving(module);
 }

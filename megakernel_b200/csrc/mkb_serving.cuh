@@ -1,0 +1,98 @@
+// Shared by the batched-serving kernels: types, the packed batch's layout, and
+// where a request's keys lie in the paged cache.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/mkb200.h"
+#include "mkb_ptx.cuh"
+
+namespace mkb {
+namespace sv {
+
+// ---- two values of a 16-bit type in one word, and back --------------------------
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 get(uint32_t u) { return make_float2(bf_lo(u), bf_hi(u)); }
+  static __device__ __forceinline__ uint32_t put(float a, float b) { return pack_bf2(a, b); }
+  static constexpr int kDtype = MKB_BF16;
+};
+template <>
+struct Pair<__half> {
+  static __device__ __forceinline__ float2 get(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+  static __device__ __forceinline__ uint32_t put(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static constexpr int kDtype = MKB_FP16;
+};
+
+// eight consecutive values from 16 (or 32) aligned bytes
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float v[8]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Pair<T>::get(w[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float v[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float v[8]) {
+  return make_uint4(Pair<T>::put(v[0], v[1]), Pair<T>::put(v[2], v[3]), Pair<T>::put(v[4], v[5]),
+                    Pair<T>::put(v[6], v[7]));
+}
+
+// ---- the packed batch ---------------------------------------------------------------
+
+// The request of packed token `t` (every lane of a warp calls it, all with the same
+// t): how many of cu[1 .. batch] are <= t. 32 probes at a time: one load deep up to
+// 32 requests, two up to 1,024.
+__device__ __forceinline__ int request_of(const int* __restrict__ cu, int batch, int t) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = batch;  // the answer lies in [lo, lo + n], cu[lo] <= t
+  while (n > 0) {
+    const int step = (n + 31) / 32;
+    const int at = lo + (lane + 1) * step;  // probes cu[at], the last of its stretch
+    const bool below = at <= lo + n && __ldg(cu + at) <= t;
+    const int full = __popc(__ballot_sync(0xffffffffu, below));
+    lo += full * step;
+    n = step == 1 ? 0 : min(step - 1, n - full * step);
+  }
+  return min(lo, batch - 1);
+}
+
+// Where packed token `t`'s request lies: its rows first .. first + n - 1, clamped to
+// the batch so that no offsets of the caller's lead out of it.
+struct Request {
+  int b, first, n;
+};
+__device__ __forceinline__ Request request_rows(const int* __restrict__ cu, int b, int q_len, int tokens) {
+  if (cu == nullptr) return {b, b * q_len, q_len};
+  const int first = min(max(__ldg(cu + b), 0), tokens);
+  return {b, first, max(min(__ldg(cu + b + 1), tokens) - first, 0)};
+}
+__device__ __forceinline__ Request request_at(const int* __restrict__ cu, int batch, int q_len, int tokens, int t) {
+  return request_rows(cu, cu == nullptr ? t / q_len : request_of(cu, batch, t), q_len, tokens);
+}
+
+// Records the first error of a launch.
+__device__ __forceinline__ void report(uint32_t* status, uint32_t code) {
+  if (status != nullptr) atomicCAS(status, 0u, code);
+}
+
+}  // namespace sv
+}  // namespace mkb
