@@ -57,6 +57,11 @@ void check_layout(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, " must be 16-byte aligned");
 }
 
+// keys at places of their own (dimension i not expanded)
+void check_apart(const Tensor& t, const char* name, int64_t i) {
+  TORCH_CHECK_VALUE(t.size(i) <= 1 || t.stride(i) != 0, name, " must not be expanded along dimension ", i);
+}
+
 int64_t stride_of(const Tensor& t, int64_t i) { return t.size(i) <= 1 ? 0 : t.stride(i); }
 
 void check_type(const Tensor& t, const char* name, const Tensor& like, const char* like_name) {
@@ -204,6 +209,10 @@ Paging paging_of(const Tensor& k_cache, const Tensor& v_cache, const Tensor& blo
   check_type(v_cache, "v_cache", k_cache, "k_cache");
   check_layout(k_cache, "k_cache");
   check_layout(v_cache, "v_cache");
+  for (const int i : {0, 2}) {
+    check_apart(k_cache, "k_cache", i);
+    check_apart(v_cache, "v_cache", i);
+  }
   p.pages = as_int(k_cache.size(0), "pages");
   p.kv_heads = as_int(k_cache.size(1), "kv_heads");
   p.page_size = as_int(k_cache.size(2), "page_size");
@@ -241,6 +250,8 @@ Tensor prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   check_layout(q, "q");
   check_layout(k, "k");
   check_layout(v, "v");
+  check_apart(k, "k", 0);
+  check_apart(v, "v", 0);
   TORCH_CHECK_VALUE(cu_seqlens.dim() == 1 && cu_seqlens.size(0) >= 1, "cu_seqlens must be [prompts + 1]");
   const Batch b = batch_of(q, "q", cu_seqlens, cu_seqlens.size(0) - 1, dev);
   const c10::cuda::CUDAGuard guard(dev);

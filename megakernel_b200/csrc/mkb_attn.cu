@@ -117,6 +117,10 @@ cudaError_t launch_dim(const mkb_attn_args& a, cudaStream_t stream) {
   return a.head_dim == 128 ? launch_rows<T, 128, kPaged>(a, stream) : launch_rows<T, 64, kPaged>(a, stream);
 }
 
+
+cudaError_t attn_tc(const mkb_attn_args& a, bool paged, cudaStream_t stream);  // mkb_attn_tc.cu
+size_t tc_workspace(const mkb_attn_args& a);
+
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 static bool strides_ok(const int64_t* s, int n) {
   for (int i = 0; i < n; ++i)
@@ -135,6 +139,7 @@ static cudaError_t check_attn(const mkb_attn_args* a, bool paged) {
   if (a->tokens == 0) return cudaSuccess;
   if (a->cu_q == nullptr && (a->q_len < 1 || (int64_t)a->q_len * a->batch != a->tokens)) return cudaErrorInvalidValue;
   if (!a->q || !a->out) return cudaErrorInvalidValue;
+  if (static_cast<int64_t>(a->tokens) * (a->heads / a->kv_heads) > 0x7fff0000) return cudaErrorInvalidValue;
   if (paged) {
     if (!a->kv_lens || a->table_width < 0 || a->pages < 0) return cudaErrorInvalidValue;
     if (a->table_width > 0 && !a->block_table) return cudaErrorInvalidValue;
@@ -147,6 +152,10 @@ static cudaError_t check_attn(const mkb_attn_args* a, bool paged) {
       !strides_ok(a->q_stride, 2) || !strides_ok(a->out_stride, 2) || !strides_ok(a->k_stride, paged ? 3 : 2) ||
       !strides_ok(a->v_stride, paged ? 3 : 2))
     return cudaErrorMisalignedAddress;
+  // keys (and pages) lie at places of their own; KV heads may share one
+  if (paged ? a->pages > 0 && ((a->pages > 1 && (!a->k_stride[0] || !a->v_stride[0])) || !a->k_stride[2] || !a->v_stride[2])
+            : a->tokens > 1 && (!a->k_stride[0] || !a->v_stride[0]))
+    return cudaErrorInvalidValue;
   return cudaSuccess;
 }
 
@@ -156,8 +165,7 @@ static cudaError_t check_attn(const mkb_attn_args* a, bool paged) {
 extern "C" {
 
 size_t mkb_attn_workspace_bytes(const mkb_attn_args* a) {
-  (void)a;
-  return 256;
+  return mkb::sv::tc_workspace(*a);
 }
 
 cudaError_t mkb_attn_workspace_reset(void* workspace, size_t bytes, cudaStream_t stream) {
@@ -168,13 +176,14 @@ cudaError_t mkb_prompt_attention(const mkb_attn_args* a, cudaStream_t stream) {
   using namespace mkb::sv;
   const cudaError_t e = check_attn(a, false);
   if (e != cudaSuccess || a->tokens == 0) return e;
-  return a->dtype == MKB_BF16 ? launch_dim<__nv_bfloat16, false>(*a, stream) : launch_dim<__half, false>(*a, stream);
+  return attn_tc(*a, false, stream);
 }
 
 cudaError_t mkb_paged_attention(const mkb_attn_args* a, cudaStream_t stream) {
   using namespace mkb::sv;
   const cudaError_t e = check_attn(a, true);
   if (e != cudaSuccess || a->tokens == 0) return e;
+  if (a->cu_q != nullptr || a->q_len > 1) return attn_tc(*a, true, stream);
   return a->dtype == MKB_BF16 ? launch_dim<__nv_bfloat16, true>(*a, stream) : launch_dim<__half, true>(*a, stream);
 }
 }

@@ -1,0 +1,976 @@
+// Attention of a packed batch on the tensor cores: prompts, and chunks of new tokens
+// over the paged cache.
+//
+//   out_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = 2^(c q_i.k_j - m_i),  c = scale log2(e),  j <= pos(i)
+//
+// A KV head's queries are rows: row r of a request is token r / G, query head r % G of
+// the G that share the KV head, so that one pass over the keys serves all of them. A CTA
+// takes 256 rows (tiles A and B of 128) of one request and KV head and walks its keys
+// 128 at a time:
+//
+//   warp 9      which piece of work comes next, and its K and V tiles by TMA into a ring
+//               (128-byte swizzle; pages are boxes of page_size rows)
+//   warp 8      tcgen05.mma: S = Q K^T (Q and K in shared memory), O += P V with P from
+//               tensor memory and V as it lies, keys by dims (an MN-major operand: no
+//               transposed copy of V is made)
+//   warps 0-3   softmax of tile A, a thread per row: S out of tensor memory, running
+//   warps 4-7   maximum and sum in FP32 registers, P back into the columns S had; tile B
+//
+// While one tile's softmax runs, the tensor core works on the other's products. The
+// running maximum that P is relative to moves only when a row's grows by more than 8
+// (a factor 256): O, in tensor memory, is then rescaled by the softmax warps; between
+// moves P stays below 2^8, which FP32 sums and 16-bit P hold without loss. P is rounded
+// to the operands' 16-bit type, as the output is: the same relative error.
+//
+// Work: a piece is (request, KV head, 256 rows, a range of key tiles). Every CTA works
+// the list out for itself from the lengths, longest pieces first, and takes every
+// grid-th one, turning round after each sweep. Rows whose keys are more than a fair
+// share are split over several pieces; each writes its O, maximum and sum, and the last
+// to arrive adds them up in order of their keys, so results do not depend on timing.
+//
+// Masked places: scores are replaced, not added to. V rows past the request's last key
+// are cleared in shared memory. A tile that is partly masked for some row is scanned for
+// V that is not finite (0 * inf would reach rows that do not see it); where one is found,
+// those rows are computed again key by key.
+
+#include <cmath>
+#include <cuda.h>
+
+#include "mkb_serving.cuh"
+#include "mkb_tc.cuh"
+
+namespace mkb {
+namespace sv {
+
+constexpr int kTcThreads = 320;
+constexpr int kRows = 256, kKeys = 128;   // rows of a piece, keys of a tile
+constexpr int kHalf = 128 * 128;          // 16 KB: 128 rows x 64 values, 128-byte swizzle
+constexpr int kMinSplit = 6;              // key tiles below which rows are not split
+constexpr int kSortBatch = 128;           // requests up to which pieces are taken longest first
+constexpr unsigned long long kTimeoutNs = 1000000000ull;
+
+struct Piece {
+  int b;            // request, -1: no more work
+  int hk;
+  int first, q;     // the request's packed rows
+  int row0, rows;   // flattened rows (token * G + head)
+  int ctx, len;     // keys before the new tokens, all keys
+  int k0;           // first key tile
+  int n[2];         // key tiles of tiles A and B
+  int splits, split, slot;
+  int bad;
+};
+
+template <int D>
+struct TcSmem {
+  static constexpr int kTileBytes = D * 256;            // 128 keys
+  static constexpr int kSlots = D == 128 ? 5 : 8;
+  uint8_t q[2][kTileBytes];
+  uint8_t kv[kSlots][kTileBytes];
+  uint64_t kv_full[kSlots], kv_empty[kSlots];
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t info_full[2], info_empty[2];
+  uint64_t tile_bar[2];   // the four softmax warps of a tile
+  Piece piece[2];
+  uint32_t tmem_base;
+  int err;
+  int odd[2];             // the last piece (+ 1) whose masked tiles held V that is not finite
+  int last[2];
+};
+
+struct TcArgs {
+  mkb_attn_args a;
+  float sl2;            // scale * log2(e)
+  int group;            // query heads of a KV head
+  int k_head, v_head;   // 0 where every KV head lies at the same place (stride 0), else 1
+  int box;              // keys of a TMA box
+  int slots;            // partial results the workspace holds
+  uint32_t* counters;   // [slots][2], zero between calls
+  float4* part;         // [slots][D / 4][256]
+  float2* stat;         // [slots][256]: maximum, sum
+};
+
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t ph, int* err) {
+  if (mbar_test(bar, ph)) return true;
+  const uint64_t t0 = global_ns();
+  while (!mbar_wait(bar, ph, 20000)) {
+    if (*reinterpret_cast<volatile int*>(err) != 0) return false;
+    if (global_ns() - t0 > kTimeoutNs) {
+      *reinterpret_cast<volatile int*>(err) = 1;
+      return false;
+    }
+  }
+  return true;
+}
+// every lane of a warp; goes on only if all saw the phase
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t ph, int* err) {
+  return __all_sync(0xffffffffu, wait_bar(bar, ph, err));
+}
+
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w),
+      "r"(smem_addr(bar))
+      : "memory");
+}
+
+// Descriptor of an operand whose contiguous dimension is N, written by TMA with the
+// 128-byte swizzle: 64 values of N a row, eight rows (of K) to an atom of 1024 bytes;
+// `n_bytes` between 64-value blocks of N (leading offset), 1024 between atoms of K
+// (stride offset).
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t n_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((addr >> 4) & 0x3fffu);
+  d |= static_cast<uint64_t>((n_bytes >> 4) & 0x3fffu) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+// FP32 accumulator, A and B of type T (FP16 0, BF16 1), B N-major where `mn`
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc16(int m, int n, bool mn) {
+  constexpr uint32_t f = Pair<T>::kDtype == MKB_BF16 ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | (mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+// D[tmem] (+)= A[tmem] B[smem desc]
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32_u(uint32_t taddr, const uint32_t v[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
+        "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
+        "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// two FP32 operations in one instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// ---- the list of pieces, worked out by one warp -------------------------------------
+
+// One request as the list sees it.
+struct Load {
+  int first, q, len, ctx, blocks, tiles, splits, bad;
+};
+template <bool kPaged>
+__device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
+  const Request rq = request_rows(g.a.cu_q, b, g.a.q_len, g.a.tokens);
+  Load l;
+  l.first = rq.first;
+  l.q = rq.n;
+  l.len = kPaged ? max(__ldg(g.a.kv_lens + b), 0) : rq.n;
+  l.bad = kPaged && static_cast<int64_t>(l.len) > static_cast<int64_t>(g.a.table_width) * g.a.page_size;
+  l.ctx = l.len - l.q;
+  l.blocks = static_cast<int>((static_cast<int64_t>(l.q) * g.group + kRows - 1) / kRows);
+  l.tiles = l.bad || l.blocks == 0 ? 0 : (l.len + kKeys - 1) / kKeys;
+  l.splits = 1;
+  return l;
+}
+// key tiles of row block i: up to its last token's position
+__device__ __forceinline__ int block_tiles(const Load& l, int group, int i) {
+  const int64_t last = min(static_cast<int64_t>(l.q), ((static_cast<int64_t>(i) + 1) * kRows - 1) / group + 1) - 1;
+  const int64_t keys = l.ctx + last + 1;
+  return l.bad || keys <= 0 ? 0 : static_cast<int>((keys + kKeys - 1) / kKeys);
+}
+// how many of the request's row blocks have more than x key tiles (they come last)
+__device__ __forceinline__ int blocks_above(const Load& l, int group, int64_t x) {
+  if (x < 0) return l.blocks;
+  if (l.tiles <= x) return 0;
+  const int64_t y = x * kKeys - l.ctx;  // the first token that sees more than x tiles
+  if (y <= 0) return l.blocks;
+  const int64_t i = y * group / kRows;
+  return i >= l.blocks ? 0 : l.blocks - static_cast<int>(i);
+}
+
+// ---- one row, key by key: what a tile with values that are not finite comes to --------
+// Warp-wide; lane holds dims [lane * D / 32, + D / 32) of O, relative to maximum m.
+template <typename T, int D, bool kPaged>
+__device__ __noinline__ void slow_row(const TcArgs& g, const Piece& p, int row, int k_end, float* o, float* m_out,
+                                      float* l_out) {
+  const mkb_attn_args& a = g.a;
+  const int lane = threadIdx.x & 31;
+  constexpr int kPer = D / 32;
+  const int token = row / g.group, h = p.hk * g.group + row % g.group;
+  const T* q = static_cast<const T*>(a.q) + (p.first + token) * a.q_stride[0] + h * a.q_stride[1];
+  const int keys = min(k_end, p.ctx + token + 1);
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) o[i] = 0.f;
+  for (int j = p.k0 * kKeys; j < keys; ++j) {
+    int64_t ko, vo;
+    if (kPaged) {
+      const int64_t page = a.block_table[p.b * a.table_stride + j / a.page_size], slot = j % a.page_size;
+      if (page < 0 || page >= a.pages) continue;  // reported; the piece is NaN already
+      ko = page * a.k_stride[0] + p.hk * a.k_stride[1] + slot * a.k_stride[2];
+      vo = page * a.v_stride[0] + p.hk * a.v_stride[1] + slot * a.v_stride[2];
+    } else {
+      ko = static_cast<int64_t>(p.first + j) * a.k_stride[0] + p.hk * a.k_stride[1];
+      vo = static_cast<int64_t>(p.first + j) * a.v_stride[0] + p.hk * a.v_stride[1];
+    }
+    const uint32_t* k2 = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.k) + ko);
+    const uint32_t* v2 = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.v) + vo);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i) {
+      const float2 x = Pair<T>::get(reinterpret_cast<const uint32_t*>(q)[lane * (kPer / 2) + i]);
+      const float2 y = Pair<T>::get(k2[lane * (kPer / 2) + i]);
+      s += x.x * y.x + x.y * y.y;
+    }
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    s *= g.sl2;
+    const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
+    const float sc = ex2_approx(m - ref), w = ex2_approx(s - ref);
+    l = l * sc + w;
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i) {
+      const float2 y = Pair<T>::get(v2[lane * (kPer / 2) + i]);
+      o[2 * i] = o[2 * i] * sc + w * y.x;
+      o[2 * i + 1] = o[2 * i + 1] * sc + w * y.y;
+    }
+    m = mn;
+  }
+  *m_out = m;
+  *l_out = l;
+}
+
+template <typename T, int D, bool kPaged>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                   const __grid_constant__ TcArgs g) {
+  using Smem = TcSmem<D>;
+  constexpr int kSlots = Smem::kSlots, kTileBytes = Smem::kTileBytes;
+  extern __shared__ uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const mkb_attn_args& a = g.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&sm.kv_full[s], 1);
+      mbar_init(&sm.kv_empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&sm.q_full[t], 4);
+      mbar_init(&sm.s_full[t], 1);
+      mbar_init(&sm.p_full[t], 4);
+      mbar_init(&sm.o_full[t], 1);
+      mbar_init(&sm.info_full[t], 1);
+      mbar_init(&sm.tile_bar[t], 4);
+      mbar_init(&sm.info_empty[t], 9);  // eight softmax warps and the MMA warp
+    }
+    sm.err = sm.odd[0] = sm.odd[1] = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tc::tmem_alloc(&sm.tmem_base, 512);
+    tc::tmem_relinquish();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tbase = sm.tmem_base;  // S/P of A and B at 0 and 128, O at 256 and 384
+
+  if (warp == 9) {
+    // ---- the next piece, and its loads ------------------------------------------------
+    if (lane == 0) {
+      tc::prefetch_tensormap(&tk);
+      tc::prefetch_tensormap(&tv);
+    }
+    const int kv_heads = a.kv_heads, grid = gridDim.x;
+    // a fair share of the key tiles; rows with more are split
+    long long total = 0;
+    int top = 0;
+    for (int b = lane; b < a.batch; b += 32) {
+      const Load l = load_of<kPaged>(g, b);
+      if (l.blocks == 0) continue;
+      total += static_cast<long long>(block_tiles(l, g.group, 0) + l.tiles) * l.blocks;  // twice the sum: linear in i
+      top = max(top, l.tiles);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    top = __reduce_max_sync(0xffffffffu, top);
+    total = total * kv_heads / 2;
+    const int share = static_cast<int>(min(total * 5 / (4 * grid) + 1, 0x7fffffffll));
+    const int cap = max(kMinSplit, share);
+    auto with_splits = [&](int b) {
+      Load l = load_of<kPaged>(g, b);
+      l.splits = l.tiles > cap ? (l.tiles + cap - 1) / cap : 1;
+      return l;
+    };
+    // pieces of more than x tiles, all requests
+    auto pieces_above = [&](int x) {
+      long long n = 0;
+      for (int b = lane; b < a.batch; b += 32) {
+        const Load l = with_splits(b);
+        n += static_cast<long long>(blocks_above(l, g.group, static_cast<int64_t>(x) * l.splits)) * l.splits;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+      return n * kv_heads;
+    };
+    const bool sorted = a.batch <= kSortBatch && a.batch > 0;
+    int it = 0, k = 0;
+    bool ok = true;
+    for (; ok; ++k) {
+      const int st = k & 1;
+      const long long want = static_cast<long long>(k) * grid + (k & 1 ? grid - 1 - blockIdx.x : blockIdx.x);
+      Piece p;
+      p.b = -1;
+      // the level (tiles of a piece) that `want` falls into, and its place there
+      int lo = 0;
+      long long r = want;
+      if (sorted) {
+        int hi = min(cap, top);
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (pieces_above(mid) <= want) hi = mid;
+          else lo = mid + 1;
+        }
+        r = want - pieces_above(lo);
+      }
+      int slot_base = 0;
+      for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        const int b = b0 + lane;
+        Load l = {};
+        int above = 0, here = 0, slots = 0;
+        if (b < a.batch) {
+          l = with_splits(b);
+          if (sorted) {
+            above = blocks_above(l, g.group, static_cast<int64_t>(lo) * l.splits);
+            here = blocks_above(l, g.group, static_cast<int64_t>(lo) * l.splits - l.splits) - above;
+          } else {
+            here = l.blocks;
+          }
+          here *= l.splits * kv_heads;
+          slots = l.splits > 1 ? l.blocks * l.splits * kv_heads : 0;
+        }
+        int inc = here, sinc = slots;  // inclusive prefix sums
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, inc, o), y = __shfl_up_sync(0xffffffffu, sinc, o);
+          if (lane >= o) {
+            inc += x;
+            sinc += y;
+          }
+        }
+        const bool mine = r >= inc - here && r < inc;
+        const uint32_t who = __ballot_sync(0xffffffffu, mine);
+        if (who != 0) {
+          if (mine) {
+            int at = static_cast<int>(r) - (inc - here);
+            p.b = b;
+            p.split = at % l.splits;
+            at /= l.splits;
+            p.hk = at % kv_heads;
+            const int i = l.blocks - 1 - above - at / kv_heads;  // longest first
+            p.first = l.first;
+            p.q = l.q;
+            p.len = l.len;
+            p.ctx = l.ctx;
+            p.row0 = i * kRows;
+            p.rows = static_cast<int>(min(static_cast<int64_t>(l.q) * g.group - p.row0, static_cast<int64_t>(kRows)));
+            const int n = block_tiles(l, g.group, i), per = (n + l.splits - 1) / l.splits;
+            p.k0 = min(p.split * per, n);
+            const int k1 = min(p.k0 + per, n);
+            p.splits = l.splits;
+            p.slot = slot_base + sinc - slots + (i * kv_heads + p.hk) * l.splits;
+            p.bad = l.bad;
+            for (int t = 0; t < 2; ++t) {  // up to the tile's last row's position
+              const int last = min(p.rows, 128 * (t + 1)) - 1;
+              const int keys = p.ctx + (p.row0 + last) / g.group + 1;
+              const int end = keys <= 0 || p.bad ? 0 : (keys + kKeys - 1) / kKeys;
+              p.n[t] = p.rows > 128 * t ? max(min(end, k1) - p.k0, 0) : 0;
+            }
+            if (l.bad) report(a.status, MKB_SERVE_BAD_LENGTH);
+          }
+          const int src = __ffs(who) - 1;
+          uint32_t* w = reinterpret_cast<uint32_t*>(&p);
+#pragma unroll
+          for (int i = 0; i < static_cast<int>(sizeof(Piece) / 4); ++i) w[i] = __shfl_sync(0xffffffffu, w[i], src);
+          break;
+        }
+        r -= __shfl_sync(0xffffffffu, inc, 31);
+        slot_base += __shfl_sync(0xffffffffu, sinc, 31);
+      }
+      if (k >= 2 && !wait_warp(&sm.info_empty[st], ((k >> 1) - 1) & 1, &sm.err)) break;
+      if (lane == 0) {
+        sm.piece[st] = p;
+        mbar_arrive(&sm.info_full[st]);
+      }
+      __syncwarp();
+      if (p.b < 0) break;
+      // K(0), then K(j + 1) and V(j): the order in which the products take them
+      const int n = max(p.n[0], p.n[1]);
+      auto load = [&](const CUtensorMap* map, int head, int j) -> bool {
+        const int s = it % kSlots;
+        if (it >= kSlots && !wait_warp(&sm.kv_empty[s], (it / kSlots - 1) & 1, &sm.err)) return false;
+        ++it;
+        const int key = (p.k0 + j) * kKeys;
+        if (lane == 0) mbar_arrive_expect_tx(&sm.kv_full[s], kTileBytes);
+        __syncwarp();
+        if (kPaged) {
+          const int box = g.box;
+          if (lane * box < kKeys) {
+            const int at = key + lane * box;
+            int page = a.pages;  // past the last key: outside the pool, which reads as zeros
+            if (at < p.len) {
+              page = __ldg(a.block_table + p.b * a.table_stride + at / a.page_size);
+              if (page < 0 || page >= a.pages) {
+                page = a.pages;
+                *reinterpret_cast<volatile int*>(&sm.piece[st].bad) = 1;
+                report(a.status, MKB_SERVE_BAD_PAGE);
+              }
+            }
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d)
+              tma_4d(sm.kv[s] + d * kHalf + lane * box * 128, map, 64 * d, at % a.page_size, head, page,
+                     &sm.kv_full[s]);
+          }
+        } else if (lane == 0) {
+#pragma unroll
+          for (int d = 0; d < D / 64; ++d)
+            tma_3d(sm.kv[s] + d * kHalf, map, 64 * d, p.first + key, head, &sm.kv_full[s]);
+        }
+        return true;
+      };
+      const int kh = p.hk * g.k_head, vh = p.hk * g.v_head;
+      if (n > 0) ok = load(&tk, kh, 0);
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n) ok = load(&tk, kh, j + 1);
+        if (ok) ok = load(&tv, vh, j);
+      }
+    }
+    // after a stop, wait (bounded) for the copies still in flight before leaving
+    if (sm.err) {
+      const uint64_t t0 = global_ns();
+      for (int i = max(it - kSlots, 0); i < it; ++i)
+        while (!mbar_wait(&sm.kv_full[i % kSlots], (i / kSlots) & 1, 20000) && global_ns() - t0 < kTimeoutNs) {
+        }
+    }
+  } else if (warp == 8) {
+    // ---- the products -------------------------------------------------------------------
+    constexpr uint32_t id_s = idesc16<T>(128, kKeys, false), id_o = idesc16<T>(128, D, true);
+    const uint64_t dq0 = tc::desc_sw128(smem_addr(sm.q[0])), dk0 = tc::desc_sw128(smem_addr(sm.kv[0]));
+    const uint64_t dv0 = desc_mn_sw128(smem_addr(sm.kv[0]), kHalf);
+    int it = 0;                       // ring slots taken so far
+    uint32_t q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      const int st = k & 1;
+      if (!wait_warp(&sm.info_full[st], (k >> 1) & 1, &sm.err)) break;
+      const int nt[2] = {sm.piece[st].n[0], sm.piece[st].n[1]}, k0 = sm.piece[st].k0, len = sm.piece[st].len;
+      const bool stop = sm.piece[st].b < 0;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.info_empty[st]);
+      if (stop) break;
+      const int n = max(nt[0], nt[1]);
+      if (n == 0) continue;
+      auto slot_k = [&](int j) { return it + (j == 0 ? 0 : 2 * j - 1); };              // K0 K1 V0 K2 V1 ...
+      auto slot_v = [&](int j) { return it + (j + 1 < n ? 2 * j + 2 : 2 * n - 1); };
+      auto scores = [&](int t, int j) -> bool {  // S of tile t
+        const int i = slot_k(j), s = i % kSlots;
+        if (j == 0) {
+          if (!wait_warp(&sm.q_full[t], q_ph[t], &sm.err)) return false;
+          q_ph[t] ^= 1;
+        }
+        if (!wait_warp(&sm.kv_full[s], (i / kSlots) & 1, &sm.err)) return false;
+        tc::fence_after_sync();
+        if (lane == 0) {
+          const uint64_t dq = tc::desc_advance(dq0, t * kTileBytes), dk = tc::desc_advance(dk0, s * kTileBytes);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * kHalf + (kk & 3) * 32;
+            tc::mma_bf16_ss(tbase + 128 * t, tc::desc_advance(dq, off), tc::desc_advance(dk, off), id_s, kk != 0);
+          }
+          tc::commit(&sm.s_full[t]);
+        }
+        __syncwarp();
+        return true;
+      };
+      for (int t = 0; t < 2 && ok; ++t)
+        if (nt[t] > 0) ok = scores(t, 0);
+      if (ok && lane == 0) tc::commit(&sm.kv_empty[slot_k(0) % kSlots]);
+      for (int j = 0; j < n && ok; ++j) {
+        const int i = slot_v(j), s = i % kSlots;
+        if (!wait_warp(&sm.kv_full[s], (i / kSlots) & 1, &sm.err)) {
+          ok = false;
+          break;
+        }
+        const int valid = len - (k0 + j) * kKeys;
+        if (valid < kKeys) {  // rows past the last key: whatever lies there, P = 0 must give 0
+          const int chunks = (kKeys - valid) * 8;
+#pragma unroll
+          for (int d = 0; d < D / 64; ++d)
+            for (int c = lane; c < chunks; c += 32)
+              reinterpret_cast<uint4*>(sm.kv[s] + d * kHalf + valid * 128)[c] = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_shared();
+          __syncwarp();
+        }
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (j >= nt[t]) continue;
+          if (!(ok = wait_warp(&sm.p_full[t], p_ph[t], &sm.err))) break;
+          p_ph[t] ^= 1;
+          tc::fence_after_sync();
+          if (lane == 0) {
+            const uint64_t dv = tc::desc_advance(dv0, s * kTileBytes);
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk)
+              mma_ts(tbase + 256 + 128 * t, tbase + 128 * t + 8 * kk, tc::desc_advance(dv, kk * 2048), id_o,
+                     (j | kk) != 0);
+          }
+          __syncwarp();
+          if (j + 1 < nt[t]) {
+            ok = scores(t, j + 1);  // its commit covers O as well: S(j + 1) seen means PV(j) done
+          } else if (lane == 0) {
+            tc::commit(&sm.o_full[t]);
+          }
+        }
+        if (ok && lane == 0) {
+          tc::commit(&sm.kv_empty[s]);
+          if (j + 1 < n) tc::commit(&sm.kv_empty[slot_k(j + 1) % kSlots]);
+        }
+        __syncwarp();
+      }
+      it += 2 * n;
+    }
+  } else {
+    // ---- softmax of a tile, a thread per row ----------------------------------------------
+    const int t = warp >> 2;                 // tile
+    const int row_in = threadIdx.x & 127;    // row of the tile = TMEM lane
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    const uint32_t t_s = tbase + lanes + 128 * t, t_o = tbase + lanes + 256 + 128 * t;
+    const float sl2 = g.sl2;
+    uint32_t s_ph = 0, o_ph = 0;
+    int v_it = 0;                            // ring slots of earlier pieces
+    bool ok = true;
+    uint32_t t_ph = 0;
+    auto tile_sync = [&]() -> bool {         // a barrier of the tile's warps, bounded like every wait
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.tile_bar[t]);
+      const bool r = wait_warp(&sm.tile_bar[t], t_ph, &sm.err);
+      t_ph ^= 1;
+      return r;
+    };
+    for (int k = 0; ok; ++k) {
+      const int st = k & 1;
+      if (!wait_warp(&sm.info_full[st], (k >> 1) & 1, &sm.err)) break;
+      const Piece p = sm.piece[st];
+      const int n_all = max(p.n[0], p.n[1]);
+      auto release = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.info_empty[st]);
+      };
+      if (p.b < 0 || p.rows <= 128 * t) {
+        release();
+        if (p.b < 0) break;
+        v_it += 2 * n_all;
+        continue;
+      }
+      const int n = p.n[t];
+      const int row = p.row0 + 128 * t + row_in;     // of the request
+      const int rows_end = p.row0 + p.rows;
+      if (n > 0) {
+        // Q rows into the swizzled layout; rows past the request's are zeros
+        constexpr int kChunks = D / 8;               // 16-byte chunks of a row
+        for (int c = threadIdx.x & 127; c < 128 * kChunks; c += 128) {
+          const int r = c / kChunks, x = c % kChunks, rr = p.row0 + 128 * t + r;
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (rr < rows_end) {
+            const int token = rr / g.group, h = p.hk * g.group + rr - token * g.group;
+            u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (p.first + token) * a.q_stride[0] +
+                                                     h * a.q_stride[1]) + x);
+          }
+          *reinterpret_cast<uint4*>(sm.q[t] + (x >> 3) * kHalf + r * 128 + (((x & 7) ^ (r & 7)) << 4)) = u;
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.q_full[t]);
+      }
+      const int lim = p.ctx + min(row, rows_end - 1) / g.group;      // this row's last key
+      const int lim0 = p.ctx + (p.row0 + 128 * t) / g.group;         // the tile's least
+      float m = -INFINITY;                                           // in units of log2
+      uint64_t l2 = 0;                                               // two partial sums
+      bool slow = false;
+      for (int j = 0; j < n; ++j) {
+        if (!(ok = wait_warp(&sm.s_full[t], s_ph, &sm.err))) break;
+        s_ph ^= 1;
+        tc::fence_after_sync();
+        uint32_t sr[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc::tmem_ld32_nowait(t_s + 32 * c, sr[c]);
+        tc::tmem_wait_ld<true>(sr[0]);
+        tc::tmem_wait_ld<false>(sr[1]);
+        tc::tmem_wait_ld<false>(sr[2]);
+        tc::tmem_wait_ld<false>(sr[3]);
+        const int key0 = (p.k0 + j) * kKeys;
+        if (key0 + kKeys - 1 > lim0) {  // some row of the tile does not see all of these keys
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (key0 + i > lim) sr[i >> 5][i & 31] = 0xff800000u;
+          // V that is not finite would reach the rows that do not see it
+          const int i = v_it + (j + 1 < n_all ? 2 * j + 2 : 2 * n_all - 1), s = i % kSlots;
+          if (!(ok = wait_warp(&sm.kv_full[s], (i / kSlots) & 1, &sm.err))) break;
+          bool odd = false;
+          if (key0 + row_in < p.len) {
+            constexpr uint32_t e = Pair<T>::kDtype == MKB_BF16 ? 0x7f807f80u : 0x7c007c00u;
+            constexpr uint32_t el = e & 0xffffu, eh = e & 0xffff0000u;
+#pragma unroll 4
+            for (int c = 0; c < D / 8; ++c) {
+              const uint4 u = *reinterpret_cast<const uint4*>(sm.kv[s] + (c >> 3) * kHalf + row_in * 128 +
+                                                              (((c & 7) ^ (row_in & 7)) << 4));
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int q = 0; q < 4; ++q) odd |= (w[q] & el) == el || (w[q] & eh) == eh;
+            }
+          }
+          slow |= odd;
+        }
+        float mx = -INFINITY;
+        {
+          float x4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x4[c] = fmaxf(x4[c], __uint_as_float(sr[c][i]));
+          mx = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])) * sl2;
+        }
+        if (__any_sync(0xffffffffu, mx > m + 8.f)) {  // (also the first tile: m = -inf)
+          const float mn = fmaxf(m, mx);
+          const float sc = mn == -INFINITY ? 0.f : ex2_approx(m - mn);
+          const uint64_t sc2 = pack2(sc, sc);
+          if (j > 0) {  // S(j) is there, so PV(j - 1) is done and O can be rescaled
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+              tc::tmem_ld32(t_o + 32 * c, o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] *= sc;
+              tc::tmem_st32(t_o + 32 * c, o);
+            }
+          }
+          l2 = fma2(l2, sc2, 0);
+          m = mn;
+        }
+        const float ref = m == -INFINITY ? 0.f : -m;
+        const uint64_t ref2 = pack2(ref, ref), sl22 = pack2(sl2, sl2);
+        uint64_t la = 0, lb = 0;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pw[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const uint32_t* s = sr[2 * half + (i >> 4)] + 2 * (i & 15);
+            const float2 x = unpack2(fma2(pack2(__uint_as_float(s[0]), __uint_as_float(s[1])), sl22, ref2));
+            const float e0 = ex2_approx(x.x), e1 = ex2_approx(x.y);
+            if (i & 1) lb = add2(lb, pack2(e0, e1));
+            else la = add2(la, pack2(e0, e1));
+            pw[i] = Pair<T>::put(e0, e1);
+          }
+          tmem_st32_u(t_s + 32 * half, pw);
+        }
+        tmem_wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[t]);
+        l2 = add2(l2, add2(la, lb));
+      }
+      if (!ok) break;
+      v_it += 2 * n_all;
+      const float2 lf = unpack2(l2);
+      float l = lf.x + lf.y;
+      if (n > 0) {
+        if (!(ok = wait_warp(&sm.o_full[t], o_ph, &sm.err))) break;
+        o_ph ^= 1;
+        tc::fence_after_sync();
+      }
+      const bool bad = *reinterpret_cast<volatile int*>(&sm.piece[st].bad) != 0;
+      release();
+      // the four warps of the tile agree whether its rows are taken again key by key
+      if (slow) *reinterpret_cast<volatile int*>(&sm.odd[t]) = k + 1;
+      if (!(ok = tile_sync())) break;
+      slow = *reinterpret_cast<volatile int*>(&sm.odd[t]) == k + 1;
+      const int k_end = min(p.len, (p.k0 + n) * kKeys);
+      const bool live = row < rows_end;
+      const int token = row / g.group, head = p.hk * g.group + row - token * g.group;
+      T* out = static_cast<T*>(a.out) + (p.first + token) * a.out_stride[0] + head * a.out_stride[1];
+      constexpr int kPer = D / 32;
+      if (p.splits == 1) {
+        if (!slow) {
+          const float inv = bad ? NAN : lim < 0 ? 0.f : 1.f / l;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            if (n > 0) {
+              tc::tmem_ld32(t_o + 32 * c, o);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = 0.f;
+            }
+            if (live) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = lim < 0 && !bad ? 0.f : o[i] * inv;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(out + 32 * c)[i] = pack8<T>(o + 8 * i);
+            }
+          }
+        } else {
+          for (int rr = 0; rr < 32; ++rr) {
+            const int r2 = p.row0 + 128 * t + 32 * (warp & 3) + rr;
+            if (r2 >= rows_end) break;
+            float o[kPer], ms, ls;
+            slow_row<T, D, kPaged>(g, p, r2, k_end, o, &ms, &ls);
+            const int tok = r2 / g.group, hd = p.hk * g.group + r2 - tok * g.group;
+            const float inv = bad ? NAN : p.ctx + tok < 0 ? 0.f : 1.f / ls;
+            uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (p.first + tok) * a.out_stride[0] +
+                                                        hd * a.out_stride[1]) + lane * (kPer / 2);
+#pragma unroll
+            for (int i = 0; i < kPer / 2; ++i) dst[i] = Pair<T>::put(o[2 * i] * inv, o[2 * i + 1] * inv);
+          }
+        }
+      } else {
+        // one of several ranges of keys: leave it for whoever comes last
+        const int at = 128 * t + row_in;
+        const size_t slot = p.slot + p.split;
+        if (slot < static_cast<size_t>(g.slots)) {
+          float4* part = g.part + slot * (D / 4) * kRows;
+          if (bad) l = NAN;
+          if (!slow) {
+            if (n > 0) {
+#pragma unroll 1
+              for (int c = 0; c < D / 32; ++c) {
+                float o[32];
+                tc::tmem_ld32(t_o + 32 * c, o);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  part[(8 * c + i) * kRows + at] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+              }
+            }
+            g.stat[slot * kRows + at] = make_float2(m, l);
+          } else {
+            for (int rr = 0; rr < 32; ++rr) {
+              const int at2 = 128 * t + 32 * (warp & 3) + rr, r2 = p.row0 + at2;
+              if (r2 >= rows_end) break;
+              float o[kPer], ms, ls;
+              slow_row<T, D, kPaged>(g, p, r2, k_end, o, &ms, &ls);
+#pragma unroll
+              for (int i = 0; i < kPer; ++i) {
+                const int d = lane * kPer + i;
+                reinterpret_cast<float*>(part + (d / 4) * kRows + at2)[d % 4] = o[i];
+              }
+              if (lane == 0) g.stat[slot * kRows + at2] = make_float2(ms, bad ? NAN : ls);
+            }
+          }
+          __threadfence();
+          if (!(ok = tile_sync())) break;
+          if (threadIdx.x % 128 == 0)
+            *reinterpret_cast<volatile int*>(&sm.last[t]) =
+                atomicInc(g.counters + 2 * static_cast<size_t>(p.slot) + t, p.splits - 1) ==
+                static_cast<uint32_t>(p.splits - 1);
+          if (!(ok = tile_sync())) break;
+          if (*reinterpret_cast<volatile int*>(&sm.last[t]) != 0) {
+            __threadfence();
+            if (live) {
+              const float2* stat = g.stat + static_cast<size_t>(p.slot) * kRows + at;
+              float mm = -INFINITY, ll = 0.f;
+              for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, __ldcg(stat + s * kRows).x);
+              const float ref = mm == -INFINITY ? 0.f : mm;
+              for (int s = 0; s < p.splits; ++s) {
+                const float2 x = __ldcg(stat + s * kRows);
+                ll += x.y * ex2_approx(x.x - ref);
+              }
+              const float inv = lim < 0 ? 0.f : 1.f / ll;
+              const float4* part0 = g.part + static_cast<size_t>(p.slot) * (D / 4) * kRows + at;
+#pragma unroll 1
+              for (int c = 0; c < D / 8; ++c) {
+                float o[8] = {};
+                for (int s = 0; s < p.splits; ++s) {
+                  const float w = __ldcg(stat + s * kRows).x;
+                  if (w == -INFINITY) continue;  // that range holds no key this row sees
+                  const float f = ex2_approx(w - ref);
+                  const float4 x = __ldcg(part0 + (static_cast<size_t>(s) * (D / 4) + 2 * c) * kRows);
+                  const float4 y = __ldcg(part0 + (static_cast<size_t>(s) * (D / 4) + 2 * c + 1) * kRows);
+                  o[0] += f * x.x; o[1] += f * x.y; o[2] += f * x.z; o[3] += f * x.w;
+                  o[4] += f * y.x; o[5] += f * y.y; o[6] += f * y.z; o[7] += f * y.w;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] *= inv;
+                reinterpret_cast<uint4*>(out)[c] = pack8<T>(o);
+              }
+            }
+          }
+        }
+      }
+      tc::fence_before_sync();  // O has been read: the next piece's first PV may overwrite it
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (threadIdx.x == 0 && sm.err) report(a.status, MKB_SERVE_TIMEOUT);
+  if (warp == 8) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tbase, 512);
+  }
+}
+
+// ---- host side -----------------------------------------------------------------------
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encoder() {
+  static EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// Rows of 64 values (of D), `box` of them a copy; the dimensions after the row's are
+// `dims` with strides of `strides` elements. What lies outside reads as zeros.
+static cudaError_t map_rows(CUtensorMap* m, int dtype, const void* base, int D, int rank, const uint64_t* dims,
+                            const int64_t* strides, uint32_t box) {
+  const EncodeTiled enc = encoder();
+  if (!enc) return cudaErrorNotSupported;
+  cuuint64_t gd[4] = {static_cast<cuuint64_t>(D)}, gs[3];
+  cuuint32_t bx[4] = {64, box, 1, 1}, es[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    gd[i + 1] = dims[i] > 0 ? dims[i] : 1;
+    // a stride of 0 (one element, or the same place for all) is never stepped along
+    gs[i] = static_cast<cuuint64_t>(strides[i] > 0 ? strides[i] : D) * 2;
+    if (strides[i] == 0) gd[i + 1] = 1;
+  }
+  const CUresult r = enc(m, dtype == MKB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         rank + 1, const_cast<void*>(base), gd, gs, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+static int sm_count() {
+  static int n[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (n[dev] == 0 && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n[dev] = 0;
+  return n[dev] > 0 ? n[dev] : 148;
+}
+
+// Upper bound of the row blocks of a call, all KV heads.
+static int64_t tc_blocks(const mkb_attn_args& a) {
+  const int64_t rows = static_cast<int64_t>(a.tokens) * (a.heads / a.kv_heads);
+  return (rows / kRows + a.batch) * a.kv_heads;
+}
+// Partial results a call can leave. Rows are split only past a fair share C >= 5/4 U /
+// grid of the U key tiles, into at most 2 n / C pieces for n tiles; a request's blocks
+// grow linearly, so U counts at least half of n for each: at most 4 U / C < 4 grid.
+static int64_t tc_slots(const mkb_attn_args& a) { return 4 * static_cast<int64_t>(sm_count()); }
+
+size_t tc_workspace(const mkb_attn_args& a) {
+  const size_t slots = tc_slots(a);
+  return 256 + slots * 8 + slots * kRows * (static_cast<size_t>(a.head_dim) * 4 + 8) + 256;
+}
+
+template <typename T, int D, bool kPaged>
+static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
+  TcArgs g;
+  g.a = a;
+  g.sl2 = a.scale * 1.4426950408889634f;
+  g.group = a.heads / a.kv_heads;
+  g.k_head = a.k_stride[1] != 0;
+  g.v_head = a.v_stride[1] != 0;
+  g.box = kPaged ? (a.page_size < kKeys ? a.page_size : kKeys) : kKeys;
+  g.slots = static_cast<int>(tc_slots(a));
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  if (ws == nullptr) return cudaErrorInvalidValue;
+  const size_t cb = (static_cast<size_t>(g.slots) * 8 + 255) / 256 * 256;
+  g.counters = reinterpret_cast<uint32_t*>(ws);
+  g.stat = reinterpret_cast<float2*>(ws + cb);
+  g.part = reinterpret_cast<float4*>(ws + cb + static_cast<size_t>(g.slots) * kRows * 8);
+  CUtensorMap mk, mv;
+  cudaError_t e;
+  const void *kb = a.k, *vb = a.v;
+  if (kPaged && a.pages == 0) kb = vb = a.q;  // an empty pool is never read: any address will do
+  if (kPaged) {
+    const uint64_t dims[3] = {static_cast<uint64_t>(a.page_size), static_cast<uint64_t>(a.kv_heads),
+                              static_cast<uint64_t>(a.pages)};
+    const int64_t ks[3] = {a.k_stride[2], a.k_stride[1], a.k_stride[0]};
+    const int64_t vs[3] = {a.v_stride[2], a.v_stride[1], a.v_stride[0]};
+    if ((e = map_rows(&mk, a.dtype, kb, D, 3, dims, ks, g.box)) != cudaSuccess) return e;
+    if ((e = map_rows(&mv, a.dtype, vb, D, 3, dims, vs, g.box)) != cudaSuccess) return e;
+  } else {
+    const uint64_t dims[2] = {static_cast<uint64_t>(a.tokens), static_cast<uint64_t>(a.kv_heads)};
+    if ((e = map_rows(&mk, a.dtype, kb, D, 2, dims, a.k_stride, kKeys)) != cudaSuccess) return e;
+    if ((e = map_rows(&mv, a.dtype, vb, D, 2, dims, a.v_stride, kKeys)) != cudaSuccess) return e;
+  }
+  constexpr int bytes = sizeof(TcSmem<D>) + 1024;
+  static_assert(bytes <= 232448, "shared memory of the attention kernel");
+  static bool configured[64] = {false};
+  int dev = 0;
+  if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    e = cudaFuncSetAttribute(attn_tc_kernel<T, D, kPaged>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  // at least one row block a CTA, unless keys are split: then every SM may have a part
+  const int64_t blocks = tc_blocks(a) * (kPaged ? (static_cast<int64_t>(a.table_width) * a.page_size / kKeys) / kMinSplit + 1
+                                                : a.tokens / (kKeys * kMinSplit) + 1);
+  const int grid = static_cast<int>(blocks < sm_count() ? blocks : sm_count());
+  attn_tc_kernel<T, D, kPaged><<<grid, kTcThreads, bytes, stream>>>(mk, mv, g);
+  return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t tc_type(const mkb_attn_args& a, bool paged, cudaStream_t stream) {
+  if (a.head_dim == 128) return paged ? tc_launch<T, 128, true>(a, stream) : tc_launch<T, 128, false>(a, stream);
+  return paged ? tc_launch<T, 64, true>(a, stream) : tc_launch<T, 64, false>(a, stream);
+}
+
+cudaError_t attn_tc(const mkb_attn_args& a, bool paged, cudaStream_t stream) {
+  return a.dtype == MKB_BF16 ? tc_type<__nv_bfloat16>(a, paged, stream) : tc_type<__half>(a, paged, stream);
+}
+
+}  // namespace sv
+}  // namespace mkb
