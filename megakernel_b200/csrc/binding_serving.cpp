@@ -167,6 +167,10 @@ Tensor output_for(const OptTensor& out, const Tensor& q, c10::Device dev) {
 
 void set_query(mkb_attn_args& a, const Tensor& q, const Tensor& out, const Batch& b, std::optional<double> scale) {
   const int64_t d = q.dim();
+  for (int64_t i = 0; i + 1 < d; ++i) {
+    check_apart(q, "q", i);
+    check_apart(out, "out", i);
+  }
   a.heads = as_int(q.size(d - 2), "heads");
   a.head_dim = as_int(q.size(d - 1), "head_dim");
   TORCH_CHECK_VALUE(a.head_dim == 64 || a.head_dim == 128, "the head dimension must be 64 or 128, got ", a.head_dim);
@@ -189,6 +193,7 @@ void set_query(mkb_attn_args& a, const Tensor& q, const Tensor& out, const Batch
 void check_heads(int heads, int64_t kv_heads) {
   TORCH_CHECK_VALUE(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, heads, " query heads are no multiple of ",
                     kv_heads, " KV heads");
+  TORCH_CHECK_VALUE(heads / kv_heads <= 128, "at most 128 query heads may share a KV head, got ", heads / kv_heads);
 }
 
 struct Paging {

@@ -139,7 +139,9 @@ static cudaError_t check_attn(const mkb_attn_args* a, bool paged) {
   if (a->tokens == 0) return cudaSuccess;
   if (a->cu_q == nullptr && (a->q_len < 1 || (int64_t)a->q_len * a->batch != a->tokens)) return cudaErrorInvalidValue;
   if (!a->q || !a->out) return cudaErrorInvalidValue;
-  if (static_cast<int64_t>(a->tokens) * (a->heads / a->kv_heads) > 0x7fff0000) return cudaErrorInvalidValue;
+  // rows of a KV head, and their blocks over all of them, are counted in 32 bits
+  if (a->heads / a->kv_heads > 128 || static_cast<int64_t>(a->tokens) + a->batch > (1ll << 30) / a->heads)
+    return cudaErrorInvalidValue;
   if (paged) {
     if (!a->kv_lens || a->table_width < 0 || a->pages < 0) return cudaErrorInvalidValue;
     if (a->table_width > 0 && !a->block_table) return cudaErrorInvalidValue;
@@ -152,7 +154,9 @@ static cudaError_t check_attn(const mkb_attn_args* a, bool paged) {
       !strides_ok(a->q_stride, 2) || !strides_ok(a->out_stride, 2) || !strides_ok(a->k_stride, paged ? 3 : 2) ||
       !strides_ok(a->v_stride, paged ? 3 : 2))
     return cudaErrorMisalignedAddress;
-  // keys (and pages) lie at places of their own; KV heads may share one
+  // rows lie at places of their own; KV heads may share one
+  if ((a->tokens > 1 && (!a->q_stride[0] || !a->out_stride[0])) || (a->heads > 1 && (!a->q_stride[1] || !a->out_stride[1])))
+    return cudaErrorInvalidValue;
   if (paged ? a->pages > 0 && ((a->pages > 1 && (!a->k_stride[0] || !a->v_stride[0])) || !a->k_stride[2] || !a->v_stride[2])
             : a->tokens > 1 && (!a->k_stride[0] || !a->v_stride[0]))
     return cudaErrorInvalidValue;

@@ -3,13 +3,13 @@
 //
 //   out_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = 2^(c q_i.k_j - m_i),  c = scale log2(e),  j <= pos(i)
 //
-// A KV head's queries are rows: row r of a request is token r / G, query head r % G of
-// the G that share the KV head, so that one pass over the keys serves all of them. A CTA
-// takes 256 rows (tiles A and B of 128) of one request and KV head and walks its keys
-// 128 at a time:
+// A KV head's queries are rows: row r of a tile is token r / G, query head r % G of the
+// G that share the KV head, so that one pass over the keys serves all of them; a tile
+// holds the 128 / G tokens that fill (nearly) 128 rows. A CTA takes two tiles (A and B)
+// of one request and KV head and walks its keys 128 at a time:
 //
-//   warp 9      which piece of work comes next, and its K and V tiles by TMA into a ring
-//               (128-byte swizzle; pages are boxes of page_size rows)
+//   warp 9      which piece of work comes next; its Q, K and V tiles by TMA (128-byte
+//               swizzle; K and V through a ring, pages are boxes of page_size rows)
 //   warp 8      tcgen05.mma: S = Q K^T (Q and K in shared memory), O += P V with P from
 //               tensor memory and V as it lies, keys by dims (an MN-major operand: no
 //               transposed copy of V is made)
@@ -22,16 +22,16 @@
 // moves P stays below 2^8, which FP32 sums and 16-bit P hold without loss. P is rounded
 // to the operands' 16-bit type, as the output is: the same relative error.
 //
-// Work: a piece is (request, KV head, 256 rows, a range of key tiles). Every CTA works
+// Work: a piece is (request, KV head, two tiles, a range of key tiles). Every CTA works
 // the list out for itself from the lengths, longest pieces first, and takes every
 // grid-th one, turning round after each sweep. Rows whose keys are more than a fair
 // share are split over several pieces; each writes its O, maximum and sum, and the last
 // to arrive adds them up in order of their keys, so results do not depend on timing.
 //
 // Masked places: scores are replaced, not added to. V rows past the request's last key
-// are cleared in shared memory. A tile that is partly masked for some row is scanned for
-// V that is not finite (0 * inf would reach rows that do not see it); where one is found,
-// those rows are computed again key by key.
+// are cleared in shared memory. V that is not finite and stands where some row of the
+// tile does not look reaches that row as 0 * inf = NaN: a row whose O is not finite is
+// computed again key by key, over the keys it sees.
 
 #include <cmath>
 #include <cuda.h>
@@ -43,17 +43,17 @@ namespace mkb {
 namespace sv {
 
 constexpr int kTcThreads = 320;
-constexpr int kRows = 256, kKeys = 128;   // rows of a piece, keys of a tile
+constexpr int kRows = 256, kKeys = 128;   // rows of a piece (two tiles), keys of a tile
 constexpr int kHalf = 128 * 128;          // 16 KB: 128 rows x 64 values, 128-byte swizzle
 constexpr int kMinSplit = 6;              // key tiles below which rows are not split
 constexpr int kSortBatch = 128;           // requests up to which pieces are taken longest first
-constexpr unsigned long long kTimeoutNs = 1000000000ull;
+constexpr int kTryNs = 20000, kTries = 50000;  // bound of every wait: about a second
 
 struct Piece {
   int b;            // request, -1: no more work
   int hk;
-  int first, q;     // the request's packed rows
-  int row0, rows;   // flattened rows (token * G + head)
+  int first;        // the request's first packed token
+  int tok0, toks;   // the piece's tokens
   int ctx, len;     // keys before the new tokens, all keys
   int k0;           // first key tile
   int n[2];         // key tiles of tiles A and B
@@ -64,17 +64,17 @@ struct Piece {
 template <int D>
 struct TcSmem {
   static constexpr int kTileBytes = D * 256;            // 128 keys
-  static constexpr int kSlots = D == 128 ? 5 : 8;
+  static constexpr int kSlots = D == 128 ? 4 : 8;
   uint8_t q[2][kTileBytes];
   uint8_t kv[kSlots][kTileBytes];
+  uint8_t stage[8][32 * 128];                           // a warp's 32 rows x 64 values on their way out
   uint64_t kv_full[kSlots], kv_empty[kSlots];
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
   uint64_t info_full[2], info_empty[2];
   uint64_t tile_bar[2];   // the four softmax warps of a tile
   Piece piece[2];
   uint32_t tmem_base;
   int err;
-  int odd[2];             // the last piece (+ 1) whose masked tiles held V that is not finite
   int last[2];
 };
 
@@ -82,6 +82,8 @@ struct TcArgs {
   mkb_attn_args a;
   float sl2;            // scale * log2(e)
   int group;            // query heads of a KV head
+  int tile_tokens;      // tokens of a tile: 128 / group
+  int group_mul;        // r / group = r * group_mul >> 16 for r < 128
   int k_head, v_head;   // 0 where every KV head lies at the same place (stride 0), else 1
   int box;              // keys of a TMA box
   int slots;            // partial results the workspace holds
@@ -90,12 +92,12 @@ struct TcArgs {
   float2* stat;         // [slots][256]: maximum, sum
 };
 
+// Bounded: each try suspends for 20 us at most. (Counted, not timed: reading the global
+// timer before the first try costs more than most waits last.)
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t ph, int* err) {
-  if (mbar_test(bar, ph)) return true;
-  const uint64_t t0 = global_ns();
-  while (!mbar_wait(bar, ph, 20000)) {
+  for (int i = 0; !mbar_wait(bar, ph, kTryNs); ++i) {
     if (*reinterpret_cast<volatile int*>(err) != 0) return false;
-    if (global_ns() - t0 > kTimeoutNs) {
+    if (i == kTries) {
       *reinterpret_cast<volatile int*>(err) = 1;
       return false;
     }
@@ -199,36 +201,33 @@ __device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
   l.len = kPaged ? max(__ldg(g.a.kv_lens + b), 0) : rq.n;
   l.bad = kPaged && static_cast<int64_t>(l.len) > static_cast<int64_t>(g.a.table_width) * g.a.page_size;
   l.ctx = l.len - l.q;
-  l.blocks = static_cast<int>((static_cast<int64_t>(l.q) * g.group + kRows - 1) / kRows);
-  l.tiles = l.bad || l.blocks == 0 ? 0 : (l.len + kKeys - 1) / kKeys;
+  const unsigned span = 2 * g.tile_tokens;
+  l.blocks = static_cast<int>((static_cast<unsigned>(l.q) + span - 1) / span);
+  l.tiles = l.bad || l.blocks == 0 ? 0 : static_cast<int>((static_cast<unsigned>(l.len) + kKeys - 1) / kKeys);
   l.splits = 1;
   return l;
 }
-// key tiles of row block i: up to its last token's position
-__device__ __forceinline__ int block_tiles(const Load& l, int group, int i) {
-  const int64_t last = min(static_cast<int64_t>(l.q), ((static_cast<int64_t>(i) + 1) * kRows - 1) / group + 1) - 1;
-  const int64_t keys = l.ctx + last + 1;
-  return l.bad || keys <= 0 ? 0 : static_cast<int>((keys + kKeys - 1) / kKeys);
+// key tiles that the first `toks` tokens of the request see
+__device__ __forceinline__ int tiles_of(const Load& l, int toks) {
+  const int keys = l.ctx + min(toks, l.q);
+  return l.bad || keys <= 0 ? 0 : static_cast<int>((static_cast<unsigned>(keys) + kKeys - 1) / kKeys);
 }
-// how many of the request's row blocks have more than x key tiles (they come last)
-__device__ __forceinline__ int blocks_above(const Load& l, int group, int64_t x) {
+// how many of the request's blocks of `span` tokens see more than x key tiles (they come last)
+__device__ __forceinline__ int blocks_above(const Load& l, int span, int x) {
   if (x < 0) return l.blocks;
   if (l.tiles <= x) return 0;
-  const int64_t y = x * kKeys - l.ctx;  // the first token that sees more than x tiles
-  if (y <= 0) return l.blocks;
-  const int64_t i = y * group / kRows;
-  return i >= l.blocks ? 0 : l.blocks - static_cast<int>(i);
+  const int y = x * kKeys - l.ctx;  // the first token that sees more (x < tiles: no overflow)
+  return y <= 0 ? l.blocks : l.blocks - static_cast<int>(static_cast<unsigned>(y) / static_cast<unsigned>(span));
 }
 
 // ---- one row, key by key: what a tile with values that are not finite comes to --------
 // Warp-wide; lane holds dims [lane * D / 32, + D / 32) of O, relative to maximum m.
 template <typename T, int D, bool kPaged>
-__device__ __noinline__ void slow_row(const TcArgs& g, const Piece& p, int row, int k_end, float* o, float* m_out,
-                                      float* l_out) {
+__device__ __noinline__ void slow_row(const TcArgs& g, const Piece& p, int token, int h, int k_end, float* o,
+                                      float* m_out, float* l_out) {
   const mkb_attn_args& a = g.a;
   const int lane = threadIdx.x & 31;
   constexpr int kPer = D / 32;
-  const int token = row / g.group, h = p.hk * g.group + row % g.group;
   const T* q = static_cast<const T*>(a.q) + (p.first + token) * a.q_stride[0] + h * a.q_stride[1];
   const int keys = min(k_end, p.ctx + token + 1);
   float m = -INFINITY, l = 0.f;
@@ -275,7 +274,7 @@ __device__ __noinline__ void slow_row(const TcArgs& g, const Piece& p, int row, 
 template <typename T, int D, bool kPaged>
 __global__ void __launch_bounds__(kTcThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                   const __grid_constant__ TcArgs g) {
+                   const __grid_constant__ CUtensorMap tq, const __grid_constant__ TcArgs g) {
   using Smem = TcSmem<D>;
   constexpr int kSlots = Smem::kSlots, kTileBytes = Smem::kTileBytes;
   extern __shared__ uint8_t smem_raw[];
@@ -288,7 +287,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&sm.kv_empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&sm.q_full[t], 4);
+      mbar_init(&sm.q_full[t], 1);
+      mbar_init(&sm.q_empty[t], 1);
       mbar_init(&sm.s_full[t], 1);
       mbar_init(&sm.p_full[t], 4);
       mbar_init(&sm.o_full[t], 1);
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&sm.tile_bar[t], 4);
       mbar_init(&sm.info_empty[t], 9);  // eight softmax warps and the MMA warp
     }
-    sm.err = sm.odd[0] = sm.odd[1] = 0;
+    sm.err = 0;
     fence_mbar_init();
   }
   if (warp == 8) {
@@ -313,41 +313,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (lane == 0) {
       tc::prefetch_tensormap(&tk);
       tc::prefetch_tensormap(&tv);
+      tc::prefetch_tensormap(&tq);
     }
-    const int kv_heads = a.kv_heads, grid = gridDim.x;
+    const int kv_heads = a.kv_heads, grid = gridDim.x, span = 2 * g.tile_tokens;
+    // a lane keeps its first request; the others are read again in every pass
+    const Load mine = lane < a.batch ? load_of<kPaged>(g, lane) : Load{};
+    auto request = [&](int b) { return b < 32 ? mine : load_of<kPaged>(g, b); };
     // a fair share of the key tiles; rows with more are split
     long long total = 0;
     int top = 0;
     for (int b = lane; b < a.batch; b += 32) {
-      const Load l = load_of<kPaged>(g, b);
-      if (l.blocks == 0) continue;
-      total += static_cast<long long>(block_tiles(l, g.group, 0) + l.tiles) * l.blocks;  // twice the sum: linear in i
+      const Load l = request(b);
+      total += static_cast<long long>(tiles_of(l, span) + l.tiles) * l.blocks;  // twice the sum: linear in the block
       top = max(top, l.tiles);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     top = __reduce_max_sync(0xffffffffu, top);
-    total = total * kv_heads / 2;
-    const int share = static_cast<int>(min(total * 5 / (4 * grid) + 1, 0x7fffffffll));
-    const int cap = max(kMinSplit, share);
-    auto with_splits = [&](int b) {
-      Load l = load_of<kPaged>(g, b);
-      l.splits = l.tiles > cap ? (l.tiles + cap - 1) / cap : 1;
-      return l;
-    };
+    const float share = static_cast<float>(total) * kv_heads * (0.5f * 1.25f) / grid;
+    const int cap = max(kMinSplit, static_cast<int>(fminf(share, 1e9f)) + 1);
+    auto splits_of = [&](const Load& l) { return l.tiles > cap ? (l.tiles + cap - 1) / cap : 1; };
     // pieces of more than x tiles, all requests
     auto pieces_above = [&](int x) {
-      long long n = 0;
+      int n = 0;
       for (int b = lane; b < a.batch; b += 32) {
-        const Load l = with_splits(b);
-        n += static_cast<long long>(blocks_above(l, g.group, static_cast<int64_t>(x) * l.splits)) * l.splits;
+        const Load l = request(b);
+        const int sp = splits_of(l);
+        n += blocks_above(l, span, x * sp) * sp;
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-      return n * kv_heads;
+      return __reduce_add_sync(0xffffffffu, n) * kv_heads;
     };
-    const bool sorted = a.batch <= kSortBatch && a.batch > 0;
-    int it = 0, k = 0;
+    // longest first, unless every piece has a CTA of its own (or the list is long: even anyway)
+    const bool sorted = a.batch <= kSortBatch && pieces_above(-1) > grid;
+    int it = 0, k = 0, q_uses[2] = {0, 0};
     bool ok = true;
     for (; ok; ++k) {
       const int st = k & 1;
@@ -372,10 +370,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         Load l = {};
         int above = 0, here = 0, slots = 0;
         if (b < a.batch) {
-          l = with_splits(b);
+          l = request(b);
+          l.splits = splits_of(l);
           if (sorted) {
-            above = blocks_above(l, g.group, static_cast<int64_t>(lo) * l.splits);
-            here = blocks_above(l, g.group, static_cast<int64_t>(lo) * l.splits - l.splits) - above;
+            above = blocks_above(l, span, lo * l.splits);
+            here = blocks_above(l, span, lo * l.splits - l.splits) - above;
           } else {
             here = l.blocks;
           }
@@ -391,34 +390,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             sinc += y;
           }
         }
-        const bool mine = r >= inc - here && r < inc;
-        const uint32_t who = __ballot_sync(0xffffffffu, mine);
+        const bool is_it = r >= inc - here && r < inc;
+        const uint32_t who = __ballot_sync(0xffffffffu, is_it);
         if (who != 0) {
-          if (mine) {
-            int at = static_cast<int>(r) - (inc - here);
+          if (is_it) {
+            unsigned at = static_cast<unsigned>(r) - (inc - here);
             p.b = b;
-            p.split = at % l.splits;
-            at /= l.splits;
-            p.hk = at % kv_heads;
-            const int i = l.blocks - 1 - above - at / kv_heads;  // longest first
+            p.split = at % static_cast<unsigned>(l.splits);
+            at /= static_cast<unsigned>(l.splits);
+            p.hk = at % static_cast<unsigned>(kv_heads);
+            const int i = l.blocks - 1 - above - static_cast<int>(at / static_cast<unsigned>(kv_heads));  // longest first
             p.first = l.first;
-            p.q = l.q;
             p.len = l.len;
             p.ctx = l.ctx;
-            p.row0 = i * kRows;
-            p.rows = static_cast<int>(min(static_cast<int64_t>(l.q) * g.group - p.row0, static_cast<int64_t>(kRows)));
-            const int n = block_tiles(l, g.group, i), per = (n + l.splits - 1) / l.splits;
+            p.tok0 = i * span;
+            p.toks = min(l.q - p.tok0, span);
+            const int n = tiles_of(l, p.tok0 + p.toks), per = (n + l.splits - 1) / l.splits;
             p.k0 = min(p.split * per, n);
             const int k1 = min(p.k0 + per, n);
             p.splits = l.splits;
             p.slot = slot_base + sinc - slots + (i * kv_heads + p.hk) * l.splits;
             p.bad = l.bad;
-            for (int t = 0; t < 2; ++t) {  // up to the tile's last row's position
-              const int last = min(p.rows, 128 * (t + 1)) - 1;
-              const int keys = p.ctx + (p.row0 + last) / g.group + 1;
-              const int end = keys <= 0 || p.bad ? 0 : (keys + kKeys - 1) / kKeys;
-              p.n[t] = p.rows > 128 * t ? max(min(end, k1) - p.k0, 0) : 0;
-            }
+            p.n[0] = max(min(tiles_of(l, p.tok0 + min(p.toks, g.tile_tokens)), k1) - p.k0, 0);
+            p.n[1] = p.toks > g.tile_tokens ? k1 - p.k0 : 0;
             if (l.bad) report(a.status, MKB_SERVE_BAD_LENGTH);
           }
           const int src = __ffs(who) - 1;
@@ -473,6 +467,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       };
       const int kh = p.hk * g.k_head, vh = p.hk * g.v_head;
       if (n > 0) ok = load(&tk, kh, 0);
+      for (int t = 0; t < 2 && ok; ++t) {  // Q once the last product of the tile's previous one has read it
+        if (p.n[t] == 0) continue;
+        if (q_uses[t] > 0 && !(ok = wait_warp(&sm.q_empty[t], (q_uses[t] - 1) & 1, &sm.err))) break;
+        ++q_uses[t];
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sm.q_full[t], g.tile_tokens * g.group * D * 2);
+#pragma unroll
+          for (int d = 0; d < D / 64; ++d)
+            tma_3d(sm.q[t] + d * kHalf, &tq, 64 * d, p.hk * g.group, p.first + p.tok0 + t * g.tile_tokens, &sm.q_full[t]);
+        }
+        __syncwarp();
+      }
       for (int j = 0; j < n && ok; ++j) {
         if (j + 1 < n) ok = load(&tk, kh, j + 1);
         if (ok) ok = load(&tv, vh, j);
@@ -480,9 +486,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     // after a stop, wait (bounded) for the copies still in flight before leaving
     if (sm.err) {
-      const uint64_t t0 = global_ns();
+      int tries = 0;
       for (int i = max(it - kSlots, 0); i < it; ++i)
-        while (!mbar_wait(&sm.kv_full[i % kSlots], (i / kSlots) & 1, 20000) && global_ns() - t0 < kTimeoutNs) {
+        while (!mbar_wait(&sm.kv_full[i % kSlots], (i / kSlots) & 1, kTryNs) && ++tries < kTries) {
+        }
+      for (int t = 0; t < 2; ++t)
+        while (q_uses[t] > 0 && !mbar_wait(&sm.q_full[t], (q_uses[t] - 1) & 1, kTryNs) && ++tries < kTries) {
         }
     }
   } else if (warp == 8) {
@@ -521,6 +530,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc::mma_bf16_ss(tbase + 128 * t, tc::desc_advance(dq, off), tc::desc_advance(dk, off), id_s, kk != 0);
           }
           tc::commit(&sm.s_full[t]);
+          if (j + 1 == nt[t]) tc::commit(&sm.q_empty[t]);
         }
         __syncwarp();
         return true;
@@ -579,7 +589,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t t_s = tbase + lanes + 128 * t, t_o = tbase + lanes + 256 + 128 * t;
     const float sl2 = g.sl2;
     uint32_t s_ph = 0, o_ph = 0;
-    int v_it = 0;                            // ring slots of earlier pieces
+    const int tok_in = row_in * g.group_mul >> 16, head_in = row_in - tok_in * g.group;
     bool ok = true;
     uint32_t t_ph = 0;
     auto tile_sync = [&]() -> bool {         // a barrier of the tile's warps, bounded like every wait
@@ -593,42 +603,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int st = k & 1;
       if (!wait_warp(&sm.info_full[st], (k >> 1) & 1, &sm.err)) break;
       const Piece p = sm.piece[st];
-      const int n_all = max(p.n[0], p.n[1]);
       auto release = [&]() {
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.info_empty[st]);
       };
-      if (p.b < 0 || p.rows <= 128 * t) {
+      if (p.b < 0 || p.toks <= g.tile_tokens * t) {
         release();
         if (p.b < 0) break;
-        v_it += 2 * n_all;
         continue;
       }
       const int n = p.n[t];
-      const int row = p.row0 + 128 * t + row_in;     // of the request
-      const int rows_end = p.row0 + p.rows;
-      if (n > 0) {
-        // Q rows into the swizzled layout; rows past the request's are zeros
-        constexpr int kChunks = D / 8;               // 16-byte chunks of a row
-        for (int c = threadIdx.x & 127; c < 128 * kChunks; c += 128) {
-          const int r = c / kChunks, x = c % kChunks, rr = p.row0 + 128 * t + r;
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (rr < rows_end) {
-            const int token = rr / g.group, h = p.hk * g.group + rr - token * g.group;
-            u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (p.first + token) * a.q_stride[0] +
-                                                     h * a.q_stride[1]) + x);
-          }
-          *reinterpret_cast<uint4*>(sm.q[t] + (x >> 3) * kHalf + r * 128 + (((x & 7) ^ (r & 7)) << 4)) = u;
-        }
-        fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.q_full[t]);
-      }
-      const int lim = p.ctx + min(row, rows_end - 1) / g.group;      // this row's last key
-      const int lim0 = p.ctx + (p.row0 + 128 * t) / g.group;         // the tile's least
+      const int tok_t = p.tok0 + g.tile_tokens * t;                  // the tile's first token
+      const bool live = row_in < g.tile_tokens * g.group && tok_t + tok_in < p.tok0 + p.toks;
+      const int lim0 = p.ctx + tok_t;                                // the last key its first row sees
+      const int lim = lim0 + tok_in;                                 // ... and this row
       float m = -INFINITY;                                           // in units of log2
       uint64_t l2 = 0;                                               // two partial sums
-      bool slow = false;
       for (int j = 0; j < n; ++j) {
         if (!(ok = wait_warp(&sm.s_full[t], s_ph, &sm.err))) break;
         s_ph ^= 1;
@@ -645,23 +635,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int i = 0; i < 128; ++i)
             if (key0 + i > lim) sr[i >> 5][i & 31] = 0xff800000u;
-          // V that is not finite would reach the rows that do not see it
-          const int i = v_it + (j + 1 < n_all ? 2 * j + 2 : 2 * n_all - 1), s = i % kSlots;
-          if (!(ok = wait_warp(&sm.kv_full[s], (i / kSlots) & 1, &sm.err))) break;
-          bool odd = false;
-          if (key0 + row_in < p.len) {
-            constexpr uint32_t e = Pair<T>::kDtype == MKB_BF16 ? 0x7f807f80u : 0x7c007c00u;
-            constexpr uint32_t el = e & 0xffffu, eh = e & 0xffff0000u;
-#pragma unroll 4
-            for (int c = 0; c < D / 8; ++c) {
-              const uint4 u = *reinterpret_cast<const uint4*>(sm.kv[s] + (c >> 3) * kHalf + row_in * 128 +
-                                                              (((c & 7) ^ (row_in & 7)) << 4));
-              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-              for (int q = 0; q < 4; ++q) odd |= (w[q] & el) == el || (w[q] & eh) == eh;
-            }
-          }
-          slow |= odd;
         }
         float mx = -INFINITY;
         {
@@ -670,7 +643,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int i = 0; i < 32; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) x4[c] = fmaxf(x4[c], __uint_as_float(sr[c][i]));
-          mx = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])) * sl2;
+          mx = live ? fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])) * sl2 : -INFINITY;
         }
         if (__any_sync(0xffffffffu, mx > m + 8.f)) {  // (also the first tile: m = -inf)
           const float mn = fmaxf(m, mx);
@@ -713,7 +686,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         l2 = add2(l2, add2(la, lb));
       }
       if (!ok) break;
-      v_it += 2 * n_all;
       const float2 lf = unpack2(l2);
       float l = lf.x + lf.y;
       if (n > 0) {
@@ -723,118 +695,134 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       const bool bad = *reinterpret_cast<volatile int*>(&sm.piece[st].bad) != 0;
       release();
-      // the four warps of the tile agree whether its rows are taken again key by key
-      if (slow) *reinterpret_cast<volatile int*>(&sm.odd[t]) = k + 1;
-      if (!(ok = tile_sync())) break;
-      slow = *reinterpret_cast<volatile int*>(&sm.odd[t]) == k + 1;
       const int k_end = min(p.len, (p.k0 + n) * kKeys);
-      const bool live = row < rows_end;
-      const int token = row / g.group, head = p.hk * g.group + row - token * g.group;
-      T* out = static_cast<T*>(a.out) + (p.first + token) * a.out_stride[0] + head * a.out_stride[1];
       constexpr int kPer = D / 32;
-      if (p.splits == 1) {
-        if (!slow) {
-          const float inv = bad ? NAN : lim < 0 ? 0.f : 1.f / l;
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            float o[32];
-            if (n > 0) {
-              tc::tmem_ld32(t_o + 32 * c, o);
-            } else {
+      uint8_t* stage = sm.stage[warp];
+      // 64 values of every row of the warp to memory, 128 bytes of four rows at a time
+      auto emit = [&](int half, const float* o) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = 0.f;
-            }
-            if (live) {
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = pack8<T>(o + 8 * c);
+        __syncwarp();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = lim < 0 && !bad ? 0.f : o[i] * inv;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(out + 32 * c)[i] = pack8<T>(o + 8 * i);
-            }
-          }
-        } else {
-          for (int rr = 0; rr < 32; ++rr) {
-            const int r2 = p.row0 + 128 * t + 32 * (warp & 3) + rr;
-            if (r2 >= rows_end) break;
-            float o[kPer], ms, ls;
-            slow_row<T, D, kPaged>(g, p, r2, k_end, o, &ms, &ls);
-            const int tok = r2 / g.group, hd = p.hk * g.group + r2 - tok * g.group;
-            const float inv = bad ? NAN : p.ctx + tok < 0 ? 0.f : 1.f / ls;
-            uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (p.first + tok) * a.out_stride[0] +
-                                                        hd * a.out_stride[1]) + lane * (kPer / 2);
-#pragma unroll
-            for (int i = 0; i < kPer / 2; ++i) dst[i] = Pair<T>::put(o[2 * i] * inv, o[2 * i + 1] * inv);
-          }
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + (lane >> 3), rt = 32 * (warp & 3) + r;
+          const int tok = rt * g.group_mul >> 16, head = p.hk * g.group + rt - tok * g.group;
+          if (rt < g.tile_tokens * g.group && tok_t + tok < p.tok0 + p.toks)
+            *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (p.first + tok_t + tok) * a.out_stride[0] +
+                                      head * a.out_stride[1] + 64 * half + 8 * (lane & 7)) =
+                *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
         }
-      } else {
+        __syncwarp();
+      };
+      // the rows of the warp whose O is not finite, key by key
+      auto again = [&](bool odd, auto&& put) {
+        uint32_t todo = __ballot_sync(0xffffffffu, odd && live);
+        while (todo != 0) {
+          const int r = __ffs(todo) - 1, rt = 32 * (warp & 3) + r;
+          todo &= todo - 1;
+          const int tok = tok_t + (rt * g.group_mul >> 16), head = p.hk * g.group + rt - (rt * g.group_mul >> 16) * g.group;
+          float o[kPer], ms, ls;
+          slow_row<T, D, kPaged>(g, p, tok, head, k_end, o, &ms, &ls);
+          put(rt, tok, head, o, ms, ls);
+        }
+        __syncwarp();
+      };
+      float odd = 0.f;  // NaN once a value of O is not finite
+      if (p.splits == 1) {
+        const float inv = bad ? NAN : lim < 0 ? 0.f : 1.f / l;
+#pragma unroll 1
+        for (int c = 0; c < D / 64; ++c) {
+          float o[64];
+          if (n > 0) {
+            tc::tmem_ld32(t_o + 64 * c, o);
+            tc::tmem_ld32(t_o + 64 * c + 32, o + 32);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) o[i] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            odd = fmaf(o[i], 0.f, odd);
+            o[i] = lim < 0 && !bad ? 0.f : o[i] * inv;
+          }
+          emit(c, o);
+        }
+        again(odd != 0.f && lim >= 0 && !bad, [&](int, int tok, int head, const float* o, float, float ls) {
+          uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (p.first + tok) * a.out_stride[0] +
+                                                      head * a.out_stride[1]) + lane * (kPer / 2);
+          const float f = 1.f / ls;
+#pragma unroll
+          for (int i = 0; i < kPer / 2; ++i) dst[i] = Pair<T>::put(o[2 * i] * f, o[2 * i + 1] * f);
+        });
+      } else if (static_cast<size_t>(p.slot) + p.splits <= static_cast<size_t>(g.slots)) {
         // one of several ranges of keys: leave it for whoever comes last
         const int at = 128 * t + row_in;
         const size_t slot = p.slot + p.split;
-        if (slot < static_cast<size_t>(g.slots)) {
-          float4* part = g.part + slot * (D / 4) * kRows;
-          if (bad) l = NAN;
-          if (!slow) {
-            if (n > 0) {
+        float4* part = g.part + slot * (D / 4) * kRows;
+        if (n > 0) {
 #pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
-                float o[32];
-                tc::tmem_ld32(t_o + 32 * c, o);
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            tc::tmem_ld32(t_o + 32 * c, o);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  part[(8 * c + i) * kRows + at] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-              }
-            }
-            g.stat[slot * kRows + at] = make_float2(m, l);
-          } else {
-            for (int rr = 0; rr < 32; ++rr) {
-              const int at2 = 128 * t + 32 * (warp & 3) + rr, r2 = p.row0 + at2;
-              if (r2 >= rows_end) break;
-              float o[kPer], ms, ls;
-              slow_row<T, D, kPaged>(g, p, r2, k_end, o, &ms, &ls);
+            for (int i = 0; i < 32; ++i) odd = fmaf(o[i], 0.f, odd);
 #pragma unroll
-              for (int i = 0; i < kPer; ++i) {
-                const int d = lane * kPer + i;
-                reinterpret_cast<float*>(part + (d / 4) * kRows + at2)[d % 4] = o[i];
-              }
-              if (lane == 0) g.stat[slot * kRows + at2] = make_float2(ms, bad ? NAN : ls);
-            }
+            for (int i = 0; i < 8; ++i)
+              part[(8 * c + i) * kRows + at] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
-          __threadfence();
-          if (!(ok = tile_sync())) break;
-          if (threadIdx.x % 128 == 0)
-            *reinterpret_cast<volatile int*>(&sm.last[t]) =
-                atomicInc(g.counters + 2 * static_cast<size_t>(p.slot) + t, p.splits - 1) ==
-                static_cast<uint32_t>(p.splits - 1);
-          if (!(ok = tile_sync())) break;
-          if (*reinterpret_cast<volatile int*>(&sm.last[t]) != 0) {
-            __threadfence();
-            if (live) {
-              const float2* stat = g.stat + static_cast<size_t>(p.slot) * kRows + at;
-              float mm = -INFINITY, ll = 0.f;
-              for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, __ldcg(stat + s * kRows).x);
-              const float ref = mm == -INFINITY ? 0.f : mm;
-              for (int s = 0; s < p.splits; ++s) {
-                const float2 x = __ldcg(stat + s * kRows);
-                ll += x.y * ex2_approx(x.x - ref);
-              }
-              const float inv = lim < 0 ? 0.f : 1.f / ll;
-              const float4* part0 = g.part + static_cast<size_t>(p.slot) * (D / 4) * kRows + at;
-#pragma unroll 1
-              for (int c = 0; c < D / 8; ++c) {
-                float o[8] = {};
-                for (int s = 0; s < p.splits; ++s) {
-                  const float w = __ldcg(stat + s * kRows).x;
-                  if (w == -INFINITY) continue;  // that range holds no key this row sees
-                  const float f = ex2_approx(w - ref);
-                  const float4 x = __ldcg(part0 + (static_cast<size_t>(s) * (D / 4) + 2 * c) * kRows);
-                  const float4 y = __ldcg(part0 + (static_cast<size_t>(s) * (D / 4) + 2 * c + 1) * kRows);
-                  o[0] += f * x.x; o[1] += f * x.y; o[2] += f * x.z; o[3] += f * x.w;
-                  o[4] += f * y.x; o[5] += f * y.y; o[6] += f * y.z; o[7] += f * y.w;
-                }
+        }
+        g.stat[slot * kRows + at] = make_float2(m, bad ? NAN : l);
+        __syncwarp();
+        again(odd != 0.f && lim >= 0 && !bad, [&](int rt, int, int, const float* o, float ms, float ls) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] *= inv;
-                reinterpret_cast<uint4*>(out)[c] = pack8<T>(o);
+          for (int i = 0; i < kPer; ++i) {
+            const int d = lane * kPer + i;
+            reinterpret_cast<float*>(part + (d / 4) * kRows + 128 * t + rt)[d % 4] = o[i];
+          }
+          if (lane == 0) g.stat[slot * kRows + 128 * t + rt] = make_float2(ms, ls);
+        });
+        __threadfence();
+        if (!(ok = tile_sync())) break;
+        if (threadIdx.x % 128 == 0)
+          *reinterpret_cast<volatile int*>(&sm.last[t]) =
+              atomicInc(g.counters + 2 * static_cast<size_t>(p.slot) + t, p.splits - 1) ==
+              static_cast<uint32_t>(p.splits - 1);
+        if (!(ok = tile_sync())) break;
+        if (*reinterpret_cast<volatile int*>(&sm.last[t]) != 0) {
+          __threadfence();
+          const float2* stat = g.stat + static_cast<size_t>(p.slot) * kRows + at;
+          float mm = -INFINITY, ll = 0.f;
+          for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, __ldcg(stat + s * kRows).x);
+          const float ref = mm == -INFINITY ? 0.f : mm;
+          for (int s = 0; s < p.splits; ++s) {
+            const float2 x = __ldcg(stat + s * kRows);
+            ll += x.y * ex2_approx(x.x - ref);
+          }
+          const float inv = lim < 0 ? 0.f : 1.f / ll;
+          const float4* part0 = g.part + static_cast<size_t>(p.slot) * (D / 4) * kRows + at;
+#pragma unroll 1
+          for (int c = 0; c < D / 64; ++c) {
+            float o[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) o[i] = 0.f;
+            for (int s = 0; s < p.splits; ++s) {
+              const float w = __ldcg(stat + s * kRows).x;
+              if (w == -INFINITY) continue;  // that range holds no key this row sees
+              const float f = ex2_approx(w - ref);
+              const float4* x4 = part0 + (static_cast<size_t>(s) * (D / 4) + 16 * c) * kRows;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float4 x = __ldcg(x4 + i * kRows);
+                o[4 * i] += f * x.x;
+                o[4 * i + 1] += f * x.y;
+                o[4 * i + 2] += f * x.z;
+                o[4 * i + 3] += f * x.w;
               }
             }
+#pragma unroll
+            for (int i = 0; i < 64; ++i) o[i] = lim < 0 ? 0.f : o[i] * inv;
+            emit(c, o);
           }
         }
       }
@@ -867,19 +855,20 @@ static EncodeTiled encoder() {
   return fn;
 }
 
-// Rows of 64 values (of D), `box` of them a copy; the dimensions after the row's are
-// `dims` with strides of `strides` elements. What lies outside reads as zeros.
+// Rows of 64 values (of D); the dimensions after the row's are `dims` with strides of
+// `strides` elements, a copy takes `box` of each. What lies outside reads as zeros.
 static cudaError_t map_rows(CUtensorMap* m, int dtype, const void* base, int D, int rank, const uint64_t* dims,
-                            const int64_t* strides, uint32_t box) {
+                            const int64_t* strides, const uint32_t* box) {
   const EncodeTiled enc = encoder();
   if (!enc) return cudaErrorNotSupported;
   cuuint64_t gd[4] = {static_cast<cuuint64_t>(D)}, gs[3];
-  cuuint32_t bx[4] = {64, box, 1, 1}, es[4] = {1, 1, 1, 1};
+  cuuint32_t bx[4] = {64, 1, 1, 1}, es[4] = {1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) {
     gd[i + 1] = dims[i] > 0 ? dims[i] : 1;
     // a stride of 0 (one element, or the same place for all) is never stepped along
     gs[i] = static_cast<cuuint64_t>(strides[i] > 0 ? strides[i] : D) * 2;
     if (strides[i] == 0) gd[i + 1] = 1;
+    bx[i + 1] = box[i];
   }
   const CUresult r = enc(m, dtype == MKB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                          rank + 1, const_cast<void*>(base), gd, gs, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -896,10 +885,10 @@ static int sm_count() {
   return n[dev] > 0 ? n[dev] : 148;
 }
 
-// Upper bound of the row blocks of a call, all KV heads.
+// Upper bound of the pieces of a call before any split, all KV heads.
 static int64_t tc_blocks(const mkb_attn_args& a) {
-  const int64_t rows = static_cast<int64_t>(a.tokens) * (a.heads / a.kv_heads);
-  return (rows / kRows + a.batch) * a.kv_heads;
+  const int64_t span = 2 * (128 / (a.heads / a.kv_heads));
+  return (a.tokens / span + a.batch) * a.kv_heads;
 }
 // Partial results a call can leave. Rows are split only past a fair share C >= 5/4 U /
 // grid of the U key tiles, into at most 2 n / C pieces for n tiles; a request's blocks
@@ -917,9 +906,11 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   g.a = a;
   g.sl2 = a.scale * 1.4426950408889634f;
   g.group = a.heads / a.kv_heads;
+  g.tile_tokens = 128 / g.group;
+  g.group_mul = 65536 / g.group + 1;
   g.k_head = a.k_stride[1] != 0;
   g.v_head = a.v_stride[1] != 0;
-  g.box = kPaged ? (a.page_size < kKeys ? a.page_size : kKeys) : kKeys;
+  g.box = kPaged && a.page_size < kKeys ? a.page_size : kKeys;
   g.slots = static_cast<int>(tc_slots(a));
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   if (ws == nullptr) return cudaErrorInvalidValue;
@@ -927,8 +918,15 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   g.counters = reinterpret_cast<uint32_t*>(ws);
   g.stat = reinterpret_cast<float2*>(ws + cb);
   g.part = reinterpret_cast<float4*>(ws + cb + static_cast<size_t>(g.slots) * kRows * 8);
-  CUtensorMap mk, mv;
+  CUtensorMap mk, mv, mq;
   cudaError_t e;
+  {
+    const uint64_t dims[2] = {static_cast<uint64_t>(a.heads), static_cast<uint64_t>(a.tokens)};
+    const int64_t qs[2] = {a.q_stride[1], a.q_stride[0]};
+    const uint32_t box[2] = {static_cast<uint32_t>(g.group), static_cast<uint32_t>(g.tile_tokens)};
+    if ((e = map_rows(&mq, a.dtype, a.q, D, 2, dims, qs, box)) != cudaSuccess) return e;
+  }
+  const uint32_t kbox[3] = {static_cast<uint32_t>(kPaged ? (a.page_size < kKeys ? a.page_size : kKeys) : kKeys), 1, 1};
   const void *kb = a.k, *vb = a.v;
   if (kPaged && a.pages == 0) kb = vb = a.q;  // an empty pool is never read: any address will do
   if (kPaged) {
@@ -936,12 +934,12 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
                               static_cast<uint64_t>(a.pages)};
     const int64_t ks[3] = {a.k_stride[2], a.k_stride[1], a.k_stride[0]};
     const int64_t vs[3] = {a.v_stride[2], a.v_stride[1], a.v_stride[0]};
-    if ((e = map_rows(&mk, a.dtype, kb, D, 3, dims, ks, g.box)) != cudaSuccess) return e;
-    if ((e = map_rows(&mv, a.dtype, vb, D, 3, dims, vs, g.box)) != cudaSuccess) return e;
+    if ((e = map_rows(&mk, a.dtype, kb, D, 3, dims, ks, kbox)) != cudaSuccess) return e;
+    if ((e = map_rows(&mv, a.dtype, vb, D, 3, dims, vs, kbox)) != cudaSuccess) return e;
   } else {
     const uint64_t dims[2] = {static_cast<uint64_t>(a.tokens), static_cast<uint64_t>(a.kv_heads)};
-    if ((e = map_rows(&mk, a.dtype, kb, D, 2, dims, a.k_stride, kKeys)) != cudaSuccess) return e;
-    if ((e = map_rows(&mv, a.dtype, vb, D, 2, dims, a.v_stride, kKeys)) != cudaSuccess) return e;
+    if ((e = map_rows(&mk, a.dtype, kb, D, 2, dims, a.k_stride, kbox)) != cudaSuccess) return e;
+    if ((e = map_rows(&mv, a.dtype, vb, D, 2, dims, a.v_stride, kbox)) != cudaSuccess) return e;
   }
   constexpr int bytes = sizeof(TcSmem<D>) + 1024;
   static_assert(bytes <= 232448, "shared memory of the attention kernel");
@@ -958,7 +956,7 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   const int64_t blocks = tc_blocks(a) * (kPaged ? (static_cast<int64_t>(a.table_width) * a.page_size / kKeys) / kMinSplit + 1
                                                 : a.tokens / (kKeys * kMinSplit) + 1);
   const int grid = static_cast<int>(blocks < sm_count() ? blocks : sm_count());
-  attn_tc_kernel<T, D, kPaged><<<grid, kTcThreads, bytes, stream>>>(mk, mv, g);
+  attn_tc_kernel<T, D, kPaged><<<grid, kTcThreads, bytes, stream>>>(mk, mv, mq, g);
   return cudaGetLastError();
 }
 
