@@ -42,9 +42,13 @@
 namespace mkb {
 namespace sv {
 
-constexpr int kTcThreads = 320;
+constexpr int kTcThreads = 384;
+// Registers of a thread: the launch's 168 are shared out again, to the softmax warps
+// that hold 128 scores a thread (2 x 128 x 208 + 128 x 88 = 384 x 168).
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 constexpr int kRows = 256, kKeys = 128;   // rows of a piece (two tiles), keys of a tile
 constexpr int kHalf = 128 * 128;          // 16 KB: 128 rows x 64 values, 128-byte swizzle
+constexpr int kFirstKeys = 96;            // of a tile's weights, what the second product starts on
 constexpr int kMinSplit = 6;              // key tiles below which rows are not split
 constexpr int kSortBatch = 128;           // requests up to which pieces are taken longest first
 constexpr int kTryNs = 20000, kTries = 50000;  // bound of every wait: about a second
@@ -69,7 +73,7 @@ struct TcSmem {
   uint8_t kv[kSlots][kTileBytes];
   uint8_t stage[8][32 * 128];                           // a warp's 32 rows x 64 values on their way out
   uint64_t kv_full[kSlots], kv_empty[kSlots];
-  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_part[2], p_full[2], o_full[2];
   uint64_t info_full[2], info_empty[2];
   uint64_t tile_bar[2];   // the four softmax warps of a tile
   Piece piece[2];
@@ -83,6 +87,8 @@ struct TcArgs {
   float sl2;            // scale * log2(e)
   int group;            // query heads of a KV head
   int tile_tokens;      // tokens of a tile: 128 / group
+  int warp_tokens;      // tokens of a warp's 32 rows, 0 where they are not whole
+  unsigned span_mul;    // x / (2 tile_tokens) is x * span_mul >> 32, or one less
   int group_mul;        // r / group = r * group_mul >> 16 for r < 128
   int k_head, v_head;   // 0 where every KV head lies at the same place (stride 0), else 1
   int box;              // keys of a TMA box
@@ -115,6 +121,15 @@ __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x,
       ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
       : "memory");
 }
+__device__ __forceinline__ void tma_store_3d(const void* src, const CUtensorMap* map, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];\n\t"
+               "cp.async.bulk.commit_group;"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+// this thread's stores: their shared memory has been read / they are done
+__device__ __forceinline__ void tma_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
@@ -143,23 +158,57 @@ __host__ __device__ constexpr uint32_t idesc16(int m, int n, bool mn) {
   return (1u << 4) | (f << 7) | (f << 10) | (mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
 }
-// D[tmem] (+)= A[tmem] B[smem desc]
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// One lane of a converged warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b32 t;\n\t"
+      "elect.sync t|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
+}
+// The tensor-core instructions are issued by one lane (`leader`), but the whole warp runs
+// through them, predicated: their operands then stay warp-uniform. Inside a branch of one
+// lane every one of them costs a round of moves into uniform registers (80 cycles an
+// MMA, measured, against 64 of tensor-core work for 128 x 128 x 16).
+// D[tmem] (+)= A[smem desc] B[smem desc]
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32_u(uint32_t taddr, const uint32_t v[32]) {
+// D[tmem] (+)= A[tmem] B[smem desc]
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+// Arrive on `bar` once all that the leader issued before has completed.
+__device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_addr(bar)), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t v[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};"
       ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
-        "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
-        "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -183,6 +232,18 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// the largest of three; NaN where one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
@@ -213,11 +274,13 @@ __device__ __forceinline__ int tiles_of(const Load& l, int toks) {
   return l.bad || keys <= 0 ? 0 : static_cast<int>((static_cast<unsigned>(keys) + kKeys - 1) / kKeys);
 }
 // how many of the request's blocks of `span` tokens see more than x key tiles (they come last)
-__device__ __forceinline__ int blocks_above(const Load& l, int span, int x) {
+__device__ __forceinline__ int blocks_above(const Load& l, int span, unsigned span_mul, int x) {
   if (x < 0) return l.blocks;
   if (l.tiles <= x) return 0;
   const int y = x * kKeys - l.ctx;  // the first token that sees more (x < tiles: no overflow)
-  return y <= 0 ? l.blocks : l.blocks - static_cast<int>(static_cast<unsigned>(y) / static_cast<unsigned>(span));
+  int i = static_cast<int>(__umulhi(static_cast<unsigned>(y), span_mul));  // y / span, once it is positive
+  if (i * span > y) --i;
+  return y <= 0 ? l.blocks : l.blocks - i;
 }
 
 // ---- one row, key by key: what a tile with values that are not finite comes to --------
@@ -274,13 +337,17 @@ __device__ __noinline__ void slow_row(const TcArgs& g, const Piece& p, int token
 template <typename T, int D, bool kPaged>
 __global__ void __launch_bounds__(kTcThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                   const __grid_constant__ CUtensorMap tq, const __grid_constant__ TcArgs g) {
+                   const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap to,
+                   const __grid_constant__ TcArgs g) {
   using Smem = TcSmem<D>;
   constexpr int kSlots = Smem::kSlots, kTileBytes = Smem::kTileBytes;
   extern __shared__ uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const mkb_attn_args& a = g.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // a lane of the loading warp keeps its first request; the others are read again in every pass
+  Load mine = {};
+  if (warp == 9 && lane < a.batch) mine = load_of<kPaged>(g, lane);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&sm.kv_full[s], 1);
@@ -290,6 +357,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&sm.q_full[t], 1);
       mbar_init(&sm.q_empty[t], 1);
       mbar_init(&sm.s_full[t], 1);
+      mbar_init(&sm.p_part[t], 4);
       mbar_init(&sm.p_full[t], 4);
       mbar_init(&sm.o_full[t], 1);
       mbar_init(&sm.info_full[t], 1);
@@ -306,8 +374,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tbase = sm.tmem_base;  // S/P of A and B at 0 and 128, O at 256 and 384
+  // all 512 columns: S/P of A and B at 0 and 128, O at 256 and 384 (the base is 0 then,
+  // which as a constant keeps the addresses out of registers)
+  constexpr uint32_t tbase = 0;
+  if (sm.tmem_base != 0) sm.err = 1;
 
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == 9) {
     // ---- the next piece, and its loads ------------------------------------------------
     if (lane == 0) {
@@ -316,8 +389,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc::prefetch_tensormap(&tq);
     }
     const int kv_heads = a.kv_heads, grid = gridDim.x, span = 2 * g.tile_tokens;
-    // a lane keeps its first request; the others are read again in every pass
-    const Load mine = lane < a.batch ? load_of<kPaged>(g, lane) : Load{};
     auto request = [&](int b) { return b < 32 ? mine : load_of<kPaged>(g, b); };
     // a fair share of the key tiles; rows with more are split
     long long total = 0;
@@ -339,7 +410,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int b = lane; b < a.batch; b += 32) {
         const Load l = request(b);
         const int sp = splits_of(l);
-        n += blocks_above(l, span, x * sp) * sp;
+        n += blocks_above(l, span, g.span_mul, x * sp) * sp;
       }
       return __reduce_add_sync(0xffffffffu, n) * kv_heads;
     };
@@ -373,8 +444,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           l = request(b);
           l.splits = splits_of(l);
           if (sorted) {
-            above = blocks_above(l, span, lo * l.splits);
-            here = blocks_above(l, span, lo * l.splits - l.splits) - above;
+            above = blocks_above(l, span, g.span_mul, lo * l.splits);
+            here = blocks_above(l, span, g.span_mul, lo * l.splits - l.splits) - above;
           } else {
             here = l.blocks;
           }
@@ -499,6 +570,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     constexpr uint32_t id_s = idesc16<T>(128, kKeys, false), id_o = idesc16<T>(128, D, true);
     const uint64_t dq0 = tc::desc_sw128(smem_addr(sm.q[0])), dk0 = tc::desc_sw128(smem_addr(sm.kv[0]));
     const uint64_t dv0 = desc_mn_sw128(smem_addr(sm.kv[0]), kHalf);
+    const uint32_t leader = elect_one();
     int it = 0;                       // ring slots taken so far
     uint32_t q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
     bool ok = true;
@@ -522,22 +594,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (!wait_warp(&sm.kv_full[s], (i / kSlots) & 1, &sm.err)) return false;
         tc::fence_after_sync();
-        if (lane == 0) {
-          const uint64_t dq = tc::desc_advance(dq0, t * kTileBytes), dk = tc::desc_advance(dk0, s * kTileBytes);
+        const uint64_t dq = tc::desc_advance(dq0, t * kTileBytes), dk = tc::desc_advance(dk0, s * kTileBytes);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * kHalf + (kk & 3) * 32;
-            tc::mma_bf16_ss(tbase + 128 * t, tc::desc_advance(dq, off), tc::desc_advance(dk, off), id_s, kk != 0);
-          }
-          tc::commit(&sm.s_full[t]);
-          if (j + 1 == nt[t]) tc::commit(&sm.q_empty[t]);
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kHalf + (kk & 3) * 32;
+          mma_ss(leader, tbase + 128 * t, tc::desc_advance(dq, off), tc::desc_advance(dk, off), id_s, kk != 0);
         }
-        __syncwarp();
+        commit(leader, &sm.s_full[t]);
+        if (j + 1 == nt[t]) commit(leader, &sm.q_empty[t]);
         return true;
       };
       for (int t = 0; t < 2 && ok; ++t)
         if (nt[t] > 0) ok = scores(t, 0);
-      if (ok && lane == 0) tc::commit(&sm.kv_empty[slot_k(0) % kSlots]);
+      if (ok) commit(leader, &sm.kv_empty[slot_k(0) % kSlots]);
       for (int j = 0; j < n && ok; ++j) {
         const int i = slot_v(j), s = i % kSlots;
         if (!wait_warp(&sm.kv_full[s], (i / kSlots) & 1, &sm.err)) {
@@ -556,32 +625,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         for (int t = 0; t < 2 && ok; ++t) {
           if (j >= nt[t]) continue;
+          const uint64_t dv = tc::desc_advance(dv0, s * kTileBytes);
+          if (!(ok = wait_warp(&sm.p_part[t], p_ph[t], &sm.err))) break;
+          tc::fence_after_sync();
+#pragma unroll
+          for (int kk = 0; kk < kFirstKeys / 16; ++kk)
+            mma_ts(leader, tbase + 256 + 128 * t, tbase + 128 * t + 8 * kk, tc::desc_advance(dv, kk * 2048), id_o,
+                   (j | kk) != 0);
           if (!(ok = wait_warp(&sm.p_full[t], p_ph[t], &sm.err))) break;
           p_ph[t] ^= 1;
           tc::fence_after_sync();
-          if (lane == 0) {
-            const uint64_t dv = tc::desc_advance(dv0, s * kTileBytes);
 #pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)
-              mma_ts(tbase + 256 + 128 * t, tbase + 128 * t + 8 * kk, tc::desc_advance(dv, kk * 2048), id_o,
-                     (j | kk) != 0);
-          }
-          __syncwarp();
-          if (j + 1 < nt[t]) {
-            ok = scores(t, j + 1);  // its commit covers O as well: S(j + 1) seen means PV(j) done
-          } else if (lane == 0) {
-            tc::commit(&sm.o_full[t]);
-          }
+          for (int kk = kFirstKeys / 16; kk < kKeys / 16; ++kk)
+            mma_ts(leader, tbase + 256 + 128 * t, tbase + 128 * t + 8 * kk, tc::desc_advance(dv, kk * 2048), id_o, 1u);
+          if (j + 1 < nt[t]) ok = scores(t, j + 1);  // its commit covers O as well: S(j + 1) seen means PV(j) done
+          else commit(leader, &sm.o_full[t]);
         }
-        if (ok && lane == 0) {
-          tc::commit(&sm.kv_empty[s]);
-          if (j + 1 < n) tc::commit(&sm.kv_empty[slot_k(j + 1) % kSlots]);
+        if (ok) {
+          commit(leader, &sm.kv_empty[s]);
+          if (j + 1 < n) commit(leader, &sm.kv_empty[slot_k(j + 1) % kSlots]);
         }
-        __syncwarp();
       }
       it += 2 * n;
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ---- softmax of a tile, a thread per row ----------------------------------------------
     const int t = warp >> 2;                 // tile
     const int row_in = threadIdx.x & 127;    // row of the tile = TMEM lane
@@ -631,22 +700,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc::tmem_wait_ld<false>(sr[2]);
         tc::tmem_wait_ld<false>(sr[3]);
         const int key0 = (p.k0 + j) * kKeys;
-        if (key0 + kKeys - 1 > lim0) {  // some row of the tile does not see all of these keys
+        const bool masked = key0 + kKeys - 1 > lim0;  // some row of the tile does not see all of these keys
+        if (masked) {
 #pragma unroll
           for (int i = 0; i < 128; ++i)
             if (key0 + i > lim) sr[i >> 5][i & 31] = 0xff800000u;
         }
-        float mx = -INFINITY;
+        float mx;
         {
-          float x4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float x4[4];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
+          for (int c = 0; c < 4; ++c) x4[c] = max_nan(__uint_as_float(sr[c][0]), __uint_as_float(sr[c][1]));
 #pragma unroll
-            for (int c = 0; c < 4; ++c) x4[c] = fmaxf(x4[c], __uint_as_float(sr[c][i]));
-          mx = live ? fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])) * sl2 : -INFINITY;
+          for (int i = 2; i < 32; i += 2)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x4[c] = max3(x4[c], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
+          mx = live ? max_nan(max_nan(x4[0], x4[1]), max_nan(x4[2], x4[3])) * sl2 : -INFINITY;
         }
-        if (__any_sync(0xffffffffu, mx > m + 8.f)) {  // (also the first tile: m = -inf)
-          const float mn = fmaxf(m, mx);
+        if (__any_sync(0xffffffffu, !(mx <= m + 8.f) && mx != -INFINITY)) {  // (also the first tile: m = -inf)
+          const float mn = max_nan(m, mx);
           const float sc = mn == -INFINITY ? 0.f : ex2_approx(m - mn);
           const uint64_t sc2 = pack2(sc, sc);
           if (j > 0) {  // S(j) is there, so PV(j - 1) is done and O can be rescaled
@@ -662,27 +734,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           l2 = fma2(l2, sc2, 0);
           m = mn;
         }
-        const float ref = m == -INFINITY ? 0.f : -m;
+        // an infinite maximum leaves no weights (inf - inf); none at all, weights of 0
+        const float ref = m == -INFINITY ? 0.f : m == INFINITY ? NAN : -m;
         const uint64_t ref2 = pack2(ref, ref), sl22 = pack2(sl2, sl2);
         uint64_t la = 0, lb = 0;
+        auto arrive = [&](uint64_t* bar) {
+          tmem_wait_st();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar);
+        };
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t pw[32];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pw[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const uint32_t* s = sr[2 * half + (i >> 4)] + 2 * (i & 15);
-            const float2 x = unpack2(fma2(pack2(__uint_as_float(s[0]), __uint_as_float(s[1])), sl22, ref2));
+          for (int i = 0; i < 16; ++i) {
+            const float2 x = unpack2(fma2(pack2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), sl22, ref2));
             const float e0 = ex2_approx(x.x), e1 = ex2_approx(x.y);
             if (i & 1) lb = add2(lb, pack2(e0, e1));
             else la = add2(la, pack2(e0, e1));
             pw[i] = Pair<T>::put(e0, e1);
           }
-          tmem_st32_u(t_s + 32 * half, pw);
+          tmem_st16(t_s + 16 * c, pw);
+          if (32 * (c + 1) == kFirstKeys) arrive(&sm.p_part[t]);
         }
-        tmem_wait_st();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[t]);
+        arrive(&sm.p_full[t]);
         l2 = add2(l2, add2(la, lb));
       }
       if (!ok) break;
@@ -698,13 +774,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int k_end = min(p.len, (p.k0 + n) * kKeys);
       constexpr int kPer = D / 32;
       uint8_t* stage = sm.stage[warp];
-      // 64 values of every row of the warp to memory, 128 bytes of four rows at a time
+      // 64 values of every row of the warp to memory: by one TMA store where all 32 rows are
+      // whole tokens of the request, else 128 bytes of four rows at a time
+      const int tok_w = tok_t + g.warp_tokens * (warp & 3);
+      const bool whole = g.warp_tokens > 0 && tok_w + g.warp_tokens <= p.tok0 + p.toks;
       auto emit = [&](int half, const float* o) {
+        if (lane == 0) tma_store_read();
+        __syncwarp();
 #pragma unroll
         for (int c = 0; c < 8; ++c)
           *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = pack8<T>(o + 8 * c);
+        if (whole) {
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) tma_store_3d(stage, &to, 64 * half, p.hk * g.group, p.first + tok_w);
+          return;
+        }
         __syncwarp();
-#pragma unroll
+#pragma unroll 2
         for (int i = 0; i < 8; ++i) {
           const int r = 4 * i + (lane >> 3), rt = 32 * (warp & 3) + r;
           const int tok = rt * g.group_mul >> 16, head = p.hk * g.group + rt - tok * g.group;
@@ -718,6 +805,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // the rows of the warp whose O is not finite, key by key
       auto again = [&](bool odd, auto&& put) {
         uint32_t todo = __ballot_sync(0xffffffffu, odd && live);
+        if (todo != 0) {
+          if (lane == 0) tma_store_done();
+          __syncwarp();
+        }
         while (todo != 0) {
           const int r = __ffs(todo) - 1, rt = 32 * (warp & 3) + r;
           todo &= todo - 1;
@@ -730,7 +821,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       };
       float odd = 0.f;  // NaN once a value of O is not finite
       if (p.splits == 1) {
-        const float inv = bad ? NAN : lim < 0 ? 0.f : 1.f / l;
+        const float inv = bad || m == -INFINITY ? NAN : 1.f / l;  // no weights: every score -inf
 #pragma unroll 1
         for (int c = 0; c < D / 64; ++c) {
           float o[64];
@@ -828,6 +919,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       tc::fence_before_sync();  // O has been read: the next piece's first PV may overwrite it
     }
+    if (lane == 0) tma_store_done();
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -907,7 +999,9 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   g.sl2 = a.scale * 1.4426950408889634f;
   g.group = a.heads / a.kv_heads;
   g.tile_tokens = 128 / g.group;
+  g.warp_tokens = 32 % g.group == 0 ? 32 / g.group : 0;
   g.group_mul = 65536 / g.group + 1;
+  g.span_mul = static_cast<unsigned>((1ull << 32) / (2 * g.tile_tokens) + 1);
   g.k_head = a.k_stride[1] != 0;
   g.v_head = a.v_stride[1] != 0;
   g.box = kPaged && a.page_size < kKeys ? a.page_size : kKeys;
@@ -918,13 +1012,19 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   g.counters = reinterpret_cast<uint32_t*>(ws);
   g.stat = reinterpret_cast<float2*>(ws + cb);
   g.part = reinterpret_cast<float4*>(ws + cb + static_cast<size_t>(g.slots) * kRows * 8);
-  CUtensorMap mk, mv, mq;
+  CUtensorMap mk, mv, mq, mo;
   cudaError_t e;
   {
     const uint64_t dims[2] = {static_cast<uint64_t>(a.heads), static_cast<uint64_t>(a.tokens)};
     const int64_t qs[2] = {a.q_stride[1], a.q_stride[0]};
     const uint32_t box[2] = {static_cast<uint32_t>(g.group), static_cast<uint32_t>(g.tile_tokens)};
     if ((e = map_rows(&mq, a.dtype, a.q, D, 2, dims, qs, box)) != cudaSuccess) return e;
+    mo = mq;
+    if (g.warp_tokens > 0) {
+      const int64_t os[2] = {a.out_stride[1], a.out_stride[0]};
+      const uint32_t obox[2] = {box[0], static_cast<uint32_t>(g.warp_tokens)};
+      if ((e = map_rows(&mo, a.dtype, a.out, D, 2, dims, os, obox)) != cudaSuccess) return e;
+    }
   }
   const uint32_t kbox[3] = {static_cast<uint32_t>(kPaged ? (a.page_size < kKeys ? a.page_size : kKeys) : kKeys), 1, 1};
   const void *kb = a.k, *vb = a.v;
@@ -956,7 +1056,7 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   const int64_t blocks = tc_blocks(a) * (kPaged ? (static_cast<int64_t>(a.table_width) * a.page_size / kKeys) / kMinSplit + 1
                                                 : a.tokens / (kKeys * kMinSplit) + 1);
   const int grid = static_cast<int>(blocks < sm_count() ? blocks : sm_count());
-  attn_tc_kernel<T, D, kPaged><<<grid, kTcThreads, bytes, stream>>>(mk, mv, mq, g);
+  attn_tc_kernel<T, D, kPaged><<<grid, kTcThreads, bytes, stream>>>(mk, mv, mq, mo, g);
   return cudaGetLastError();
 }
 
