@@ -6,18 +6,25 @@
 // A KV head's queries are rows: row r of a tile is token r / G, query head r % G of the
 // G that share the KV head, so that one pass over the keys serves all of them; a tile
 // holds the 128 / G tokens that fill (nearly) 128 rows. A CTA takes two tiles (A and B)
-// of one request and KV head and walks its keys 128 at a time:
+// of one request and KV head and walks its keys a tile of 80 (heads of 128) or 128
+// (heads of 64) at a time:
 //
 //   warp 9      which piece of work comes next; its Q, K and V tiles by TMA (128-byte
 //               swizzle; K and V through a ring, pages are boxes of page_size rows)
-//   warp 8      tcgen05.mma: S = Q K^T (Q and K in shared memory), O += P V with P from
+//   warps 8, 10 tcgen05.mma of tile A, B: S = Q K^T (Q and K in shared memory), O += P V with P from
 //               tensor memory and V as it lies, keys by dims (an MN-major operand: no
 //               transposed copy of V is made)
 //   warps 0-3   softmax of tile A, a thread per row: S out of tensor memory, running
-//   warps 4-7   maximum and sum in FP32 registers, P back into the columns S had; tile B
+//   warps 4-7   maximum and sum in FP32 registers, P into tensor memory; tile B
 //
-// While one tile's softmax runs, the tensor core works on the other's products. The
-// running maximum that P is relative to moves only when a row's grows by more than 8
+// Tensor memory holds S, P and O of both tiles, each at columns of its own: 2 (80 + 40 +
+// 128) = 496 of 512, which is what makes a tile 80 keys. A softmax warp frees S as soon
+// as it has it in registers, so the tensor core has the next scores done while this
+// tile's weights are computed; with P in S's columns (tiles of 128 keys) every tile
+// waited for the two products in turn, 3,580 cycles a pair of 128 x 128 tiles where the
+// products take 2,048.
+//
+// The running maximum that P is relative to moves only when a row's grows by more than 8
 // (a factor 256): O, in tensor memory, is then rescaled by the softmax warps; between
 // moves P stays below 2^8, which FP32 sums and 16-bit P hold without loss. P is rounded
 // to the operands' 16-bit type, as the output is: the same relative error.
@@ -46,10 +53,9 @@ constexpr int kTcThreads = 384;
 // Registers of a thread: the launch's 168 are shared out again, to the softmax warps
 // that hold 128 scores a thread (2 x 128 x 208 + 128 x 88 = 384 x 168).
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
-constexpr int kRows = 256, kKeys = 128;   // rows of a piece (two tiles), keys of a tile
-constexpr int kHalf = 128 * 128;          // 16 KB: 128 rows x 64 values, 128-byte swizzle
-constexpr int kFirstKeys = 96;            // of a tile's weights, what the second product starts on
-constexpr int kMinSplit = 6;              // key tiles below which rows are not split
+constexpr int kRows = 256;                // rows of a piece (two tiles)
+constexpr int kQHalf = 128 * 128;         // 16 KB: 128 rows x 64 values, 128-byte swizzle
+constexpr int kMinSplit = 8;              // key tiles below which rows are not split
 constexpr int kSortBatch = 128;           // requests up to which pieces are taken longest first
 constexpr int kTryNs = 20000, kTries = 50000;  // bound of every wait: about a second
 
@@ -66,14 +72,24 @@ struct Piece {
 };
 
 template <int D>
+struct TcShape {
+  static constexpr int kKeys = D == 128 ? 80 : 128;     // of a tile
+  static constexpr int kSlots = D == 128 ? 6 : 7;       // K and V tiles in flight
+  static constexpr int kTileBytes = kKeys * D * 2;
+  static constexpr int kTileHalf = kKeys * 128;         // 64 values of every key
+  // tensor memory columns
+  static constexpr uint32_t kS = 0, kP = 2 * kKeys, kO = 512 - 2 * D;
+  static_assert(3 * kKeys <= 512 - 2 * D, "tensor memory");
+};
+
+template <int D>
 struct TcSmem {
-  static constexpr int kTileBytes = D * 256;            // 128 keys
-  static constexpr int kSlots = D == 128 ? 4 : 8;
-  uint8_t q[2][kTileBytes];
-  uint8_t kv[kSlots][kTileBytes];
+  using Shape = TcShape<D>;
+  uint8_t q[2][128 * D * 2];
+  uint8_t kv[Shape::kSlots][Shape::kTileBytes];
   uint8_t stage[8][32 * 128];                           // a warp's 32 rows x 64 values on their way out
-  uint64_t kv_full[kSlots], kv_empty[kSlots];
-  uint64_t q_full[2], q_empty[2], s_full[2], p_part[2], p_full[2], o_full[2];
+  uint64_t kv_full[Shape::kSlots], kv_empty[Shape::kSlots];
+  uint64_t q_full[2], q_empty[2], s_full[2], s_free[2], p_full[2], o_done[2];
   uint64_t info_full[2], info_empty[2];
   uint64_t tile_bar[2];   // the four softmax warps of a tile
   Piece piece[2];
@@ -98,21 +114,24 @@ struct TcArgs {
   float2* stat;         // [slots][256]: maximum, sum
 };
 
-// Bounded: each try suspends for 20 us at most. (Counted, not timed: reading the global
-// timer before the first try costs more than most waits last.)
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t ph, int* err) {
-  for (int i = 0; !mbar_wait(bar, ph, kTryNs); ++i) {
-    if (*reinterpret_cast<volatile int*>(err) != 0) return false;
-    if (i == kTries) {
-      *reinterpret_cast<volatile int*>(err) = 1;
-      return false;
+// A warp's wait for a phase of a barrier. Bounded: each try suspends for 20 us at most.
+// Once one has expired (here or in another warp) the warp is `dead`: it runs through what
+// is left of its part without waiting, so that nothing depends on the state of a lane.
+// (Short on purpose: the loops of the softmax warps fill the instruction caches, and what
+// the other warps run between two MMAs is fetched anew every time.)
+__device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t ph, int* err, bool& dead) {
+  if (!mbar_test(bar, ph) && !dead) {
+    int i = 0;
+#pragma unroll 1
+    while (!mbar_wait(bar, ph, kTryNs)) {
+      if (++i > kTries || *reinterpret_cast<volatile int*>(err) != 0) {
+        *reinterpret_cast<volatile int*>(err) = 1;
+        dead = true;
+        break;
+      }
     }
   }
-  return true;
-}
-// every lane of a warp; goes on only if all saw the phase
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t ph, int* err) {
-  return __all_sync(0xffffffffu, wait_bar(bar, ph, err));
+  dead = __any_sync(0xffffffffu, dead);
 }
 
 __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
@@ -168,6 +187,8 @@ __device__ __forceinline__ uint32_t elect_one() {
       : "=r"(r));
   return r;
 }
+// A value that every lane holds, in a uniform register.
+__device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }
 // The tensor-core instructions are issued by one lane (`leader`), but the whole warp runs
 // through them, predicated: their operands then stay warp-uniform. Inside a branch of one
 // lane every one of them costs a round of moves into uniform registers (80 cycles an
@@ -203,14 +224,29 @@ __device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
       ::"r"(smem_addr(bar)), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t v[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16};"
-      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-      : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t v[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
+// 16 columns of this thread's lane; valid after tmem_wait_ld, which takes the first of
+// several such loads (the others go through pin16, so that no use moves before it)
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+#define MKB_PIN16(text)                                                                                              \
+  asm volatile(text                                                                                                  \
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),     \
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) \
+               :: "memory")
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) { MKB_PIN16("tcgen05.wait::ld.sync.aligned;"); }
+__device__ __forceinline__ void pin16(uint32_t* r) { MKB_PIN16(""); }
+#undef MKB_PIN16
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // two FP32 operations in one instruction
@@ -253,7 +289,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 struct Load {
   int first, q, len, ctx, blocks, tiles, splits, bad;
 };
-template <bool kPaged>
+template <int kKeys, bool kPaged>
 __device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
   const Request rq = request_rows(g.a.cu_q, b, g.a.q_len, g.a.tokens);
   Load l;
@@ -269,11 +305,13 @@ __device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
   return l;
 }
 // key tiles that the first `toks` tokens of the request see
+template <int kKeys>
 __device__ __forceinline__ int tiles_of(const Load& l, int toks) {
   const int keys = l.ctx + min(toks, l.q);
   return l.bad || keys <= 0 ? 0 : static_cast<int>((static_cast<unsigned>(keys) + kKeys - 1) / kKeys);
 }
 // how many of the request's blocks of `span` tokens see more than x key tiles (they come last)
+template <int kKeys>
 __device__ __forceinline__ int blocks_above(const Load& l, int span, unsigned span_mul, int x) {
   if (x < 0) return l.blocks;
   if (l.tiles <= x) return 0;
@@ -296,7 +334,7 @@ __device__ __noinline__ void slow_row(const TcArgs& g, const Piece& p, int token
   float m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-  for (int j = p.k0 * kKeys; j < keys; ++j) {
+  for (int j = p.k0 * TcShape<D>::kKeys; j < keys; ++j) {
     int64_t ko, vo;
     if (kPaged) {
       const int64_t page = a.block_table[p.b * a.table_stride + j / a.page_size], slot = j % a.page_size;
@@ -340,29 +378,30 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                    const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap to,
                    const __grid_constant__ TcArgs g) {
   using Smem = TcSmem<D>;
-  constexpr int kSlots = Smem::kSlots, kTileBytes = Smem::kTileBytes;
+  using Shape = TcShape<D>;
+  constexpr int kKeys = Shape::kKeys, kSlots = Shape::kSlots, kTileBytes = Shape::kTileBytes, kHalf = Shape::kTileHalf;
   extern __shared__ uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const mkb_attn_args& a = g.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // a lane of the loading warp keeps its first request; the others are read again in every pass
   Load mine = {};
-  if (warp == 9 && lane < a.batch) mine = load_of<kPaged>(g, lane);
+  if (warp == 9 && lane < a.batch) mine = load_of<kKeys, kPaged>(g, lane);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&sm.kv_full[s], 1);
-      mbar_init(&sm.kv_empty[s], 1);
+      mbar_init(&sm.kv_empty[s], 2);  // both tiles' products
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sm.q_full[t], 1);
       mbar_init(&sm.q_empty[t], 1);
       mbar_init(&sm.s_full[t], 1);
-      mbar_init(&sm.p_part[t], 4);
+      mbar_init(&sm.s_free[t], 4);
       mbar_init(&sm.p_full[t], 4);
-      mbar_init(&sm.o_full[t], 1);
+      mbar_init(&sm.o_done[t], 1);
       mbar_init(&sm.info_full[t], 1);
       mbar_init(&sm.tile_bar[t], 4);
-      mbar_init(&sm.info_empty[t], 9);  // eight softmax warps and the MMA warp
+      mbar_init(&sm.info_empty[t], 10);  // eight softmax warps, two MMA warps
     }
     sm.err = 0;
     fence_mbar_init();
@@ -374,9 +413,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  // all 512 columns: S/P of A and B at 0 and 128, O at 256 and 384 (the base is 0 then,
-  // which as a constant keeps the addresses out of registers)
+  // all 512 columns: the base is 0 then, which as a constant keeps the addresses out of registers
   constexpr uint32_t tbase = 0;
+  bool dead = false;
   if (sm.tmem_base != 0) sm.err = 1;
 
   if (warp >= 8) {
@@ -389,13 +428,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc::prefetch_tensormap(&tq);
     }
     const int kv_heads = a.kv_heads, grid = gridDim.x, span = 2 * g.tile_tokens;
-    auto request = [&](int b) { return b < 32 ? mine : load_of<kPaged>(g, b); };
+    auto request = [&](int b) { return b < 32 ? mine : load_of<kKeys, kPaged>(g, b); };
     // a fair share of the key tiles; rows with more are split
     long long total = 0;
     int top = 0;
     for (int b = lane; b < a.batch; b += 32) {
       const Load l = request(b);
-      total += static_cast<long long>(tiles_of(l, span) + l.tiles) * l.blocks;  // twice the sum: linear in the block
+      total += static_cast<long long>(tiles_of<kKeys>(l, span) + l.tiles) * l.blocks;  // twice the sum: linear in the block
       top = max(top, l.tiles);
     }
 #pragma unroll
@@ -410,15 +449,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int b = lane; b < a.batch; b += 32) {
         const Load l = request(b);
         const int sp = splits_of(l);
-        n += blocks_above(l, span, g.span_mul, x * sp) * sp;
+        n += blocks_above<kKeys>(l, span, g.span_mul, x * sp) * sp;
       }
       return __reduce_add_sync(0xffffffffu, n) * kv_heads;
     };
     // longest first, unless every piece has a CTA of its own (or the list is long: even anyway)
     const bool sorted = a.batch <= kSortBatch && pieces_above(-1) > grid;
-    int it = 0, k = 0, q_uses[2] = {0, 0};
-    bool ok = true;
-    for (; ok; ++k) {
+    int slot = 0, k = 0, q_uses[2] = {0, 0};  // the ring's next slot, and how often it has gone round
+    uint32_t round = 0;
+    for (; !dead; ++k) {
       const int st = k & 1;
       const long long want = static_cast<long long>(k) * grid + (k & 1 ? grid - 1 - blockIdx.x : blockIdx.x);
       Piece p;
@@ -444,8 +483,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           l = request(b);
           l.splits = splits_of(l);
           if (sorted) {
-            above = blocks_above(l, span, g.span_mul, lo * l.splits);
-            here = blocks_above(l, span, g.span_mul, lo * l.splits - l.splits) - above;
+            above = blocks_above<kKeys>(l, span, g.span_mul, lo * l.splits);
+            here = blocks_above<kKeys>(l, span, g.span_mul, lo * l.splits - l.splits) - above;
           } else {
             here = l.blocks;
           }
@@ -476,13 +515,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             p.ctx = l.ctx;
             p.tok0 = i * span;
             p.toks = min(l.q - p.tok0, span);
-            const int n = tiles_of(l, p.tok0 + p.toks), per = (n + l.splits - 1) / l.splits;
+            const int n = tiles_of<kKeys>(l, p.tok0 + p.toks), per = (n + l.splits - 1) / l.splits;
             p.k0 = min(p.split * per, n);
             const int k1 = min(p.k0 + per, n);
             p.splits = l.splits;
             p.slot = slot_base + sinc - slots + (i * kv_heads + p.hk) * l.splits;
             p.bad = l.bad;
-            p.n[0] = max(min(tiles_of(l, p.tok0 + min(p.toks, g.tile_tokens)), k1) - p.k0, 0);
+            p.n[0] = max(min(tiles_of<kKeys>(l, p.tok0 + min(p.toks, g.tile_tokens)), k1) - p.k0, 0);
             p.n[1] = p.toks > g.tile_tokens ? k1 - p.k0 : 0;
             if (l.bad) report(a.status, MKB_SERVE_BAD_LENGTH);
           }
@@ -495,7 +534,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         r -= __shfl_sync(0xffffffffu, inc, 31);
         slot_base += __shfl_sync(0xffffffffu, sinc, 31);
       }
-      if (k >= 2 && !wait_warp(&sm.info_empty[st], ((k >> 1) - 1) & 1, &sm.err)) break;
+      if (k >= 2) wait_for(&sm.info_empty[st], ((k >> 1) - 1) & 1, &sm.err, dead);
       if (lane == 0) {
         sm.piece[st] = p;
         mbar_arrive(&sm.info_full[st]);
@@ -504,10 +543,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (p.b < 0) break;
       // K(0), then K(j + 1) and V(j): the order in which the products take them
       const int n = max(p.n[0], p.n[1]);
-      auto load = [&](const CUtensorMap* map, int head, int j) -> bool {
-        const int s = it % kSlots;
-        if (it >= kSlots && !wait_warp(&sm.kv_empty[s], (it / kSlots - 1) & 1, &sm.err)) return false;
-        ++it;
+      auto load = [&](const CUtensorMap* map, int head, int j) {
+        const int s = slot;
+        if (round > 0) wait_for(&sm.kv_empty[s], (round - 1) & 1, &sm.err, dead);
+        if (dead) return;
+        if (++slot == kSlots) {
+          slot = 0;
+          ++round;
+        }
         const int key = (p.k0 + j) * kKeys;
         if (lane == 0) mbar_arrive_expect_tx(&sm.kv_full[s], kTileBytes);
         __syncwarp();
@@ -534,119 +577,120 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int d = 0; d < D / 64; ++d)
             tma_3d(sm.kv[s] + d * kHalf, map, 64 * d, p.first + key, head, &sm.kv_full[s]);
         }
-        return true;
       };
       const int kh = p.hk * g.k_head, vh = p.hk * g.v_head;
-      if (n > 0) ok = load(&tk, kh, 0);
-      for (int t = 0; t < 2 && ok; ++t) {  // Q once the last product of the tile's previous one has read it
+      if (n > 0) load(&tk, kh, 0);
+      for (int t = 0; t < 2; ++t) {  // Q once the last product of the tile's previous one has read it
         if (p.n[t] == 0) continue;
-        if (q_uses[t] > 0 && !(ok = wait_warp(&sm.q_empty[t], (q_uses[t] - 1) & 1, &sm.err))) break;
+        if (q_uses[t] > 0) wait_for(&sm.q_empty[t], (q_uses[t] - 1) & 1, &sm.err, dead);
+        if (dead) break;
         ++q_uses[t];
         if (lane == 0) {
           mbar_arrive_expect_tx(&sm.q_full[t], g.tile_tokens * g.group * D * 2);
 #pragma unroll
           for (int d = 0; d < D / 64; ++d)
-            tma_3d(sm.q[t] + d * kHalf, &tq, 64 * d, p.hk * g.group, p.first + p.tok0 + t * g.tile_tokens, &sm.q_full[t]);
+            tma_3d(sm.q[t] + d * kQHalf, &tq, 64 * d, p.hk * g.group, p.first + p.tok0 + t * g.tile_tokens, &sm.q_full[t]);
         }
         __syncwarp();
       }
-      for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n) ok = load(&tk, kh, j + 1);
-        if (ok) ok = load(&tv, vh, j);
+      for (int j = 0; j < n && !dead; ++j) {
+        if (j + 1 < n) load(&tk, kh, j + 1);
+        load(&tv, vh, j);
       }
     }
     // after a stop, wait (bounded) for the copies still in flight before leaving
     if (sm.err) {
       int tries = 0;
-      for (int i = max(it - kSlots, 0); i < it; ++i)
-        while (!mbar_wait(&sm.kv_full[i % kSlots], (i / kSlots) & 1, kTryNs) && ++tries < kTries) {
+      for (int s = 0; s < kSlots; ++s) {  // its last use: in this round, or in the one before
+        const uint32_t r = s < slot ? round : round - 1;
+        while ((s < slot || round > 0) && !mbar_wait(&sm.kv_full[s], r & 1, kTryNs) && ++tries < kTries) {
         }
+      }
       for (int t = 0; t < 2; ++t)
         while (q_uses[t] > 0 && !mbar_wait(&sm.q_full[t], (q_uses[t] - 1) & 1, kTryNs) && ++tries < kTries) {
         }
     }
-  } else if (warp == 8) {
-    // ---- the products -------------------------------------------------------------------
+  } else if (warp == 8 || warp == 10) {
+    // ---- the products of a tile -------------------------------------------------------------------
     constexpr uint32_t id_s = idesc16<T>(128, kKeys, false), id_o = idesc16<T>(128, D, true);
     const uint64_t dq0 = tc::desc_sw128(smem_addr(sm.q[0])), dk0 = tc::desc_sw128(smem_addr(sm.kv[0]));
     const uint64_t dv0 = desc_mn_sw128(smem_addr(sm.kv[0]), kHalf);
     const uint32_t leader = elect_one();
-    int it = 0;                       // ring slots taken so far
-    uint32_t q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
-    bool ok = true;
-    for (int k = 0; ok; ++k) {
+    const int t = uniform((warp - 8) >> 1);
+    const uint32_t ts = tbase + Shape::kS + kKeys * t, tp = tbase + Shape::kP + kKeys / 2 * t, to_ = tbase + Shape::kO + D * t;
+    const uint64_t dq = tc::desc_advance(dq0, t * (128 * D * 2));
+    // the ring's next slot and the parity of its phase; K(j + 1) and V(j) of a turn are
+    // neighbours in it, in that order
+    int slot = 0;
+    uint32_t ring = 0, p_ph = 0, s_ph = 1, q_ph = 0;  // (S is free before its first use)
+    auto next = [&]() {
+      if (++slot == kSlots) {
+        slot = 0;
+        ring ^= 1;
+      }
+    };
+    auto scores = [&]() {  // S = Q K^T, once the softmax has taken the last one out
+      wait_for(&sm.s_free[t], s_ph, &sm.err, dead);
+      s_ph ^= 1;
+      tc::fence_after_sync();
+      const uint64_t dk = tc::desc_advance(dk0, slot * kTileBytes);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        mma_ss(leader, ts, tc::desc_advance(dq, (kk >> 2) * kQHalf + (kk & 3) * 32),
+               tc::desc_advance(dk, (kk >> 2) * kHalf + (kk & 3) * 32), id_s, kk != 0);
+      commit(leader, &sm.s_full[t]);
+    };
+#pragma unroll 1
+    for (int k = 0; !dead; ++k) {
       const int st = k & 1;
-      if (!wait_warp(&sm.info_full[st], (k >> 1) & 1, &sm.err)) break;
-      const int nt[2] = {sm.piece[st].n[0], sm.piece[st].n[1]}, k0 = sm.piece[st].k0, len = sm.piece[st].len;
-      const bool stop = sm.piece[st].b < 0;
+      wait_for(&sm.info_full[st], (k >> 1) & 1, &sm.err, dead);
+      // (uniform by construction: loop counts and ring slots feed the MMAs' descriptors)
+      const int n = uniform(max(sm.piece[st].n[0], sm.piece[st].n[1])), mine_n = uniform(sm.piece[st].n[t]);
+      const int left = uniform(sm.piece[st].len) - uniform(sm.piece[st].k0) * kKeys;  // keys from the first tile on
+      const bool stop = uniform(sm.piece[st].b) < 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.info_empty[st]);
-      if (stop) break;
-      const int n = max(nt[0], nt[1]);
-      if (n == 0) continue;
-      auto slot_k = [&](int j) { return it + (j == 0 ? 0 : 2 * j - 1); };              // K0 K1 V0 K2 V1 ...
-      auto slot_v = [&](int j) { return it + (j + 1 < n ? 2 * j + 2 : 2 * n - 1); };
-      auto scores = [&](int t, int j) -> bool {  // S of tile t
-        const int i = slot_k(j), s = i % kSlots;
-        if (j == 0) {
-          if (!wait_warp(&sm.q_full[t], q_ph[t], &sm.err)) return false;
-          q_ph[t] ^= 1;
+      if (stop || dead) break;
+      if (mine_n > 0) {
+        wait_for(&sm.q_full[t], q_ph, &sm.err, dead);
+        q_ph ^= 1;
+      }
+      // every K and V tile is released by both tiles' warps, by those too that have no use for it
+#pragma unroll 1
+      for (int j = -1; j < n; ++j) {
+        if (j + 1 < n) {  // K(j + 1)
+          wait_for(&sm.kv_full[slot], ring, &sm.err, dead);
+          if (j + 1 < mine_n) scores();
+          commit(leader, &sm.kv_empty[slot]);
+          if (j + 2 == mine_n) commit(leader, &sm.q_empty[t]);
+          next();
         }
-        if (!wait_warp(&sm.kv_full[s], (i / kSlots) & 1, &sm.err)) return false;
-        tc::fence_after_sync();
-        const uint64_t dq = tc::desc_advance(dq0, t * kTileBytes), dk = tc::desc_advance(dk0, s * kTileBytes);
+        if (j >= 0) {  // V(j)
+          wait_for(&sm.kv_full[slot], ring, &sm.err, dead);
+          if (j < mine_n) {
+            const int valid = left - j * kKeys;
+            if (valid < kKeys) {  // rows past the last key: whatever lies there, P = 0 must give 0 (both warps clear them)
+              const int chunks = (kKeys - valid) * 8;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kHalf + (kk & 3) * 32;
-          mma_ss(leader, tbase + 128 * t, tc::desc_advance(dq, off), tc::desc_advance(dk, off), id_s, kk != 0);
-        }
-        commit(leader, &sm.s_full[t]);
-        if (j + 1 == nt[t]) commit(leader, &sm.q_empty[t]);
-        return true;
-      };
-      for (int t = 0; t < 2 && ok; ++t)
-        if (nt[t] > 0) ok = scores(t, 0);
-      if (ok) commit(leader, &sm.kv_empty[slot_k(0) % kSlots]);
-      for (int j = 0; j < n && ok; ++j) {
-        const int i = slot_v(j), s = i % kSlots;
-        if (!wait_warp(&sm.kv_full[s], (i / kSlots) & 1, &sm.err)) {
-          ok = false;
-          break;
-        }
-        const int valid = len - (k0 + j) * kKeys;
-        if (valid < kKeys) {  // rows past the last key: whatever lies there, P = 0 must give 0
-          const int chunks = (kKeys - valid) * 8;
+              for (int d = 0; d < D / 64; ++d)
+                for (int c = lane; c < chunks; c += 32)
+                  reinterpret_cast<uint4*>(sm.kv[slot] + d * kHalf + valid * 128)[c] = make_uint4(0, 0, 0, 0);
+              fence_proxy_async_shared();
+              __syncwarp();
+            }
+            wait_for(&sm.p_full[t], p_ph, &sm.err, dead);
+            p_ph ^= 1;
+            tc::fence_after_sync();
+            const uint64_t dv = tc::desc_advance(dv0, slot * kTileBytes);
 #pragma unroll
-          for (int d = 0; d < D / 64; ++d)
-            for (int c = lane; c < chunks; c += 32)
-              reinterpret_cast<uint4*>(sm.kv[s] + d * kHalf + valid * 128)[c] = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_shared();
-          __syncwarp();
-        }
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (j >= nt[t]) continue;
-          const uint64_t dv = tc::desc_advance(dv0, s * kTileBytes);
-          if (!(ok = wait_warp(&sm.p_part[t], p_ph[t], &sm.err))) break;
-          tc::fence_after_sync();
-#pragma unroll
-          for (int kk = 0; kk < kFirstKeys / 16; ++kk)
-            mma_ts(leader, tbase + 256 + 128 * t, tbase + 128 * t + 8 * kk, tc::desc_advance(dv, kk * 2048), id_o,
-                   (j | kk) != 0);
-          if (!(ok = wait_warp(&sm.p_full[t], p_ph[t], &sm.err))) break;
-          p_ph[t] ^= 1;
-          tc::fence_after_sync();
-#pragma unroll
-          for (int kk = kFirstKeys / 16; kk < kKeys / 16; ++kk)
-            mma_ts(leader, tbase + 256 + 128 * t, tbase + 128 * t + 8 * kk, tc::desc_advance(dv, kk * 2048), id_o, 1u);
-          if (j + 1 < nt[t]) ok = scores(t, j + 1);  // its commit covers O as well: S(j + 1) seen means PV(j) done
-          else commit(leader, &sm.o_full[t]);
-        }
-        if (ok) {
-          commit(leader, &sm.kv_empty[s]);
-          if (j + 1 < n) commit(leader, &sm.kv_empty[slot_k(j + 1) % kSlots]);
+            for (int kk = 0; kk < kKeys / 16; ++kk)  // O (+)= P V
+              mma_ts(leader, to_, tp + 8 * kk, tc::desc_advance(dv, kk * 2048), id_o, (j | kk) != 0);
+            commit(leader, &sm.o_done[t]);
+          }
+          commit(leader, &sm.kv_empty[slot]);
+          next();
         }
       }
-      it += 2 * n;
     }
   }
   } else {
@@ -655,22 +699,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int t = warp >> 2;                 // tile
     const int row_in = threadIdx.x & 127;    // row of the tile = TMEM lane
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-    const uint32_t t_s = tbase + lanes + 128 * t, t_o = tbase + lanes + 256 + 128 * t;
+    const uint32_t t_s = tbase + lanes + Shape::kS + kKeys * t, t_p = tbase + lanes + Shape::kP + kKeys / 2 * t;
+    const uint32_t t_o = tbase + lanes + Shape::kO + D * t;
     const float sl2 = g.sl2;
     uint32_t s_ph = 0, o_ph = 0;
     const int tok_in = row_in * g.group_mul >> 16, head_in = row_in - tok_in * g.group;
-    bool ok = true;
     uint32_t t_ph = 0;
-    auto tile_sync = [&]() -> bool {         // a barrier of the tile's warps, bounded like every wait
+    auto tile_sync = [&]() {                 // a barrier of the tile's warps
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.tile_bar[t]);
-      const bool r = wait_warp(&sm.tile_bar[t], t_ph, &sm.err);
+      wait_for(&sm.tile_bar[t], t_ph, &sm.err, dead);
       t_ph ^= 1;
-      return r;
     };
-    for (int k = 0; ok; ++k) {
+#pragma unroll 1
+    for (int k = 0; !dead; ++k) {
       const int st = k & 1;
-      if (!wait_warp(&sm.info_full[st], (k >> 1) & 1, &sm.err)) break;
+      wait_for(&sm.info_full[st], (k >> 1) & 1, &sm.err, dead);
       const Piece p = sm.piece[st];
       auto release = [&]() {
         __syncwarp();
@@ -688,40 +732,60 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int lim = lim0 + tok_in;                                 // ... and this row
       float m = -INFINITY;                                           // in units of log2
       uint64_t l2 = 0;                                               // two partial sums
+#pragma unroll 1
       for (int j = 0; j < n; ++j) {
-        if (!(ok = wait_warp(&sm.s_full[t], s_ph, &sm.err))) break;
+        wait_for(&sm.s_full[t], s_ph, &sm.err, dead);
         s_ph ^= 1;
         tc::fence_after_sync();
-        uint32_t sr[4][32];
+        uint32_t sr[kKeys];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tc::tmem_ld32_nowait(t_s + 32 * c, sr[c]);
-        tc::tmem_wait_ld<true>(sr[0]);
-        tc::tmem_wait_ld<false>(sr[1]);
-        tc::tmem_wait_ld<false>(sr[2]);
-        tc::tmem_wait_ld<false>(sr[3]);
+        for (int c = 0; c < kKeys / 16; ++c) tmem_ld16(t_s + 16 * c, sr + 16 * c);
+        tmem_wait_ld(sr);
+#pragma unroll
+        for (int c = 1; c < kKeys / 16; ++c) pin16(sr + 16 * c);
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.s_free[t]);
         const int key0 = (p.k0 + j) * kKeys;
-        const bool masked = key0 + kKeys - 1 > lim0;  // some row of the tile does not see all of these keys
-        if (masked) {
+        if (key0 + kKeys - 1 > lim0) {  // some row of the tile does not see all of these keys
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (key0 + i > lim) sr[i >> 5][i & 31] = 0xff800000u;
+          for (int i = 0; i < kKeys; ++i)
+            if (key0 + i > lim) sr[i] = 0xff800000u;
         }
         float mx;
         {
-          float x4[4];
+          float x4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) x4[c] = max_nan(__uint_as_float(sr[c][0]), __uint_as_float(sr[c][1]));
-#pragma unroll
-          for (int i = 2; i < 32; i += 2)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) x4[c] = max3(x4[c], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
-          mx = live ? max_nan(max_nan(x4[0], x4[1]), max_nan(x4[2], x4[3])) * sl2 : -INFINITY;
+          for (int i = 0; i < kKeys; i += 2)
+            x4[(i >> 1) & 3] = max3(x4[(i >> 1) & 3], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
+          mx = live ? fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])) * sl2 : -INFINITY;
         }
-        if (__any_sync(0xffffffffu, !(mx <= m + 8.f) && mx != -INFINITY)) {  // (also the first tile: m = -inf)
-          const float mn = max_nan(m, mx);
-          const float sc = mn == -INFINITY ? 0.f : ex2_approx(m - mn);
-          const uint64_t sc2 = pack2(sc, sc);
-          if (j > 0) {  // S(j) is there, so PV(j - 1) is done and O can be rescaled
+        const bool moves = __any_sync(0xffffffffu, mx > m + 8.f);  // (also the first tile: m = -inf)
+        float sc = 1.f;
+        if (moves) {
+          const float mn = fmaxf(m, mx);
+          sc = mn == -INFINITY ? 0.f : ex2_approx(m - mn);
+          l2 = fma2(l2, pack2(sc, sc), 0);
+          m = mn;
+        }
+        // an infinite maximum leaves no weights (inf - inf); none at all, weights of 0
+        const float ref = m == -INFINITY ? 0.f : -m;
+        const uint64_t ref2 = pack2(ref, ref), sl22 = pack2(sl2, sl2);
+        uint64_t la = 0, lb = 0;
+        uint32_t pw[kKeys / 2];
+#pragma unroll
+        for (int i = 0; i < kKeys / 2; ++i) {
+          const float2 x = unpack2(fma2(pack2(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), sl22, ref2));
+          const float e0 = ex2_approx(x.x), e1 = ex2_approx(x.y);
+          if (i & 1) lb = add2(lb, pack2(e0, e1));
+          else la = add2(la, pack2(e0, e1));
+          pw[i] = Pair<T>::put(e0, e1);
+        }
+        if (j > 0) {  // the product before has read P, and O may be rescaled
+          wait_for(&sm.o_done[t], o_ph, &sm.err, dead);
+          o_ph ^= 1;
+          if (moves) {
+            tc::fence_after_sync();
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               float o[32];
@@ -731,41 +795,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tc::tmem_st32(t_o + 32 * c, o);
             }
           }
-          l2 = fma2(l2, sc2, 0);
-          m = mn;
         }
-        // an infinite maximum leaves no weights (inf - inf); none at all, weights of 0
-        const float ref = m == -INFINITY ? 0.f : m == INFINITY ? NAN : -m;
-        const uint64_t ref2 = pack2(ref, ref), sl22 = pack2(sl2, sl2);
-        uint64_t la = 0, lb = 0;
-        auto arrive = [&](uint64_t* bar) {
-          tmem_wait_st();
-          tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar);
-        };
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pw[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 x = unpack2(fma2(pack2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), sl22, ref2));
-            const float e0 = ex2_approx(x.x), e1 = ex2_approx(x.y);
-            if (i & 1) lb = add2(lb, pack2(e0, e1));
-            else la = add2(la, pack2(e0, e1));
-            pw[i] = Pair<T>::put(e0, e1);
-          }
-          tmem_st16(t_s + 16 * c, pw);
-          if (32 * (c + 1) == kFirstKeys) arrive(&sm.p_part[t]);
-        }
-        arrive(&sm.p_full[t]);
+        for (int c = 0; c < kKeys / 16; ++c) tmem_st8(t_p + 8 * c, pw + 8 * c);
+        tmem_wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[t]);
         l2 = add2(l2, add2(la, lb));
       }
-      if (!ok) break;
       const float2 lf = unpack2(l2);
       float l = lf.x + lf.y;
       if (n > 0) {
-        if (!(ok = wait_warp(&sm.o_full[t], o_ph, &sm.err))) break;
+        wait_for(&sm.o_done[t], o_ph, &sm.err, dead);
         o_ph ^= 1;
         tc::fence_after_sync();
       }
@@ -874,12 +916,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (lane == 0) g.stat[slot * kRows + 128 * t + rt] = make_float2(ms, ls);
         });
         __threadfence();
-        if (!(ok = tile_sync())) break;
+        tile_sync();
         if (threadIdx.x % 128 == 0)
           *reinterpret_cast<volatile int*>(&sm.last[t]) =
               atomicInc(g.counters + 2 * static_cast<size_t>(p.slot) + t, p.splits - 1) ==
               static_cast<uint32_t>(p.splits - 1);
-        if (!(ok = tile_sync())) break;
+        tile_sync();
         if (*reinterpret_cast<volatile int*>(&sm.last[t]) != 0) {
           __threadfence();
           const float2* stat = g.stat + static_cast<size_t>(p.slot) * kRows + at;
@@ -1004,7 +1046,6 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   g.span_mul = static_cast<unsigned>((1ull << 32) / (2 * g.tile_tokens) + 1);
   g.k_head = a.k_stride[1] != 0;
   g.v_head = a.v_stride[1] != 0;
-  g.box = kPaged && a.page_size < kKeys ? a.page_size : kKeys;
   g.slots = static_cast<int>(tc_slots(a));
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   if (ws == nullptr) return cudaErrorInvalidValue;
@@ -1026,7 +1067,10 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
       if ((e = map_rows(&mo, a.dtype, a.out, D, 2, dims, os, obox)) != cudaSuccess) return e;
     }
   }
-  const uint32_t kbox[3] = {static_cast<uint32_t>(kPaged ? (a.page_size < kKeys ? a.page_size : kKeys) : kKeys), 1, 1};
+  constexpr int kKeys = TcShape<D>::kKeys;
+  // the largest part of a page that tiles of kKeys keys are made of
+  g.box = !kPaged ? kKeys : kKeys % 128 != 0 ? 16 : a.page_size < kKeys ? a.page_size : kKeys;
+  const uint32_t kbox[3] = {static_cast<uint32_t>(g.box), 1, 1};
   const void *kb = a.k, *vb = a.v;
   if (kPaged && a.pages == 0) kb = vb = a.q;  // an empty pool is never read: any address will do
   if (kPaged) {
