@@ -6,8 +6,9 @@
 // A KV head's queries are rows: row r of a tile is token r / G, query head r % G of the
 // G that share the KV head, so that one pass over the keys serves all of them; a tile
 // holds the 128 / G tokens that fill (nearly) 128 rows. A CTA takes two tiles (A and B)
-// of one request and KV head and walks its keys a tile of 80 (heads of 128) or 128
-// (heads of 64) at a time:
+// of one request and KV head and walks its keys 128 at a time; where there are rows for
+// one only, A takes them with the even and B with the odd tiles of keys, and A adds the
+// two up in the end:
 //
 //   warp 9      which piece of work comes next; its Q, K and V tiles by TMA (128-byte
 //               swizzle; K and V through a ring, pages are boxes of page_size rows)
@@ -17,12 +18,10 @@
 //   warps 0-3   softmax of tile A, a thread per row: S out of tensor memory, running
 //   warps 4-7   maximum and sum in FP32 registers, P into tensor memory; tile B
 //
-// Tensor memory holds S, P and O of both tiles, each at columns of its own: 2 (80 + 40 +
-// 128) = 496 of 512, which is what makes a tile 80 keys. A softmax warp frees S as soon
-// as it has it in registers, so the tensor core has the next scores done while this
-// tile's weights are computed; with P in S's columns (tiles of 128 keys) every tile
-// waited for the two products in turn, 3,580 cycles a pair of 128 x 128 tiles where the
-// products take 2,048.
+// While one tile's softmax runs, the tensor core works on the other's products. (P in
+// columns of its own, so that the next S need not wait for it, leaves room for 80 keys a
+// tile only; both tiles' softmax then run at once and hold each other up: 2,330 cycles a
+// pair of 128 x 80 tiles.)
 //
 // The running maximum that P is relative to moves only when a row's grows by more than 8
 // (a factor 256): O, in tensor memory, is then rescaled by the softmax warps; between
@@ -53,9 +52,10 @@ constexpr int kTcThreads = 384;
 // Registers of a thread: the launch's 168 are shared out again, to the softmax warps
 // that hold 128 scores a thread (2 x 128 x 208 + 128 x 88 = 384 x 168).
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
-constexpr int kRows = 256;                // rows of a piece (two tiles)
-constexpr int kQHalf = 128 * 128;         // 16 KB: 128 rows x 64 values, 128-byte swizzle
-constexpr int kMinSplit = 8;              // key tiles below which rows are not split
+constexpr int kRows = 256, kKeys = 128;   // rows of a piece (two tiles), keys of a tile
+constexpr int kFirstKeys = 96;            // of a tile's weights, what the second product starts on
+constexpr int kHalf = 128 * 128;          // 16 KB: 128 rows x 64 values, 128-byte swizzle
+constexpr int kMinSplit = 6;              // key tiles below which rows are not split
 constexpr int kSortBatch = 128;           // requests up to which pieces are taken longest first
 constexpr int kTryNs = 20000, kTries = 50000;  // bound of every wait: about a second
 
@@ -65,37 +65,38 @@ struct Piece {
   int first;        // the request's first packed token
   int tok0, toks;   // the piece's tokens
   int ctx, len;     // keys before the new tokens, all keys
-  int k0;           // first key tile
-  int n[2];         // key tiles of tiles A and B
+  int k0, total;    // first key tile, how many
+  int n[2];         // those of tiles A and B
+  int halves;       // A and B have the same rows, and every other key tile
   int splits, split, slot;
   int bad;
 };
 
 template <int D>
 struct TcShape {
-  static constexpr int kKeys = D == 128 ? 80 : 128;     // of a tile
-  static constexpr int kSlots = D == 128 ? 6 : 7;       // K and V tiles in flight
+  static constexpr int kSlots = D == 128 ? 4 : 8;       // K and V tiles in flight
   static constexpr int kTileBytes = kKeys * D * 2;
-  static constexpr int kTileHalf = kKeys * 128;         // 64 values of every key
-  // tensor memory columns
-  static constexpr uint32_t kS = 0, kP = 2 * kKeys, kO = 512 - 2 * D;
-  static_assert(3 * kKeys <= 512 - 2 * D, "tensor memory");
+  // tensor memory columns: S of tile t at 128 t (P over its first half), O from kO on
+  static constexpr uint32_t kO = 512 - 2 * D;
 };
 
 template <int D>
 struct TcSmem {
   using Shape = TcShape<D>;
-  uint8_t q[2][128 * D * 2];
+  uint8_t q[2][Shape::kTileBytes];
   uint8_t kv[Shape::kSlots][Shape::kTileBytes];
   uint8_t stage[8][32 * 128];                           // a warp's 32 rows x 64 values on their way out
   uint64_t kv_full[Shape::kSlots], kv_empty[Shape::kSlots];
-  uint64_t q_full[2], q_empty[2], s_full[2], s_free[2], p_full[2], o_done[2];
+  uint64_t q_full[2], q_empty[2], s_full[2], p_part[2], p_full[2], o_full[2];
   uint64_t info_full[2], info_empty[2];
   uint64_t tile_bar[2];   // the four softmax warps of a tile
+  uint64_t pair_full, pair_empty;
+  float2 pair[128];       // maximum and sum of B's rows, where they are A's too
   Piece piece[2];
   uint32_t tmem_base;
   int err;
   int last[2];
+  int turn;               // turns of A's products issued so far
 };
 
 struct TcArgs {
@@ -120,18 +121,16 @@ struct TcArgs {
 // (Short on purpose: the loops of the softmax warps fill the instruction caches, and what
 // the other warps run between two MMAs is fetched anew every time.)
 __device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t ph, int* err, bool& dead) {
-  if (!mbar_test(bar, ph) && !dead) {
-    int i = 0;
+  if (__all_sync(0xffffffffu, mbar_test(bar, ph)) || dead) return;
 #pragma unroll 1
-    while (!mbar_wait(bar, ph, kTryNs)) {
-      if (++i > kTries || *reinterpret_cast<volatile int*>(err) != 0) {
-        *reinterpret_cast<volatile int*>(err) = 1;
-        dead = true;
-        break;
-      }
+  for (int i = 0; !__all_sync(0xffffffffu, mbar_wait(bar, ph, kTryNs)); ++i) {
+    const bool other = *reinterpret_cast<volatile int*>(err) != 0;
+    if (__any_sync(0xffffffffu, i > kTries || other)) {
+      *reinterpret_cast<volatile int*>(err) = 1;
+      dead = true;
+      return;
     }
   }
-  dead = __any_sync(0xffffffffu, dead);
 }
 
 __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
@@ -224,10 +223,13 @@ __device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
       ::"r"(smem_addr(bar)), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t v[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]),
-               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t v[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
 }
 // 16 columns of this thread's lane; valid after tmem_wait_ld, which takes the first of
 // several such loads (the others go through pin16, so that no use moves before it)
@@ -289,7 +291,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 struct Load {
   int first, q, len, ctx, blocks, tiles, splits, bad;
 };
-template <int kKeys, bool kPaged>
+template <bool kPaged>
 __device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
   const Request rq = request_rows(g.a.cu_q, b, g.a.q_len, g.a.tokens);
   Load l;
@@ -305,13 +307,11 @@ __device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
   return l;
 }
 // key tiles that the first `toks` tokens of the request see
-template <int kKeys>
 __device__ __forceinline__ int tiles_of(const Load& l, int toks) {
   const int keys = l.ctx + min(toks, l.q);
   return l.bad || keys <= 0 ? 0 : static_cast<int>((static_cast<unsigned>(keys) + kKeys - 1) / kKeys);
 }
 // how many of the request's blocks of `span` tokens see more than x key tiles (they come last)
-template <int kKeys>
 __device__ __forceinline__ int blocks_above(const Load& l, int span, unsigned span_mul, int x) {
   if (x < 0) return l.blocks;
   if (l.tiles <= x) return 0;
@@ -334,7 +334,7 @@ __device__ __noinline__ void slow_row(const TcArgs& g, const Piece& p, int token
   float m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-  for (int j = p.k0 * TcShape<D>::kKeys; j < keys; ++j) {
+  for (int j = p.k0 * kKeys; j < keys; ++j) {
     int64_t ko, vo;
     if (kPaged) {
       const int64_t page = a.block_table[p.b * a.table_stride + j / a.page_size], slot = j % a.page_size;
@@ -379,14 +379,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                    const __grid_constant__ TcArgs g) {
   using Smem = TcSmem<D>;
   using Shape = TcShape<D>;
-  constexpr int kKeys = Shape::kKeys, kSlots = Shape::kSlots, kTileBytes = Shape::kTileBytes, kHalf = Shape::kTileHalf;
+  constexpr int kSlots = Shape::kSlots, kTileBytes = Shape::kTileBytes;
   extern __shared__ uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const mkb_attn_args& a = g.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // a lane of the loading warp keeps its first request; the others are read again in every pass
   Load mine = {};
-  if (warp == 9 && lane < a.batch) mine = load_of<kKeys, kPaged>(g, lane);
+  if (warp == 9 && lane < a.batch) mine = load_of<kPaged>(g, lane);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&sm.kv_full[s], 1);
@@ -396,14 +396,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&sm.q_full[t], 1);
       mbar_init(&sm.q_empty[t], 1);
       mbar_init(&sm.s_full[t], 1);
-      mbar_init(&sm.s_free[t], 4);
+      mbar_init(&sm.p_part[t], 4);
       mbar_init(&sm.p_full[t], 4);
-      mbar_init(&sm.o_done[t], 1);
+      mbar_init(&sm.o_full[t], 1);
       mbar_init(&sm.info_full[t], 1);
       mbar_init(&sm.tile_bar[t], 4);
       mbar_init(&sm.info_empty[t], 10);  // eight softmax warps, two MMA warps
     }
-    sm.err = 0;
+    mbar_init(&sm.pair_full, 4);
+    mbar_init(&sm.pair_empty, 4);
+    sm.err = sm.turn = 0;
     fence_mbar_init();
   }
   if (warp == 8) {
@@ -428,13 +430,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc::prefetch_tensormap(&tq);
     }
     const int kv_heads = a.kv_heads, grid = gridDim.x, span = 2 * g.tile_tokens;
-    auto request = [&](int b) { return b < 32 ? mine : load_of<kKeys, kPaged>(g, b); };
+    auto request = [&](int b) { return b < 32 ? mine : load_of<kPaged>(g, b); };
     // a fair share of the key tiles; rows with more are split
     long long total = 0;
     int top = 0;
     for (int b = lane; b < a.batch; b += 32) {
       const Load l = request(b);
-      total += static_cast<long long>(tiles_of<kKeys>(l, span) + l.tiles) * l.blocks;  // twice the sum: linear in the block
+      total += static_cast<long long>(tiles_of(l, span) + l.tiles) * l.blocks;  // twice the sum: linear in the block
       top = max(top, l.tiles);
     }
 #pragma unroll
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int b = lane; b < a.batch; b += 32) {
         const Load l = request(b);
         const int sp = splits_of(l);
-        n += blocks_above<kKeys>(l, span, g.span_mul, x * sp) * sp;
+        n += blocks_above(l, span, g.span_mul, x * sp) * sp;
       }
       return __reduce_add_sync(0xffffffffu, n) * kv_heads;
     };
@@ -483,8 +485,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           l = request(b);
           l.splits = splits_of(l);
           if (sorted) {
-            above = blocks_above<kKeys>(l, span, g.span_mul, lo * l.splits);
-            here = blocks_above<kKeys>(l, span, g.span_mul, lo * l.splits - l.splits) - above;
+            above = blocks_above(l, span, g.span_mul, lo * l.splits);
+            here = blocks_above(l, span, g.span_mul, lo * l.splits - l.splits) - above;
           } else {
             here = l.blocks;
           }
@@ -515,14 +517,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             p.ctx = l.ctx;
             p.tok0 = i * span;
             p.toks = min(l.q - p.tok0, span);
-            const int n = tiles_of<kKeys>(l, p.tok0 + p.toks), per = (n + l.splits - 1) / l.splits;
+            const int n = tiles_of(l, p.tok0 + p.toks), per = (n + l.splits - 1) / l.splits;
             p.k0 = min(p.split * per, n);
             const int k1 = min(p.k0 + per, n);
             p.splits = l.splits;
             p.slot = slot_base + sinc - slots + (i * kv_heads + p.hk) * l.splits;
             p.bad = l.bad;
-            p.n[0] = max(min(tiles_of<kKeys>(l, p.tok0 + min(p.toks, g.tile_tokens)), k1) - p.k0, 0);
-            p.n[1] = p.toks > g.tile_tokens ? k1 - p.k0 : 0;
+            p.total = k1 - p.k0;
+            p.halves = p.toks <= g.tile_tokens;
+            p.n[0] = p.halves ? (p.total + 1) / 2 : max(min(tiles_of(l, p.tok0 + g.tile_tokens), k1) - p.k0, 0);
+            p.n[1] = p.halves ? p.total / 2 : p.total;
             if (l.bad) report(a.status, MKB_SERVE_BAD_LENGTH);
           }
           const int src = __ffs(who) - 1;
@@ -542,7 +546,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       __syncwarp();
       if (p.b < 0) break;
       // K(0), then K(j + 1) and V(j): the order in which the products take them
-      const int n = max(p.n[0], p.n[1]);
+      const int n = p.total;
       auto load = [&](const CUtensorMap* map, int head, int j) {
         const int s = slot;
         if (round > 0) wait_for(&sm.kv_empty[s], (round - 1) & 1, &sm.err, dead);
@@ -589,7 +593,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           mbar_arrive_expect_tx(&sm.q_full[t], g.tile_tokens * g.group * D * 2);
 #pragma unroll
           for (int d = 0; d < D / 64; ++d)
-            tma_3d(sm.q[t] + d * kQHalf, &tq, 64 * d, p.hk * g.group, p.first + p.tok0 + t * g.tile_tokens, &sm.q_full[t]);
+            tma_3d(sm.q[t] + d * kHalf, &tq, 64 * d, p.hk * g.group, p.first + p.tok0 + (p.halves ? 0 : t * g.tile_tokens),
+                   &sm.q_full[t]);
         }
         __syncwarp();
       }
@@ -617,79 +622,110 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint64_t dv0 = desc_mn_sw128(smem_addr(sm.kv[0]), kHalf);
     const uint32_t leader = elect_one();
     const int t = uniform((warp - 8) >> 1);
-    const uint32_t ts = tbase + Shape::kS + kKeys * t, tp = tbase + Shape::kP + kKeys / 2 * t, to_ = tbase + Shape::kO + D * t;
-    const uint64_t dq = tc::desc_advance(dq0, t * (128 * D * 2));
+    const uint32_t ts = tbase + 128 * t, to_ = tbase + Shape::kO + D * t;
+    const uint64_t dq = tc::desc_advance(dq0, t * kTileBytes);
     // the ring's next slot and the parity of its phase; K(j + 1) and V(j) of a turn are
     // neighbours in it, in that order
-    int slot = 0;
-    uint32_t ring = 0, p_ph = 0, s_ph = 1, q_ph = 0;  // (S is free before its first use)
+    int slot = 0, turn = 0;
+    uint32_t ring = 0, p_ph = 0, q_ph = 0;
     auto next = [&]() {
       if (++slot == kSlots) {
         slot = 0;
         ring ^= 1;
       }
     };
-    auto scores = [&]() {  // S = Q K^T, once the softmax has taken the last one out
-      wait_for(&sm.s_free[t], s_ph, &sm.err, dead);
-      s_ph ^= 1;
-      tc::fence_after_sync();
-      const uint64_t dk = tc::desc_advance(dk0, slot * kTileBytes);
+    auto scores = [&](int s) {  // S = Q K^T (over the P that the last product has read: MMAs run in order)
+      const uint64_t dk = tc::desc_advance(dk0, s * kTileBytes);
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        mma_ss(leader, ts, tc::desc_advance(dq, (kk >> 2) * kQHalf + (kk & 3) * 32),
-               tc::desc_advance(dk, (kk >> 2) * kHalf + (kk & 3) * 32), id_s, kk != 0);
-      commit(leader, &sm.s_full[t]);
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off = (kk >> 2) * kHalf + (kk & 3) * 32;
+        mma_ss(leader, ts, tc::desc_advance(dq, off), tc::desc_advance(dk, off), id_s, kk != 0);
+      }
+      commit(leader, &sm.s_full[t]);  // covers O as well: S(j + 1) seen means PV(j) done
     };
 #pragma unroll 1
     for (int k = 0; !dead; ++k) {
       const int st = k & 1;
       wait_for(&sm.info_full[st], (k >> 1) & 1, &sm.err, dead);
       // (uniform by construction: loop counts and ring slots feed the MMAs' descriptors)
-      const int n = uniform(max(sm.piece[st].n[0], sm.piece[st].n[1])), mine_n = uniform(sm.piece[st].n[t]);
+      const int n = uniform(sm.piece[st].total), mine_n = uniform(sm.piece[st].n[t]);
+      const int step = uniform(sm.piece[st].halves) ? 2 : 1, from = step == 2 ? t : 0;  // its key tiles
+      const int last = from + step * (mine_n - 1);                                     // (below `from`: none)
       const int left = uniform(sm.piece[st].len) - uniform(sm.piece[st].k0) * kKeys;  // keys from the first tile on
       const bool stop = uniform(sm.piece[st].b) < 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.info_empty[st]);
       if (stop || dead) break;
+      if (n == 0) continue;
       if (mine_n > 0) {
         wait_for(&sm.q_full[t], q_ph, &sm.err, dead);
         q_ph ^= 1;
       }
+      wait_for(&sm.kv_full[slot], ring, &sm.err, dead);
+      int todo = from, done = from;  // the next tile of scores, of outputs
+      auto maybe_scores = [&](int j, int s) {
+        if (j != todo || j > last) return;
+        scores(s);
+        if (j == last) commit(leader, &sm.q_empty[t]);
+        todo += step;
+      };
+      maybe_scores(0, slot);
+      commit(leader, &sm.kv_empty[slot]);
+      next();
       // every K and V tile is released by both tiles' warps, by those too that have no use for it
 #pragma unroll 1
-      for (int j = -1; j < n; ++j) {
-        if (j + 1 < n) {  // K(j + 1)
-          wait_for(&sm.kv_full[slot], ring, &sm.err, dead);
-          if (j + 1 < mine_n) scores();
-          commit(leader, &sm.kv_empty[slot]);
-          if (j + 2 == mine_n) commit(leader, &sm.q_empty[t]);
+      for (int j = 0; j < n; ++j) {
+        const int sk = slot;
+        if (j + 1 < n) {
+          wait_for(&sm.kv_full[sk], ring, &sm.err, dead);  // K(j + 1)
           next();
         }
-        if (j >= 0) {  // V(j)
-          wait_for(&sm.kv_full[slot], ring, &sm.err, dead);
-          if (j < mine_n) {
-            const int valid = left - j * kKeys;
-            if (valid < kKeys) {  // rows past the last key: whatever lies there, P = 0 must give 0 (both warps clear them)
-              const int chunks = (kKeys - valid) * 8;
+        wait_for(&sm.kv_full[slot], ring, &sm.err, dead);  // V(j)
+        if (j == done && j <= last) {
+          const int valid = left - j * kKeys;
+          if (valid < kKeys) {  // rows past the last key: whatever lies there, P = 0 must give 0 (both warps clear them)
+            const int chunks = (kKeys - valid) * 8;
 #pragma unroll
-              for (int d = 0; d < D / 64; ++d)
-                for (int c = lane; c < chunks; c += 32)
-                  reinterpret_cast<uint4*>(sm.kv[slot] + d * kHalf + valid * 128)[c] = make_uint4(0, 0, 0, 0);
-              fence_proxy_async_shared();
-              __syncwarp();
-            }
-            wait_for(&sm.p_full[t], p_ph, &sm.err, dead);
-            p_ph ^= 1;
-            tc::fence_after_sync();
-            const uint64_t dv = tc::desc_advance(dv0, slot * kTileBytes);
-#pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)  // O (+)= P V
-              mma_ts(leader, to_, tp + 8 * kk, tc::desc_advance(dv, kk * 2048), id_o, (j | kk) != 0);
-            commit(leader, &sm.o_done[t]);
+            for (int d = 0; d < D / 64; ++d)
+              for (int c = lane; c < chunks; c += 32)
+                reinterpret_cast<uint4*>(sm.kv[slot] + d * kHalf + valid * 128)[c] = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_shared();
+            __syncwarp();
           }
-          commit(leader, &sm.kv_empty[slot]);
-          next();
+          const uint64_t dv = tc::desc_advance(dv0, slot * kTileBytes);
+          // B's products queue behind A's of the same turn: side by side they would end
+          // together, and both tiles' softmax run at once, on the same units (4,900 cycles
+          // a turn instead of 3,250)
+          if (t == 1 && step == 1) {
+            for (int i = 0; *reinterpret_cast<volatile int*>(&sm.turn) - turn <= 0 && !dead; ++i) {
+              __nanosleep(20);
+              if (i > kTries * (kTryNs / 20) || *reinterpret_cast<volatile int*>(&sm.err) != 0)
+                dead = *reinterpret_cast<volatile int*>(&sm.err) = 1;
+            }
+            dead = __any_sync(0xffffffffu, dead);
+          }
+          wait_for(&sm.p_part[t], p_ph, &sm.err, dead);
+          tc::fence_after_sync();
+#pragma unroll
+          for (int kk = 0; kk < kFirstKeys / 16; ++kk)  // O (+)= P V
+            mma_ts(leader, to_, ts + 8 * kk, tc::desc_advance(dv, kk * 2048), id_o, (j - from | kk) != 0);
+          wait_for(&sm.p_full[t], p_ph, &sm.err, dead);
+          p_ph ^= 1;
+          tc::fence_after_sync();
+#pragma unroll
+          for (int kk = kFirstKeys / 16; kk < kKeys / 16; ++kk)
+            mma_ts(leader, to_, ts + 8 * kk, tc::desc_advance(dv, kk * 2048), id_o, 1u);
+          if (j == last) commit(leader, &sm.o_full[t]);
+          done += step;
         }
+        commit(leader, &sm.kv_empty[slot]);
+        if (j + 1 < n) {
+          maybe_scores(j + 1, sk);
+          commit(leader, &sm.kv_empty[sk]);
+        }
+        ++turn;
+        if (t == 0 && lane == 0) *reinterpret_cast<volatile int*>(&sm.turn) = turn;
+        next();
       }
     }
   }
@@ -699,12 +735,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int t = warp >> 2;                 // tile
     const int row_in = threadIdx.x & 127;    // row of the tile = TMEM lane
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-    const uint32_t t_s = tbase + lanes + Shape::kS + kKeys * t, t_p = tbase + lanes + Shape::kP + kKeys / 2 * t;
-    const uint32_t t_o = tbase + lanes + Shape::kO + D * t;
+    const uint32_t t_s = tbase + lanes + 128 * t, t_o = tbase + lanes + Shape::kO + D * t;
     const float sl2 = g.sl2;
     uint32_t s_ph = 0, o_ph = 0;
-    const int tok_in = row_in * g.group_mul >> 16, head_in = row_in - tok_in * g.group;
-    uint32_t t_ph = 0;
+    const int tok_in = row_in * g.group_mul >> 16;
+    uint32_t t_ph = 0, pair_ph = 0;
     auto tile_sync = [&]() {                 // a barrier of the tile's warps
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.tile_bar[t]);
@@ -720,13 +755,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.info_empty[st]);
       };
-      if (p.b < 0 || p.toks <= g.tile_tokens * t) {
+      if (p.b < 0) {
         release();
-        if (p.b < 0) break;
-        continue;
+        break;
       }
       const int n = p.n[t];
-      const int tok_t = p.tok0 + g.tile_tokens * t;                  // the tile's first token
+      const int tok_t = p.tok0 + (p.halves ? 0 : g.tile_tokens * t); // the tile's first token
       const bool live = row_in < g.tile_tokens * g.group && tok_t + tok_in < p.tok0 + p.toks;
       const int lim0 = p.ctx + tok_t;                                // the last key its first row sees
       const int lim = lim0 + tok_in;                                 // ... and this row
@@ -743,10 +777,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_wait_ld(sr);
 #pragma unroll
         for (int c = 1; c < kKeys / 16; ++c) pin16(sr + 16 * c);
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.s_free[t]);
-        const int key0 = (p.k0 + j) * kKeys;
+        const int key0 = (p.k0 + (p.halves ? 2 * j + t : j)) * kKeys;
         if (key0 + kKeys - 1 > lim0) {  // some row of the tile does not see all of these keys
 #pragma unroll
           for (int i = 0; i < kKeys; ++i)
@@ -760,32 +791,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             x4[(i >> 1) & 3] = max3(x4[(i >> 1) & 3], __uint_as_float(sr[i]), __uint_as_float(sr[i + 1]));
           mx = live ? fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])) * sl2 : -INFINITY;
         }
-        const bool moves = __any_sync(0xffffffffu, mx > m + 8.f);  // (also the first tile: m = -inf)
-        float sc = 1.f;
-        if (moves) {
+        if (__any_sync(0xffffffffu, mx > m + 8.f)) {  // (also the first tile: m = -inf)
           const float mn = fmaxf(m, mx);
-          sc = mn == -INFINITY ? 0.f : ex2_approx(m - mn);
-          l2 = fma2(l2, pack2(sc, sc), 0);
-          m = mn;
-        }
-        // an infinite maximum leaves no weights (inf - inf); none at all, weights of 0
-        const float ref = m == -INFINITY ? 0.f : -m;
-        const uint64_t ref2 = pack2(ref, ref), sl22 = pack2(sl2, sl2);
-        uint64_t la = 0, lb = 0;
-        uint32_t pw[kKeys / 2];
-#pragma unroll
-        for (int i = 0; i < kKeys / 2; ++i) {
-          const float2 x = unpack2(fma2(pack2(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), sl22, ref2));
-          const float e0 = ex2_approx(x.x), e1 = ex2_approx(x.y);
-          if (i & 1) lb = add2(lb, pack2(e0, e1));
-          else la = add2(la, pack2(e0, e1));
-          pw[i] = Pair<T>::put(e0, e1);
-        }
-        if (j > 0) {  // the product before has read P, and O may be rescaled
-          wait_for(&sm.o_done[t], o_ph, &sm.err, dead);
-          o_ph ^= 1;
-          if (moves) {
-            tc::fence_after_sync();
+          const float sc = mn == -INFINITY ? 0.f : ex2_approx(m - mn);
+          if (j > 0) {  // S(j) is there, so PV(j - 1) is done and O can be rescaled
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               float o[32];
@@ -795,126 +804,201 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tc::tmem_st32(t_o + 32 * c, o);
             }
           }
+          l2 = fma2(l2, pack2(sc, sc), 0);
+          m = mn;
         }
+        // an infinite maximum leaves no weights (inf - inf); none at all, weights of 0
+        const float ref = m == -INFINITY ? 0.f : -m;
+        const uint64_t ref2 = pack2(ref, ref), sl22 = pack2(sl2, sl2);
+        uint64_t la = 0, lb = 0;
+        auto arrive = [&](uint64_t* bar) {
+          tmem_wait_st();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar);
+        };
 #pragma unroll
-        for (int c = 0; c < kKeys / 16; ++c) tmem_st8(t_p + 8 * c, pw + 8 * c);
-        tmem_wait_st();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[t]);
+        for (int c = 0; c < kKeys / 32; ++c) {
+          uint32_t pw[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t* x2 = sr + 32 * c + 2 * i;
+            const float2 x = unpack2(fma2(pack2(__uint_as_float(x2[0]), __uint_as_float(x2[1])), sl22, ref2));
+            const float e0 = ex2_approx(x.x), e1 = ex2_approx(x.y);
+            if (i & 1) lb = add2(lb, pack2(e0, e1));
+            else la = add2(la, pack2(e0, e1));
+            pw[i] = Pair<T>::put(e0, e1);
+            if (32 * c == kFirstKeys && i == 7) arrive(&sm.p_part[t]);  // its stores have had time to land
+          }
+          tmem_st16(t_s + 16 * c, pw);
+        }
+        arrive(&sm.p_full[t]);
         l2 = add2(l2, add2(la, lb));
       }
       const float2 lf = unpack2(l2);
       float l = lf.x + lf.y;
       if (n > 0) {
-        wait_for(&sm.o_done[t], o_ph, &sm.err, dead);
+        wait_for(&sm.o_full[t], o_ph, &sm.err, dead);
         o_ph ^= 1;
         tc::fence_after_sync();
       }
+      // B's rows are A's: A adds the two up, each relative to its own maximum
+      const bool pair = p.halves && p.n[1] > 0;
+      float own = 1.f, other = 0.f;  // the weights of the two
+      if (p.halves && t == 1) {
+        release();
+        if (pair) {
+          sm.pair[row_in] = make_float2(m, l);
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.pair_full);
+          wait_for(&sm.pair_empty, pair_ph, &sm.err, dead);  // until A has read O
+          pair_ph ^= 1;
+        }
+        continue;
+      }
+      if (pair) {
+        wait_for(&sm.pair_full, pair_ph, &sm.err, dead);
+        pair_ph ^= 1;
+        tc::fence_after_sync();
+        const float2 x = sm.pair[row_in];
+        const float mm = fmaxf(m, x.x), ref = mm == -INFINITY ? 0.f : mm;
+        own = ex2_approx(m - ref);
+        other = ex2_approx(x.x - ref);
+        l = l * own + x.y * other;
+        m = mm;
+      }
       const bool bad = *reinterpret_cast<volatile int*>(&sm.piece[st].bad) != 0;
       release();
-      const int k_end = min(p.len, (p.k0 + n) * kKeys);
+      const int k_end = min(p.len, (p.k0 + p.total) * kKeys);
       constexpr int kPer = D / 32;
       uint8_t* stage = sm.stage[warp];
-      // 64 values of every row of the warp to memory: by one TMA store where all 32 rows are
-      // whole tokens of the request, else 128 bytes of four rows at a time
+      // Rows on their way out, 32 values at a time (a small loop: this code is not in the
+      // instruction cache when a piece ends) and 64 to a store: by TMA where all 32 rows of
+      // the warp are whole tokens of the request, else 128 bytes of four rows at a time
       const int tok_w = tok_t + g.warp_tokens * (warp & 3);
       const bool whole = g.warp_tokens > 0 && tok_w + g.warp_tokens <= p.tok0 + p.toks;
-      auto emit = [&](int half, const float* o) {
-        if (lane == 0) tma_store_read();
-        __syncwarp();
+      auto emit = [&](int c, const uint32_t* w) {  // values 32 c .. + 31 of every row, packed
+        if ((c & 1) == 0) {
+          if (lane == 0) tma_store_read();
+          __syncwarp();
+        }
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = pack8<T>(o + 8 * c);
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * (c & 1) + i) ^ (lane & 7)) << 4)) =
+              make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        if ((c & 1) == 0) return;
         if (whole) {
           fence_proxy_async_shared();
           __syncwarp();
-          if (lane == 0) tma_store_3d(stage, &to, 64 * half, p.hk * g.group, p.first + tok_w);
+          if (lane == 0) tma_store_3d(stage, &to, 32 * (c - 1), p.hk * g.group, p.first + tok_w);
           return;
         }
         __syncwarp();
-#pragma unroll 2
+#pragma unroll 1
         for (int i = 0; i < 8; ++i) {
           const int r = 4 * i + (lane >> 3), rt = 32 * (warp & 3) + r;
           const int tok = rt * g.group_mul >> 16, head = p.hk * g.group + rt - tok * g.group;
           if (rt < g.tile_tokens * g.group && tok_t + tok < p.tok0 + p.toks)
             *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (p.first + tok_t + tok) * a.out_stride[0] +
-                                      head * a.out_stride[1] + 64 * half + 8 * (lane & 7)) =
+                                      head * a.out_stride[1] + 32 * (c - 1) + 8 * (lane & 7)) =
                 *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
         }
         __syncwarp();
       };
-      // the rows of the warp whose O is not finite, key by key
-      auto again = [&](bool odd, auto&& put) {
-        uint32_t todo = __ballot_sync(0xffffffffu, odd && live);
-        if (todo != 0) {
-          if (lane == 0) tma_store_done();
-          __syncwarp();
-        }
-        while (todo != 0) {
-          const int r = __ffs(todo) - 1, rt = 32 * (warp & 3) + r;
-          todo &= todo - 1;
-          const int tok = tok_t + (rt * g.group_mul >> 16), head = p.hk * g.group + rt - (rt * g.group_mul >> 16) * g.group;
-          float o[kPer], ms, ls;
-          slow_row<T, D, kPaged>(g, p, tok, head, k_end, o, &ms, &ls);
-          put(rt, tok, head, o, ms, ls);
-        }
-        __syncwarp();
-      };
-      float odd = 0.f;  // NaN once a value of O is not finite
-      if (p.splits == 1) {
-        const float inv = bad || m == -INFINITY ? NAN : 1.f / l;  // no weights: every score -inf
+      const bool split = p.splits > 1;
+      const int at = 128 * t + row_in;
+      const size_t slot = p.slot + p.split;
+      float4* part = g.part + slot * (D / 4) * kRows;
+      if (split && static_cast<size_t>(p.slot) + p.splits > static_cast<size_t>(g.slots)) continue;  // (cannot be: tc_slots)
+      uint64_t odd2 = 0;  // NaN once a value of O is not finite
+      // no weights at all (every score -inf) are no mean; a row that sees no key is zero
+      const bool zero = lim < 0 && !bad, zeros = __any_sync(0xffffffffu, zero);
+      const float inv = bad || m == -INFINITY ? NAN : 1.f / l;
+      const uint64_t inv2 = pack2(inv, inv), own2 = pack2(own, own), other2 = pack2(other, other);
 #pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
-          float o[64];
-          if (n > 0) {
-            tc::tmem_ld32(t_o + 64 * c, o);
-            tc::tmem_ld32(t_o + 64 * c + 32, o + 32);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) o[i] = 0.f;
-          }
-#pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            odd = fmaf(o[i], 0.f, odd);
-            o[i] = lim < 0 && !bad ? 0.f : o[i] * inv;
-          }
-          emit(c, o);
-        }
-        again(odd != 0.f && lim >= 0 && !bad, [&](int, int tok, int head, const float* o, float, float ls) {
-          uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (p.first + tok) * a.out_stride[0] +
-                                                      head * a.out_stride[1]) + lane * (kPer / 2);
-          const float f = 1.f / ls;
-#pragma unroll
-          for (int i = 0; i < kPer / 2; ++i) dst[i] = Pair<T>::put(o[2 * i] * f, o[2 * i + 1] * f);
-        });
-      } else if (static_cast<size_t>(p.slot) + p.splits <= static_cast<size_t>(g.slots)) {
-        // one of several ranges of keys: leave it for whoever comes last
-        const int at = 128 * t + row_in;
-        const size_t slot = p.slot + p.split;
-        float4* part = g.part + slot * (D / 4) * kRows;
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t x[32];
+        uint64_t o2[16];
         if (n > 0) {
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            float o[32];
-            tc::tmem_ld32(t_o + 32 * c, o);
+          tmem_ld16(t_o + 32 * c, x);
+          tmem_ld16(t_o + 32 * c + 16, x + 16);
+          tmem_wait_ld(x);
+          pin16(x + 16);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) odd = fmaf(o[i], 0.f, odd);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              part[(8 * c + i) * kRows + at] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          }
+          for (int i = 0; i < 32; ++i) x[i] = 0;
         }
-        g.stat[slot * kRows + at] = make_float2(m, bad ? NAN : l);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o2[i] = pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+        if (pair) {
+          tmem_ld16(t_o + D + 32 * c, x);
+          tmem_ld16(t_o + D + 32 * c + 16, x + 16);
+          tmem_wait_ld(x);
+          pin16(x + 16);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            o2[i] = fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), other2, fma2(o2[i], own2, 0));
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) odd2 = fma2(o2[i], 0, odd2);
+        if (split) {  // one of several ranges of keys: left for whoever comes last
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 u = unpack2(o2[2 * i]), v = unpack2(o2[2 * i + 1]);
+            part[(8 * c + i) * kRows + at] = make_float4(u.x, u.y, v.x, v.y);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 u = unpack2(fma2(o2[i], inv2, 0));
+            x[i] = Pair<T>::put(u.x, u.y);
+          }
+          if (zeros) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = zero ? 0 : x[i];
+          }
+          emit(c, x);
+        }
+      }
+      const float2 oddf = unpack2(odd2);
+      const float odd = oddf.x + oddf.y;
+      if (pair) {
+        tc::fence_before_sync();
         __syncwarp();
-        again(odd != 0.f && lim >= 0 && !bad, [&](int rt, int, int, const float* o, float ms, float ls) {
+        if (lane == 0) mbar_arrive(&sm.pair_empty);
+      }
+      if (split) g.stat[slot * kRows + at] = make_float2(m, bad ? NAN : l);
+      // the rows of the warp whose O is not finite, key by key
+      uint32_t todo = __ballot_sync(0xffffffffu, odd != 0.f && live && lim >= 0 && !bad);
+      if (todo != 0) {
+        if (lane == 0) tma_store_done();
+        __syncwarp();
+      }
+#pragma unroll 1
+      while (todo != 0) {
+        const int r = __ffs(todo) - 1, rt = 32 * (warp & 3) + r, tok = rt * g.group_mul >> 16;
+        const int head = p.hk * g.group + rt - tok * g.group;
+        todo &= todo - 1;
+        float o[kPer], ms, ls;
+        slow_row<T, D, kPaged>(g, p, tok_t + tok, head, k_end, o, &ms, &ls);
+        if (split) {
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
             const int d = lane * kPer + i;
             reinterpret_cast<float*>(part + (d / 4) * kRows + 128 * t + rt)[d % 4] = o[i];
           }
           if (lane == 0) g.stat[slot * kRows + 128 * t + rt] = make_float2(ms, ls);
-        });
+        } else {
+          uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (p.first + tok_t + tok) * a.out_stride[0] +
+                                                      head * a.out_stride[1]) + lane * (kPer / 2);
+          const float f = 1.f / ls;
+#pragma unroll
+          for (int i = 0; i < kPer / 2; ++i) dst[i] = Pair<T>::put(o[2 * i] * f, o[2 * i + 1] * f);
+        }
+      }
+      __syncwarp();
+      if (split) {
         __threadfence();
         tile_sync();
         if (threadIdx.x % 128 == 0)
@@ -932,20 +1016,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const float2 x = __ldcg(stat + s * kRows);
             ll += x.y * ex2_approx(x.x - ref);
           }
-          const float inv = lim < 0 ? 0.f : 1.f / ll;
+          const float f0 = 1.f / ll;
           const float4* part0 = g.part + static_cast<size_t>(p.slot) * (D / 4) * kRows + at;
 #pragma unroll 1
-          for (int c = 0; c < D / 64; ++c) {
-            float o[64];
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) o[i] = 0.f;
+            for (int i = 0; i < 32; ++i) o[i] = 0.f;
             for (int s = 0; s < p.splits; ++s) {
               const float w = __ldcg(stat + s * kRows).x;
               if (w == -INFINITY) continue;  // that range holds no key this row sees
               const float f = ex2_approx(w - ref);
-              const float4* x4 = part0 + (static_cast<size_t>(s) * (D / 4) + 16 * c) * kRows;
+              const float4* x4 = part0 + (static_cast<size_t>(s) * (D / 4) + 8 * c) * kRows;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
+              for (int i = 0; i < 8; ++i) {
                 const float4 x = __ldcg(x4 + i * kRows);
                 o[4 * i] += f * x.x;
                 o[4 * i + 1] += f * x.y;
@@ -953,9 +1037,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 o[4 * i + 3] += f * x.w;
               }
             }
+            uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) o[i] = lim < 0 ? 0.f : o[i] * inv;
-            emit(c, o);
+            for (int i = 0; i < 16; ++i) w[i] = lim < 0 ? 0 : Pair<T>::put(o[2 * i] * f0, o[2 * i + 1] * f0);
+            emit(c, w);
           }
         }
       }
@@ -1067,9 +1152,7 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
       if ((e = map_rows(&mo, a.dtype, a.out, D, 2, dims, os, obox)) != cudaSuccess) return e;
     }
   }
-  constexpr int kKeys = TcShape<D>::kKeys;
-  // the largest part of a page that tiles of kKeys keys are made of
-  g.box = !kPaged ? kKeys : kKeys % 128 != 0 ? 16 : a.page_size < kKeys ? a.page_size : kKeys;
+  g.box = kPaged && a.page_size < kKeys ? a.page_size : kKeys;
   const uint32_t kbox[3] = {static_cast<uint32_t>(g.box), 1, 1};
   const void *kb = a.k, *vb = a.v;
   if (kPaged && a.pages == 0) kb = vb = a.q;  // an empty pool is never read: any address will do
