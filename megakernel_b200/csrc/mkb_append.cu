@@ -31,6 +31,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const mkb_append
   const int d0 = 8 * part, d1 = D / 2 + 8 * part;
   const int rows = a.heads + 2 * a.kv_heads;
 
+  depend_launch();
+  depend_wait();
   const Request rq = request_at(a.cu_q, a.batch, a.q_len, a.tokens, t);
   const int b = rq.b, at = t - rq.first;
   const int pos = at >= 0 && at < rq.n ? a.kv_lens[b] - rq.n + at : -1;
@@ -132,9 +134,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const mkb_append
 
 template <typename S, typename T>
 cudaError_t append_dim(const mkb_append_args& a, cudaStream_t stream) {
-  if (a.head_dim == 128) append_kernel<S, T, 128><<<a.tokens, kAppendThreads, 0, stream>>>(a);
-  else append_kernel<S, T, 64><<<a.tokens, kAppendThreads, 0, stream>>>(a);
-  return cudaGetLastError();
+  if (a.head_dim == 128) return launch_early(append_kernel<S, T, 128>, a.tokens, kAppendThreads, 0, stream, a);
+  return launch_early(append_kernel<S, T, 64>, a.tokens, kAppendThreads, 0, stream, a);
 }
 template <typename T>
 cudaError_t append_source(const mkb_append_args& a, cudaStream_t stream) {

@@ -28,11 +28,12 @@
 // moves P stays below 2^8, which FP32 sums and 16-bit P hold without loss. P is rounded
 // to the operands' 16-bit type, as the output is: the same relative error.
 //
-// Work: a piece is (request, KV head, two tiles, a range of key tiles). Every CTA works
-// the list out for itself from the lengths, longest pieces first, and takes every
-// grid-th one, turning round after each sweep. Rows whose keys are more than a fair
-// share are split over several pieces; each writes its O, maximum and sum, and the last
-// to arrive adds them up in order of their keys, so results do not depend on timing.
+// Work: a piece is (request, KV head, two tiles); its weight is its keys and a fixed
+// part. The pieces' weights are laid end to end and cut into as many equal ranges as
+// there are CTAs; a cut inside a long enough piece splits its keys. Every part of a split
+// piece leaves its O, maximum and sum in memory, and the last part to be done adds them
+// up in order of their keys, so results do not depend on timing. Every CTA works its range
+// out for itself from the lengths: no list is written, nothing is asked of the host.
 //
 // Masked places: scores are replaced, not added to. V rows past the request's last key
 // are cleared in shared memory. V that is not finite and stands where some row of the
@@ -55,8 +56,10 @@ constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 constexpr int kRows = 256, kKeys = 128;   // rows of a piece (two tiles), keys of a tile
 constexpr int kFirstKeys = 96;            // of a tile's weights, what the second product starts on
 constexpr int kHalf = 128 * 128;          // 16 KB: 128 rows x 64 values, 128-byte swizzle
-constexpr int kMinSplit = 6;              // key tiles below which rows are not split
-constexpr int kSortBatch = 128;           // requests up to which pieces are taken longest first
+constexpr int kMinSplit = 6;              // key tiles of a piece below which it is not split
+constexpr int kMinPart = 2;               // key tiles of a part
+constexpr int kFixed = 256;               // a piece's fixed part, in keys (about what its start and end take)
+constexpr int kMinShare = 384;            // the least weight that is worth a CTA
 constexpr int kTryNs = 20000, kTries = 50000;  // bound of every wait: about a second
 
 struct Piece {
@@ -68,7 +71,8 @@ struct Piece {
   int k0, total;    // first key tile, how many
   int n[2];         // those of tiles A and B
   int halves;       // A and B have the same rows, and every other key tile
-  int splits, split, slot;
+  int splits, split;  // parts of the piece, and which this is
+  int cta0;           // the CTA of its first part
   int bad;
 };
 
@@ -104,15 +108,15 @@ struct TcArgs {
   float sl2;            // scale * log2(e)
   int group;            // query heads of a KV head
   int tile_tokens;      // tokens of a tile: 128 / group
-  int warp_tokens;      // tokens of a warp's 32 rows, 0 where they are not whole
-  unsigned span_mul;    // x / (2 tile_tokens) is x * span_mul >> 32, or one less
   int group_mul;        // r / group = r * group_mul >> 16 for r < 128
-  int k_head, v_head;   // 0 where every KV head lies at the same place (stride 0), else 1
+  int warp_tokens;      // tokens of a warp's 32 rows, 0 where they are not whole
   int box;              // keys of a TMA box
-  int slots;            // partial results the workspace holds
-  uint32_t* counters;   // [slots][2], zero between calls
-  float4* part;         // [slots][D / 4][256]
-  float2* stat;         // [slots][256]: maximum, sum
+  int k_head, v_head;   // 0 where every KV head lies at the same place (stride 0), else 1
+  // Parts of split pieces: a CTA has at most one that begins a piece (slot 2 cta + 1) and
+  // one that does not (slot 2 cta).
+  uint32_t* counters;   // [ctas][2], of the piece that the CTA begins, by tile; zero between calls
+  float4* part;         // [2 ctas][D / 4][256]
+  float2* stat;         // [2 ctas][256]: maximum, sum
 };
 
 // A warp's wait for a phase of a barrier. Bounded: each try suspends for 20 us at most.
@@ -285,11 +289,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// ---- the list of pieces, worked out by one warp -------------------------------------
+// ---- the pieces, worked out by one warp ------------------------------------------------
 
-// One request as the list sees it.
+// One request as the work sees it.
 struct Load {
-  int first, q, len, ctx, blocks, tiles, splits, bad;
+  int first, q, len, ctx, blocks, bad;
 };
 template <bool kPaged>
 __device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
@@ -302,8 +306,6 @@ __device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
   l.ctx = l.len - l.q;
   const unsigned span = 2 * g.tile_tokens;
   l.blocks = static_cast<int>((static_cast<unsigned>(l.q) + span - 1) / span);
-  l.tiles = l.bad || l.blocks == 0 ? 0 : static_cast<int>((static_cast<unsigned>(l.len) + kKeys - 1) / kKeys);
-  l.splits = 1;
   return l;
 }
 // key tiles that the first `toks` tokens of the request see
@@ -311,14 +313,29 @@ __device__ __forceinline__ int tiles_of(const Load& l, int toks) {
   const int keys = l.ctx + min(toks, l.q);
   return l.bad || keys <= 0 ? 0 : static_cast<int>((static_cast<unsigned>(keys) + kKeys - 1) / kKeys);
 }
-// how many of the request's blocks of `span` tokens see more than x key tiles (they come last)
-__device__ __forceinline__ int blocks_above(const Load& l, int span, unsigned span_mul, int x) {
-  if (x < 0) return l.blocks;
-  if (l.tiles <= x) return 0;
-  const int y = x * kKeys - l.ctx;  // the first token that sees more (x < tiles: no overflow)
-  int i = static_cast<int>(__umulhi(static_cast<unsigned>(y), span_mul));  // y / span, once it is positive
-  if (i * span > y) --i;
-  return y <= 0 ? l.blocks : l.blocks - i;
+// Weight of a request's blocks [0, i) of one KV head; block i weighs kFixed + the keys
+// before the request's new tokens + (i + 1) span, where there are rows for one tile (its
+// keys then take half the time) kFixed + half of them. (`even`: each block the same.)
+__device__ __forceinline__ int64_t weight_to(const Load& l, int span, bool even, int i) {
+  const int64_t n = i;
+  if (even) return n;
+  if (2 * l.q <= span) return n * (kFixed + (max(l.ctx, 0) + span) / 2);
+  return n * (kFixed + max(l.ctx, 0)) + span * (n * (n + 1) / 2);
+}
+// Where the work is cut: what lies before CTA c's range. (Any function that all CTAs
+// agree on and that grows with c would do.)
+__device__ __forceinline__ int64_t cut_at(int64_t total, int ctas, double per, int c) {
+  return c >= ctas ? total : static_cast<int64_t>(per * c);
+}
+// A cut `y` into a piece of weight `w` as a key tile of its `n`, short ends left out. The
+// tiles of a piece that is split weigh at most 256 each, a range at least kMinShare: two
+// cuts of one piece never fall together, except at its ends.
+__device__ __forceinline__ int cut_tile(int64_t y, int64_t w, int n) {
+  if (y <= 0) return 0;
+  if (y >= w) return n;
+  if (n < kMinSplit || w > 256 * static_cast<int64_t>(n)) return 2 * y >= w ? n : 0;
+  const int t = static_cast<int>(static_cast<float>(y) / static_cast<float>(w) * n + 0.5f);
+  return t < kMinPart ? 0 : t > n - kMinPart ? n : t;
 }
 
 // ---- one row, key by key: what a tile with values that are not finite comes to --------
@@ -384,9 +401,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const mkb_attn_args& a = g.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // a lane of the loading warp keeps its first request; the others are read again in every pass
-  Load mine = {};
-  if (warp == 9 && lane < a.batch) mine = load_of<kPaged>(g, lane);
+  depend_launch();
+  // (a lane of the loading warp keeps its first request; the others are read again in every pass)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&sm.kv_full[s], 1);
@@ -412,6 +428,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc::tmem_alloc(&sm.tmem_base, 512);
     tc::tmem_relinquish();
   }
+  depend_wait();  // what came before in the stream is done: its results may be read
+  Load mine = {};
+  if (warp == 9 && lane < a.batch) mine = load_of<kPaged>(g, lane);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -429,114 +448,114 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc::prefetch_tensormap(&tv);
       tc::prefetch_tensormap(&tq);
     }
-    const int kv_heads = a.kv_heads, grid = gridDim.x, span = 2 * g.tile_tokens;
-    auto request = [&](int b) { return b < 32 ? mine : load_of<kPaged>(g, b); };
-    // a fair share of the key tiles; rows with more are split
-    long long total = 0;
-    int top = 0;
+    const int kv_heads = a.kv_heads, span = 2 * g.tile_tokens;
+    auto request = [&](int b) { return b < 32 ? mine : load_of<kPaged>(g, b); };  // of lane b % 32
+    // all there is to do; pieces that are short and few have a CTA each
+    int64_t total = 0;
+    int pieces = 0, top = 0;
     for (int b = lane; b < a.batch; b += 32) {
       const Load l = request(b);
-      total += static_cast<long long>(tiles_of(l, span) + l.tiles) * l.blocks;  // twice the sum: linear in the block
-      top = max(top, l.tiles);
+      total += weight_to(l, span, false, l.blocks);
+      pieces += l.blocks;
+      top = max(top, l.blocks > 0 ? tiles_of(l, l.q) : 0);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    pieces = __reduce_add_sync(0xffffffffu, pieces) * kv_heads;
     top = __reduce_max_sync(0xffffffffu, top);
-    const float share = static_cast<float>(total) * kv_heads * (0.5f * 1.25f) / grid;
-    const int cap = max(kMinSplit, static_cast<int>(fminf(share, 1e9f)) + 1);
-    auto splits_of = [&](const Load& l) { return l.tiles > cap ? (l.tiles + cap - 1) / cap : 1; };
-    // pieces of more than x tiles, all requests
-    auto pieces_above = [&](int x) {
-      int n = 0;
-      for (int b = lane; b < a.batch; b += 32) {
-        const Load l = request(b);
-        const int sp = splits_of(l);
-        n += blocks_above(l, span, g.span_mul, x * sp) * sp;
+    const bool even = pieces <= static_cast<int>(gridDim.x) && top < kMinSplit;
+    total = even ? pieces : total * kv_heads;
+    const int ctas = even ? pieces : static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(total / kMinShare, static_cast<int64_t>(1))));
+    const double per = static_cast<double>(total) / ctas;
+    const int cta = blockIdx.x;
+    const bool work = cta < ctas && total > 0;
+    const int64_t from = cut_at(total, ctas, per, cta), to_end = cut_at(total, ctas, per, cta + 1);
+    // the piece that `from` falls into
+    Load l = {};
+    int b = a.batch, hk = 0, blk = 0;
+    int64_t pos = 0;  // what lies before it
+    for (int b0 = 0; b0 < a.batch && work; b0 += 32) {
+      const Load x = b0 + lane < a.batch ? request(b0 + lane) : Load{};
+      const int64_t w = weight_to(x, span, even, x.blocks) * kv_heads;
+      int64_t inc = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
       }
-      return __reduce_add_sync(0xffffffffu, n) * kv_heads;
-    };
-    // longest first, unless every piece has a CTA of its own (or the list is long: even anyway)
-    const bool sorted = a.batch <= kSortBatch && pieces_above(-1) > grid;
+      const uint32_t who = __ballot_sync(0xffffffffu, from - pos < inc);
+      if (who != 0) {
+        const int src = __ffs(who) - 1;
+        b = b0 + src;
+        l.first = __shfl_sync(0xffffffffu, x.first, src);
+        l.q = __shfl_sync(0xffffffffu, x.q, src);
+        l.len = __shfl_sync(0xffffffffu, x.len, src);
+        l.bad = __shfl_sync(0xffffffffu, x.bad, src);
+        l.blocks = __shfl_sync(0xffffffffu, x.blocks, src);
+        l.ctx = l.len - l.q;
+        pos += __shfl_sync(0xffffffffu, inc - w, src);
+        const int64_t head = weight_to(l, span, even, l.blocks);
+        hk = static_cast<int>(static_cast<float>(from - pos) / static_cast<float>(head));
+        hk = max(min(hk, kv_heads - 1), 0);
+        while (hk > 0 && head * hk > from - pos) --hk;
+        while (hk + 1 < kv_heads && head * (hk + 1) <= from - pos) ++hk;
+        pos += head * hk;
+        const float r = static_cast<float>(from - pos), c = kFixed + max(l.ctx, 0) + 0.5f * span;
+        blk = even ? static_cast<int>(from - pos) : static_cast<int>((sqrtf(c * c + 2.f * span * r) - c) / span);
+        blk = max(min(blk, l.blocks - 1), 0);
+        while (blk > 0 && weight_to(l, span, even, blk) > from - pos) --blk;
+        while (blk + 1 < l.blocks && weight_to(l, span, even, blk + 1) <= from - pos) ++blk;
+        pos += weight_to(l, span, even, blk);
+        break;
+      }
+      pos += __shfl_sync(0xffffffffu, inc, 31);
+    }
     int slot = 0, k = 0, q_uses[2] = {0, 0};  // the ring's next slot, and how often it has gone round
     uint32_t round = 0;
     for (; !dead; ++k) {
       const int st = k & 1;
-      const long long want = static_cast<long long>(k) * grid + (k & 1 ? grid - 1 - blockIdx.x : blockIdx.x);
       Piece p;
       p.b = -1;
-      // the level (tiles of a piece) that `want` falls into, and its place there
-      int lo = 0;
-      long long r = want;
-      if (sorted) {
-        int hi = min(cap, top);
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if (pieces_above(mid) <= want) hi = mid;
-          else lo = mid + 1;
+      auto advance = [&](int64_t w) {  // on to the next piece
+        pos += w;
+        if (++blk < l.blocks) return;
+        blk = 0;
+        if (++hk < kv_heads) return;
+        hk = 0;
+        do {
+          if (++b < a.batch) l = load_of<kPaged>(g, b);
+        } while (b < a.batch && l.blocks == 0);
+      };
+      while (b < a.batch && pos < to_end) {
+        const int64_t w = weight_to(l, span, even, blk + 1) - weight_to(l, span, even, blk);
+        const int n = tiles_of(l, (blk + 1) * span), n1 = max(n, 1);  // (a piece without keys has its zeros to write)
+        const int k0 = cut_tile(from - pos, w, n1), k1 = cut_tile(to_end - pos, w, n1);
+        if (k0 < k1) {
+          p.b = b;
+          p.hk = hk;
+          p.first = l.first;
+          p.len = l.len;
+          p.ctx = l.ctx;
+          p.bad = l.bad;
+          p.tok0 = blk * span;
+          p.toks = min(l.q - p.tok0, span);
+          p.k0 = k0;
+          p.total = min(k1, n) - k0;
+          p.halves = p.toks <= g.tile_tokens;
+          p.n[0] = p.halves ? (p.total + 1) / 2 : max(min(tiles_of(l, p.tok0 + g.tile_tokens), k1) - k0, 0);
+          p.n[1] = p.halves ? p.total / 2 : p.total;
+          int c0 = cta, c1 = cta;  // the CTAs of its first and last part
+          if (k0 > 0)
+            while (cut_tile(cut_at(total, ctas, per, c0) - pos, w, n1) > 0) --c0;
+          if (k1 < n1)
+            while (cut_tile(cut_at(total, ctas, per, c1 + 1) - pos, w, n1) < n1) ++c1;
+          p.cta0 = c0;
+          p.splits = c1 - c0 + 1;
+          p.split = cta - c0;
+          if (l.bad && lane == 0) report(a.status, MKB_SERVE_BAD_LENGTH);
         }
-        r = want - pieces_above(lo);
-      }
-      int slot_base = 0;
-      for (int b0 = 0; b0 < a.batch; b0 += 32) {
-        const int b = b0 + lane;
-        Load l = {};
-        int above = 0, here = 0, slots = 0;
-        if (b < a.batch) {
-          l = request(b);
-          l.splits = splits_of(l);
-          if (sorted) {
-            above = blocks_above(l, span, g.span_mul, lo * l.splits);
-            here = blocks_above(l, span, g.span_mul, lo * l.splits - l.splits) - above;
-          } else {
-            here = l.blocks;
-          }
-          here *= l.splits * kv_heads;
-          slots = l.splits > 1 ? l.blocks * l.splits * kv_heads : 0;
-        }
-        int inc = here, sinc = slots;  // inclusive prefix sums
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int x = __shfl_up_sync(0xffffffffu, inc, o), y = __shfl_up_sync(0xffffffffu, sinc, o);
-          if (lane >= o) {
-            inc += x;
-            sinc += y;
-          }
-        }
-        const bool is_it = r >= inc - here && r < inc;
-        const uint32_t who = __ballot_sync(0xffffffffu, is_it);
-        if (who != 0) {
-          if (is_it) {
-            unsigned at = static_cast<unsigned>(r) - (inc - here);
-            p.b = b;
-            p.split = at % static_cast<unsigned>(l.splits);
-            at /= static_cast<unsigned>(l.splits);
-            p.hk = at % static_cast<unsigned>(kv_heads);
-            const int i = l.blocks - 1 - above - static_cast<int>(at / static_cast<unsigned>(kv_heads));  // longest first
-            p.first = l.first;
-            p.len = l.len;
-            p.ctx = l.ctx;
-            p.tok0 = i * span;
-            p.toks = min(l.q - p.tok0, span);
-            const int n = tiles_of(l, p.tok0 + p.toks), per = (n + l.splits - 1) / l.splits;
-            p.k0 = min(p.split * per, n);
-            const int k1 = min(p.k0 + per, n);
-            p.splits = l.splits;
-            p.slot = slot_base + sinc - slots + (i * kv_heads + p.hk) * l.splits;
-            p.bad = l.bad;
-            p.total = k1 - p.k0;
-            p.halves = p.toks <= g.tile_tokens;
-            p.n[0] = p.halves ? (p.total + 1) / 2 : max(min(tiles_of(l, p.tok0 + g.tile_tokens), k1) - p.k0, 0);
-            p.n[1] = p.halves ? p.total / 2 : p.total;
-            if (l.bad) report(a.status, MKB_SERVE_BAD_LENGTH);
-          }
-          const int src = __ffs(who) - 1;
-          uint32_t* w = reinterpret_cast<uint32_t*>(&p);
-#pragma unroll
-          for (int i = 0; i < static_cast<int>(sizeof(Piece) / 4); ++i) w[i] = __shfl_sync(0xffffffffu, w[i], src);
-          break;
-        }
-        r -= __shfl_sync(0xffffffffu, inc, 31);
-        slot_base += __shfl_sync(0xffffffffu, sinc, 31);
+        if (p.b >= 0) break;
+        advance(w);
       }
       if (k >= 2) wait_for(&sm.info_empty[st], ((k >> 1) - 1) & 1, &sm.err, dead);
       if (lane == 0) {
@@ -545,6 +564,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       __syncwarp();
       if (p.b < 0) break;
+      advance(weight_to(l, span, even, blk + 1) - weight_to(l, span, even, blk));
       // K(0), then K(j + 1) and V(j): the order in which the products take them
       const int n = p.total;
       auto load = [&](const CUtensorMap* map, int head, int j) {
@@ -874,11 +894,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       constexpr int kPer = D / 32;
       uint8_t* stage = sm.stage[warp];
       // Rows on their way out, 32 values at a time (a small loop: this code is not in the
-      // instruction cache when a piece ends) and 64 to a store: by TMA where all 32 rows of
-      // the warp are whole tokens of the request, else 128 bytes of four rows at a time
+      // instruction cache when a piece ends): 64 values of all 32 rows of the warp by a TMA
+      // store where they are whole tokens of the request, else a thread its own row
       const int tok_w = tok_t + g.warp_tokens * (warp & 3);
       const bool whole = g.warp_tokens > 0 && tok_w + g.warp_tokens <= p.tok0 + p.toks;
       auto emit = [&](int c, const uint32_t* w) {  // values 32 c .. + 31 of every row, packed
+        if (!whole) {
+          if (live) {
+            T* out = static_cast<T*>(a.out) + (p.first + tok_t + tok_in) * a.out_stride[0] +
+                     (p.hk * g.group + row_in - tok_in * g.group) * a.out_stride[1] + 32 * c;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              reinterpret_cast<uint4*>(out)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          }
+          return;
+        }
         if ((c & 1) == 0) {
           if (lane == 0) tma_store_read();
           __syncwarp();
@@ -888,29 +918,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * (c & 1) + i) ^ (lane & 7)) << 4)) =
               make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
         if ((c & 1) == 0) return;
-        if (whole) {
-          fence_proxy_async_shared();
-          __syncwarp();
-          if (lane == 0) tma_store_3d(stage, &to, 32 * (c - 1), p.hk * g.group, p.first + tok_w);
-          return;
-        }
+        fence_proxy_async_shared();
         __syncwarp();
-#pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
-          const int r = 4 * i + (lane >> 3), rt = 32 * (warp & 3) + r;
-          const int tok = rt * g.group_mul >> 16, head = p.hk * g.group + rt - tok * g.group;
-          if (rt < g.tile_tokens * g.group && tok_t + tok < p.tok0 + p.toks)
-            *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (p.first + tok_t + tok) * a.out_stride[0] +
-                                      head * a.out_stride[1] + 32 * (c - 1) + 8 * (lane & 7)) =
-                *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-        }
-        __syncwarp();
+        if (lane == 0) tma_store_3d(stage, &to, 32 * (c - 1), p.hk * g.group, p.first + tok_w);
       };
       const bool split = p.splits > 1;
       const int at = 128 * t + row_in;
-      const size_t slot = p.slot + p.split;
+      auto slot_of = [&](int s) { return static_cast<size_t>(2 * (p.cta0 + s) + (s == 0)); };
+      const size_t slot = slot_of(p.split);
       float4* part = g.part + slot * (D / 4) * kRows;
-      if (split && static_cast<size_t>(p.slot) + p.splits > static_cast<size_t>(g.slots)) continue;  // (cannot be: tc_slots)
       uint64_t odd2 = 0;  // NaN once a value of O is not finite
       // no weights at all (every score -inf) are no mean; a row that sees no key is zero
       const bool zero = lim < 0 && !bad, zeros = __any_sync(0xffffffffu, zero);
@@ -943,10 +959,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int i = 0; i < 16; ++i) odd2 = fma2(o2[i], 0, odd2);
         if (split) {  // one of several ranges of keys: left for whoever comes last
+          if (live) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 u = unpack2(o2[2 * i]), v = unpack2(o2[2 * i + 1]);
-            part[(8 * c + i) * kRows + at] = make_float4(u.x, u.y, v.x, v.y);
+            for (int i = 0; i < 8; ++i) {
+              const float2 u = unpack2(o2[2 * i]), v = unpack2(o2[2 * i + 1]);
+              part[(8 * c + i) * kRows + at] = make_float4(u.x, u.y, v.x, v.y);
+            }
           }
         } else {
 #pragma unroll
@@ -968,7 +986,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.pair_empty);
       }
-      if (split) g.stat[slot * kRows + at] = make_float2(m, bad ? NAN : l);
+      if (split && live) g.stat[slot * kRows + at] = make_float2(m, bad ? NAN : l);
       // the rows of the warp whose O is not finite, key by key
       uint32_t todo = __ballot_sync(0xffffffffu, odd != 0.f && live && lim >= 0 && !bad);
       if (todo != 0) {
@@ -1003,38 +1021,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tile_sync();
         if (threadIdx.x % 128 == 0)
           *reinterpret_cast<volatile int*>(&sm.last[t]) =
-              atomicInc(g.counters + 2 * static_cast<size_t>(p.slot) + t, p.splits - 1) ==
+              atomicInc(g.counters + 2 * p.cta0 + t, p.splits - 1) ==
               static_cast<uint32_t>(p.splits - 1);
         tile_sync();
         if (*reinterpret_cast<volatile int*>(&sm.last[t]) != 0) {
           __threadfence();
-          const float2* stat = g.stat + static_cast<size_t>(p.slot) * kRows + at;
           float mm = -INFINITY, ll = 0.f;
-          for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, __ldcg(stat + s * kRows).x);
+          for (int s = 0; s < p.splits && live; ++s) mm = fmaxf(mm, __ldcg(g.stat + slot_of(s) * kRows + at).x);
           const float ref = mm == -INFINITY ? 0.f : mm;
-          for (int s = 0; s < p.splits; ++s) {
-            const float2 x = __ldcg(stat + s * kRows);
+          for (int s = 0; s < p.splits && live; ++s) {
+            const float2 x = __ldcg(g.stat + slot_of(s) * kRows + at);
             ll += x.y * ex2_approx(x.x - ref);
           }
           const float f0 = 1.f / ll;
-          const float4* part0 = g.part + static_cast<size_t>(p.slot) * (D / 4) * kRows + at;
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             float o[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0.f;
-            for (int s = 0; s < p.splits; ++s) {
-              const float w = __ldcg(stat + s * kRows).x;
+#pragma unroll 2
+            for (int s = 0; s < p.splits && live; ++s) {
+              const float w = __ldcg(g.stat + slot_of(s) * kRows + at).x;
+              const float4* x4 = g.part + (slot_of(s) * (D / 4) + 8 * c) * kRows + at;
+              float4 x[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[i] = __ldcg(x4 + i * kRows);
               if (w == -INFINITY) continue;  // that range holds no key this row sees
               const float f = ex2_approx(w - ref);
-              const float4* x4 = part0 + (static_cast<size_t>(s) * (D / 4) + 8 * c) * kRows;
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float4 x = __ldcg(x4 + i * kRows);
-                o[4 * i] += f * x.x;
-                o[4 * i + 1] += f * x.y;
-                o[4 * i + 2] += f * x.z;
-                o[4 * i + 3] += f * x.w;
+                o[4 * i] += f * x[i].x;
+                o[4 * i + 1] += f * x[i].y;
+                o[4 * i + 2] += f * x[i].z;
+                o[4 * i + 3] += f * x[i].w;
               }
             }
             uint32_t w[16];
@@ -1109,14 +1128,10 @@ static int64_t tc_blocks(const mkb_attn_args& a) {
   const int64_t span = 2 * (128 / (a.heads / a.kv_heads));
   return (a.tokens / span + a.batch) * a.kv_heads;
 }
-// Partial results a call can leave. Rows are split only past a fair share C >= 5/4 U /
-// grid of the U key tiles, into at most 2 n / C pieces for n tiles; a request's blocks
-// grow linearly, so U counts at least half of n for each: at most 4 U / C < 4 grid.
-static int64_t tc_slots(const mkb_attn_args& a) { return 4 * static_cast<int64_t>(sm_count()); }
-
+// Counters, then two partial results a CTA.
+static size_t tc_counter_bytes() { return (static_cast<size_t>(sm_count()) * 8 + 255) / 256 * 256; }
 size_t tc_workspace(const mkb_attn_args& a) {
-  const size_t slots = tc_slots(a);
-  return 256 + slots * 8 + slots * kRows * (static_cast<size_t>(a.head_dim) * 4 + 8) + 256;
+  return tc_counter_bytes() + 2 * static_cast<size_t>(sm_count()) * kRows * (static_cast<size_t>(a.head_dim) * 4 + 8);
 }
 
 template <typename T, int D, bool kPaged>
@@ -1128,16 +1143,13 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   g.tile_tokens = 128 / g.group;
   g.warp_tokens = 32 % g.group == 0 ? 32 / g.group : 0;
   g.group_mul = 65536 / g.group + 1;
-  g.span_mul = static_cast<unsigned>((1ull << 32) / (2 * g.tile_tokens) + 1);
   g.k_head = a.k_stride[1] != 0;
   g.v_head = a.v_stride[1] != 0;
-  g.slots = static_cast<int>(tc_slots(a));
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   if (ws == nullptr) return cudaErrorInvalidValue;
-  const size_t cb = (static_cast<size_t>(g.slots) * 8 + 255) / 256 * 256;
   g.counters = reinterpret_cast<uint32_t*>(ws);
-  g.stat = reinterpret_cast<float2*>(ws + cb);
-  g.part = reinterpret_cast<float4*>(ws + cb + static_cast<size_t>(g.slots) * kRows * 8);
+  g.stat = reinterpret_cast<float2*>(ws + tc_counter_bytes());
+  g.part = reinterpret_cast<float4*>(g.stat + 2 * static_cast<size_t>(sm_count()) * kRows);
   CUtensorMap mk, mv, mq, mo;
   cudaError_t e;
   {
@@ -1183,8 +1195,7 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   const int64_t blocks = tc_blocks(a) * (kPaged ? (static_cast<int64_t>(a.table_width) * a.page_size / kKeys) / kMinSplit + 1
                                                 : a.tokens / (kKeys * kMinSplit) + 1);
   const int grid = static_cast<int>(blocks < sm_count() ? blocks : sm_count());
-  attn_tc_kernel<T, D, kPaged><<<grid, kTcThreads, bytes, stream>>>(mk, mv, mq, mo, g);
-  return cudaGetLastError();
+  return launch_early(attn_tc_kernel<T, D, kPaged>, grid, kTcThreads, bytes, stream, mk, mv, mq, mo, g);
 }
 
 template <typename T>

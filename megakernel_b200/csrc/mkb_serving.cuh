@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cstdint>
+#include <utility>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -87,6 +88,28 @@ __device__ __forceinline__ Request request_rows(const int* __restrict__ cu, int 
 }
 __device__ __forceinline__ Request request_at(const int* __restrict__ cu, int batch, int q_len, int tokens, int t) {
   return request_rows(cu, cu == nullptr ? t / q_len : request_of(cu, batch, t), q_len, tokens);
+}
+
+// ---- early launch ----------------------------------------------------------------------
+// A kernel of this family may be brought in while the one before it in the stream is
+// still running its last blocks: it sets itself up, and waits (depend_wait) before it
+// touches memory until all that came before has completed.
+__device__ __forceinline__ void depend_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void depend_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), int grid, int threads, size_t smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, std::forward<A>(args)...);
 }
 
 // Records the first error of a launch.
