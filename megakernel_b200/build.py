@@ -22,7 +22,7 @@ LIB = os.path.join(HERE, "libmkb200.so")
 EXT_DIR = os.path.join(HERE, "_build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 KERNEL_SOURCES = ["mkb_decode.cu", "mkb_host.cu", "mkb_noalloc.cu", "mkb_prefill.cu", "mkb_append.cu", "mkb_attn.cu",
-                  "mkb_attn_tc.cu"]
+                  "mkb_attn_tc.cu", "mkb_attn_decode.cu"]
 EXT_SOURCES = ["binding.cpp", "binding_serving.cpp"]
 
 

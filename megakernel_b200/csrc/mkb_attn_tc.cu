@@ -338,57 +338,6 @@ __device__ __forceinline__ int cut_tile(int64_t y, int64_t w, int n) {
   return t < kMinPart ? 0 : t > n - kMinPart ? n : t;
 }
 
-// ---- one row, key by key: what a tile with values that are not finite comes to --------
-// Warp-wide; lane holds dims [lane * D / 32, + D / 32) of O, relative to maximum m.
-template <typename T, int D, bool kPaged>
-__device__ __noinline__ void slow_row(const TcArgs& g, const Piece& p, int token, int h, int k_end, float* o,
-                                      float* m_out, float* l_out) {
-  const mkb_attn_args& a = g.a;
-  const int lane = threadIdx.x & 31;
-  constexpr int kPer = D / 32;
-  const T* q = static_cast<const T*>(a.q) + (p.first + token) * a.q_stride[0] + h * a.q_stride[1];
-  const int keys = min(k_end, p.ctx + token + 1);
-  float m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-  for (int j = p.k0 * kKeys; j < keys; ++j) {
-    int64_t ko, vo;
-    if (kPaged) {
-      const int64_t page = a.block_table[p.b * a.table_stride + j / a.page_size], slot = j % a.page_size;
-      if (page < 0 || page >= a.pages) continue;  // reported; the piece is NaN already
-      ko = page * a.k_stride[0] + p.hk * a.k_stride[1] + slot * a.k_stride[2];
-      vo = page * a.v_stride[0] + p.hk * a.v_stride[1] + slot * a.v_stride[2];
-    } else {
-      ko = static_cast<int64_t>(p.first + j) * a.k_stride[0] + p.hk * a.k_stride[1];
-      vo = static_cast<int64_t>(p.first + j) * a.v_stride[0] + p.hk * a.v_stride[1];
-    }
-    const uint32_t* k2 = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.k) + ko);
-    const uint32_t* v2 = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.v) + vo);
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPer / 2; ++i) {
-      const float2 x = Pair<T>::get(reinterpret_cast<const uint32_t*>(q)[lane * (kPer / 2) + i]);
-      const float2 y = Pair<T>::get(k2[lane * (kPer / 2) + i]);
-      s += x.x * y.x + x.y * y.y;
-    }
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= g.sl2;
-    const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
-    const float sc = ex2_approx(m - ref), w = ex2_approx(s - ref);
-    l = l * sc + w;
-#pragma unroll
-    for (int i = 0; i < kPer / 2; ++i) {
-      const float2 y = Pair<T>::get(v2[lane * (kPer / 2) + i]);
-      o[2 * i] = o[2 * i] * sc + w * y.x;
-      o[2 * i + 1] = o[2 * i + 1] * sc + w * y.y;
-    }
-    m = mn;
-  }
-  *m_out = m;
-  *l_out = l;
-}
-
 template <typename T, int D, bool kPaged>
 __global__ void __launch_bounds__(kTcThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -999,7 +948,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int head = p.hk * g.group + rt - tok * g.group;
         todo &= todo - 1;
         float o[kPer], ms, ls;
-        slow_row<T, D, kPaged>(g, p, tok_t + tok, head, k_end, o, &ms, &ls);
+        row_by_key<T, D, kPaged>(a, g.sl2, p.b, p.first, p.first + tok_t + tok, head, p.hk, p.k0 * kKeys,
+                                 min(k_end, p.ctx + tok_t + tok + 1), o, &ms, &ls);
         if (split) {
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
@@ -1115,7 +1065,7 @@ static cudaError_t map_rows(CUtensorMap* m, int dtype, const void* base, int D, 
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-static int sm_count() {
+int sm_count() {
   static int n[64] = {0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
@@ -1128,10 +1078,11 @@ static int64_t tc_blocks(const mkb_attn_args& a) {
   const int64_t span = 2 * (128 / (a.heads / a.kv_heads));
   return (a.tokens / span + a.batch) * a.kv_heads;
 }
-// Counters, then two partial results a CTA.
-static size_t tc_counter_bytes() { return (static_cast<size_t>(sm_count()) * 8 + 255) / 256 * 256; }
+// Counters (the place of both attention kernels', zero between calls), then two partial
+// results a CTA.
+size_t counter_bytes() { return (static_cast<size_t>(sm_count()) * 8 + 255) / 256 * 256; }
 size_t tc_workspace(const mkb_attn_args& a) {
-  return tc_counter_bytes() + 2 * static_cast<size_t>(sm_count()) * kRows * (static_cast<size_t>(a.head_dim) * 4 + 8);
+  return counter_bytes() + 2 * static_cast<size_t>(sm_count()) * kRows * (static_cast<size_t>(a.head_dim) * 4 + 8);
 }
 
 template <typename T, int D, bool kPaged>
@@ -1148,7 +1099,7 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   if (ws == nullptr) return cudaErrorInvalidValue;
   g.counters = reinterpret_cast<uint32_t*>(ws);
-  g.stat = reinterpret_cast<float2*>(ws + tc_counter_bytes());
+  g.stat = reinterpret_cast<float2*>(ws + counter_bytes());
   g.part = reinterpret_cast<float4*>(g.stat + 2 * static_cast<size_t>(sm_count()) * kRows);
   CUtensorMap mk, mv, mq, mo;
   cudaError_t e;
