@@ -4,10 +4,9 @@
 //
 // Every key and value is read once from memory and used for the handful of rows (new
 // tokens x the query heads that share the KV head, 16 at most) that need it: bytes bound
-// this kernel, at 4 D bytes a key and KV head. It reads them straight into shared memory
-// (cp.async, 16 bytes a lane, chunks swizzled within a row so that the matrix loads below
-// meet no bank twice), a ring of stages per warp, with no barrier between warps: a warp
-// waits for its own copies only.
+// this kernel, at 4 D bytes a key and KV head. TMA brings them into shared memory (a box
+// of 16 keys x 64 values, 128-byte swizzle, so that the matrix loads below meet no bank
+// twice), a ring of tiles per warp, with no barrier between warps.
 //
 // The products run on mma.sync m16n8k16 with the keys as the 16 rows of S^T = K Q^T and
 // the queries as its columns (8 or 16 of them), so that the tile is filled by keys however
@@ -16,48 +15,46 @@
 // and the remainder: memory leaves time for the second product, and P then costs no
 // precision.
 //
-// Work: the requests' tiles of 16 keys, KV head by KV head, are laid end to end and cut
-// into equal ranges, one a CTA; a CTA's warps take every eighth tile of each
-// stretch that belongs to one request and KV head, and add up at its end. A stretch that
-// is not the whole of its keys leaves O, maximum and sum in memory; the last one to be done
-// adds them up in order.
+// Work: the tiles of 16 keys, request by request and KV head by KV head, are laid end to
+// end and cut into equal ranges, one a CTA, and those into eight, one a warp. A warp runs
+// through its range on its own, its copies a few tiles ahead and across the ends of
+// requests; what lies in one warp's range as a whole it writes out itself. The others
+// leave O, maximum and sum in shared memory, where the CTA adds them up at its end; those
+// that go on in another CTA, in memory, where the last CTA to be done adds them up in
+// order of their keys.
 
 #include <cmath>
 
 #include "mkb_serving.cuh"
+#include "mkb_tc.cuh"
 
 namespace mkb {
 namespace sv {
 
 constexpr int kDecWarps = 8;
-constexpr int kTileKeys = 16;  // keys of a tile: the rows of one mma
-constexpr int kDecTileMin = 16;  // tiles (of 16 keys) that are worth a CTA
+constexpr int kTileKeys = 16;    // keys of a tile: the rows of one mma
+constexpr int kCtaTiles = 16;    // tiles that are worth a CTA where few requests are long ...
+constexpr int kLongTiles = 48;   // ... which is what more tiles than this a request and KV head is
+constexpr int kWholeTiles = 8;   // below this a request's tiles (of a KV head) stay with one warp
+constexpr int kDecTryNs = 20000, kDecTries = 50000;  // bound of a wait: about a second
 
 struct DecArgs {
   mkb_attn_args a;
   float sl2;
+  int k_head, v_head;  // 0 where every KV head lies at the same place (stride 0), else 1
   int group, rows;     // query heads of a KV head; rows (q_len * group)
+  int cols;            // rows up to a power of two: columns of a part
+  int stages;          // tiles of a warp's ring
+  int warp_bytes;      // a warp's shared memory: the ring, then the part that it does not begin
   uint32_t* counters;  // [ctas], zero between calls
-  float* part;         // [2 ctas][D][16] O^T, then its maxima and sums [2 ctas][2][16]
+  float* part;         // [2 ctas][D][16] O^T, the maxima and sums in stat [2 ctas][2][16]
   float* stat;
 };
 
+constexpr int kMaxStages = 6;
 template <int D>
-struct DecShape {
-  static constexpr int kStages = D == 128 ? 3 : 6;       // tiles of a warp in flight (one being worked on)
-  static constexpr int kStageBytes = kTileKeys * D * 2 * 2;  // K and V
-  static constexpr size_t kSmem = static_cast<size_t>(kDecWarps) * kStages * kStageBytes;
-};
+constexpr int kStageBytes = kTileKeys * D * 2 * 2;  // K and V of a tile
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
-  const int n = there ? 16 : 0;  // 0: zeros, nothing is read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t r[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -94,49 +91,75 @@ __device__ __forceinline__ int dec_tiles(const DecArgs& g, int b, int* len_out, 
   return bad ? 1 : max((len + kTileKeys - 1) / kTileKeys, 1);
 }
 
+// A place in the work: tile t of [.., t_end) of request b, KV head hk, whose tiles follow
+// `pos` and one unit for its fixed cost.
+struct Cursor {
+  int b, hk, n, len, t, t_end;
+  bool bad;
+  int64_t pos;
+};
+
 // kN: columns of 8 rows each (1 or 2)
 template <typename T, int D, int kN>
-__global__ void __launch_bounds__(32 * kDecWarps, 1) attn_decode_kernel(const __grid_constant__ DecArgs g) {
-  using Shape = DecShape<D>;
-  constexpr int kStages = Shape::kStages, kChunks = D / 8;  // 16-byte chunks of a row
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float red_m[kDecWarps][16], red_l[kDecWarps][16];
-  __shared__ int flag;
-  __shared__ uint32_t odd_rows;  // rows whose O is not finite
+__global__ void __launch_bounds__(32 * kDecWarps, 1)
+    attn_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                       const __grid_constant__ DecArgs g) {
+  constexpr int kBytes = kStageBytes<D>, kHalf = kTileKeys * 128;  // (64 values of 16 keys)
+  constexpr int kPer = D / 32;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[kDecWarps][kMaxStages];
+  __shared__ float part_m[kDecWarps][2][16], part_l[kDecWarps][2][16];
+  __shared__ int64_t part_pos[kDecWarps][2];                   // the request's and KV head's place, -1: none
+  __shared__ int part_at[kDecWarps][2][4];                     // b, hk, len, n
+  __shared__ float fac_mem[(2 * kDecWarps + 1) * 16];
+  __shared__ int flag, err;
   const mkb_attn_args& a = g.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   depend_launch();
-  const uint32_t ring = smem_addr(smem) + warp * (kStages * Shape::kStageBytes);
+  uint8_t* const mine = smem + warp * g.warp_bytes;
+  const uint32_t ring = smem_addr(mine);
+  // parts: 0 goes on from the warp before, 1 begins here (and lies over the ring, at the end)
+  float* const part_o[2] = {reinterpret_cast<float*>(mine + g.stages * kBytes), reinterpret_cast<float*>(mine)};
+  if (lane < 2) part_pos[warp][lane] = -1;
+  if (lane == 0) {
+    tc::prefetch_tensormap(&tk);
+    tc::prefetch_tensormap(&tv);
+    for (int i = 0; i < g.stages; ++i) mbar_init(&full[warp][i], 1);
+    fence_mbar_init();
+  }
+  if (threadIdx.x == 0) err = 0;
+  __syncthreads();
   depend_wait();
 
-  // ---- this CTA's range of tiles ---------------------------------------------------------
-  // (every warp works it out for itself; a lane keeps the first 32 requests' tiles)
+  // ---- the work, and this warp's range of it ----------------------------------------------
   int len0 = 0;
   bool bad0 = false;
-  const int tiles0 = lane < a.batch ? dec_tiles(g, lane, &len0, &bad0) : 0;
+  const int tiles0 = lane < a.batch ? dec_tiles(g, lane, &len0, &bad0) + 1 : 0;  // (a lane keeps its first request's)
   int64_t total = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
     int n = tiles0, x;
     bool y;
-    if (b0 > 0) n = b0 + lane < a.batch ? dec_tiles(g, b0 + lane, &x, &y) : 0;
+    if (b0 > 0) n = b0 + lane < a.batch ? dec_tiles(g, b0 + lane, &x, &y) + 1 : 0;
     total += __reduce_add_sync(0xffffffffu, n);
   }
   total *= a.kv_heads;
-  // a CTA for every kDecTileMin tiles, or for every request and KV head if those are more
   const int64_t heads = static_cast<int64_t>(a.batch) * a.kv_heads;
-  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(total / kDecTileMin, heads)));
+  const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x),
+                                        total > heads * kLongTiles ? max(total / kCtaTiles, heads) : heads));
   const int cta = blockIdx.x;
   if (cta >= ctas) return;
   const double per = static_cast<double>(total) / ctas;
   auto cut = [&](int c) { return c >= ctas ? total : static_cast<int64_t>(per * c); };
-  const int64_t from = cut(cta), to = cut(cta + 1);
-  int b = a.batch, n = 0, len = 0, hk = 0;
-  bool bad = false;
-  int64_t pos = 0;  // tiles before the stretch's request and KV head
-  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+  const int64_t cta_from = cut(cta), cta_units = cut(cta + 1) - cta_from;
+  const int64_t from = cta_from + cta_units * warp / kDecWarps, to = cta_from + cta_units * (warp + 1) / kDecWarps;
+  Cursor ahead;  // of the next tile to load
+  ahead.b = a.batch;
+  ahead.pos = 0;
+  for (int b0 = 0; b0 < a.batch && from < to; b0 += 32) {
     int t = tiles0, ln = len0;
     bool bd = bad0;
-    if (b0 > 0) t = b0 + lane < a.batch ? dec_tiles(g, b0 + lane, &ln, &bd) : 0;
+    if (b0 > 0) t = b0 + lane < a.batch ? dec_tiles(g, b0 + lane, &ln, &bd) + 1 : 0;
     int64_t inc = static_cast<int64_t>(t) * a.kv_heads;
     const int64_t own = inc;
 #pragma unroll
@@ -144,68 +167,101 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) attn_decode_kernel(const __
       const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
     }
-    const uint32_t who = __ballot_sync(0xffffffffu, from - pos < inc);
+    const uint32_t who = __ballot_sync(0xffffffffu, from - ahead.pos < inc);
     if (who != 0) {
       const int src = __ffs(who) - 1;
-      b = b0 + src;
-      n = __shfl_sync(0xffffffffu, t, src);
-      len = __shfl_sync(0xffffffffu, ln, src);
-      bad = __shfl_sync(0xffffffffu, static_cast<int>(bd), src) != 0;
-      pos += __shfl_sync(0xffffffffu, inc - own, src);
-      hk = static_cast<int>((from - pos) / n);
-      pos += static_cast<int64_t>(n) * hk;
+      ahead.b = b0 + src;
+      ahead.n = __shfl_sync(0xffffffffu, t, src) - 1;
+      ahead.len = __shfl_sync(0xffffffffu, ln, src);
+      ahead.bad = __shfl_sync(0xffffffffu, static_cast<int>(bd), src) != 0;
+      ahead.pos += __shfl_sync(0xffffffffu, inc - own, src);
+      const unsigned at = static_cast<unsigned>(from - ahead.pos);  // (under 2^31: tiles of one request, all heads)
+      ahead.hk = static_cast<int>(at / static_cast<unsigned>(ahead.n + 1));
+      ahead.pos += static_cast<int64_t>(ahead.n + 1) * ahead.hk;
       break;
     }
-    pos += __shfl_sync(0xffffffffu, inc, 31);
+    ahead.pos += __shfl_sync(0xffffffffu, inc, 31);
   }
+  // a cut at x as a tile of the request and KV head that c stands at
+  auto tile_at = [&](int64_t x, int64_t pos, int n) {
+    const int64_t y = x - pos;
+    if (y <= 0) return 0;
+    if (y >= n + 1) return n;
+    if (n < kWholeTiles) return 2 * y >= n + 1 ? n : 0;
+    return static_cast<int>(y) - 1;
+  };
+  auto enter = [&](Cursor& c) {  // the part of c's tiles that is this warp's
+    c.t = tile_at(from, c.pos, c.n);
+    c.t_end = tile_at(to, c.pos, c.n);
+  };
+  auto leave = [&](Cursor& c) {  // on to the next request and KV head
+    c.pos += c.n + 1;
+    if (++c.hk == a.kv_heads) {
+      c.hk = 0;
+      if (++c.b < a.batch) c.n = dec_tiles(g, c.b, &c.len, &c.bad);
+    }
+    enter(c);
+  };
+  auto open = [&](const Cursor& c) { return c.b < a.batch && c.pos < to; };
+  enter(ahead);
+  Cursor cur = ahead;
 
-  // ---- stretches ----------------------------------------------------------------------------
-  while (pos < to && b < a.batch) {
-    const int t0 = static_cast<int>(max(from - pos, static_cast<int64_t>(0)));
-    const int t1 = static_cast<int>(min(to - pos, static_cast<int64_t>(n)));
-    uint32_t page_bad = 0;
-    const T* kbase = static_cast<const T*>(a.k) + hk * a.k_stride[1];
-    const T* vbase = static_cast<const T*>(a.v) + hk * a.v_stride[1];
-    const int first_pos = len - a.q_len;  // position of the request's first new token
-    // a tile of the warp into a stage: 16 keys lie in one page
-    const int mine = t1 > t0 + warp ? (t1 - t0 - warp + kDecWarps - 1) / kDecWarps : 0;
-    auto page_of = [&](int i) {
-      return i < mine && !bad && len > 0
-                 ? __ldg(a.block_table + b * a.table_stride + (t0 + warp + i * kDecWarps) * kTileKeys / a.page_size)
-                 : 0;
-    };
-    int ahead[kStages];  // the pages of the next tiles to load, read that much earlier
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) ahead[i] = page_of(i);
-    auto load = [&](int i) {
-      if (i < mine && !bad && len > 0) {
-        const int key = (t0 + warp + i * kDecWarps) * kTileKeys;
-        const int page = ahead[0];
-        const bool ok = page >= 0 && page < a.pages;
-        if (!ok) page_bad = 1;
-        const int64_t ko = ok ? page * a.k_stride[0] : 0, vo = ok ? page * a.v_stride[0] : 0;
-        const int slot = key & (a.page_size - 1);
-        const uint32_t dst = ring + (i % kStages) * Shape::kStageBytes;
-#pragma unroll
-        for (int c0 = 0; c0 < kTileKeys * kChunks; c0 += 32) {
-          const int c = c0 + lane, r = c / kChunks, x = c % kChunks;
-          const bool there = ok && key + r < len;  // (past the last key: zeros, whatever lies there)
-          const uint32_t at = dst + r * (D * 2) + ((x ^ (r & 7)) << 4);
-          cp_async16(at, there ? static_cast<const void*>(kbase + ko + (slot + r) * a.k_stride[2] + 8 * x) : a.k, there);
-          cp_async16(at + Shape::kStageBytes / 2,
-                     there ? static_cast<const void*>(vbase + vo + (slot + r) * a.v_stride[2] + 8 * x) : a.k, there);
+  bool dead = false;             // a wait has expired: nothing is loaded or waited for any more
+  int fill = 0;                  // the ring's next stage to load
+  int pages = 0, pages_at = -1;  // the lanes' pages of tiles pages_at .. + 31 of request pages_b
+  int pages_b = -1;
+  uint32_t bad_pages = 0;          // of the tiles in flight, a bit each, whether their page is outside the pool
+  int load_bit = 0, bad_bit = 0;
+  auto load = [&]() {
+    while (open(ahead) && ahead.t >= ahead.t_end) leave(ahead);
+    if (dead || !open(ahead)) return;
+    bool oob = false;
+    if (!ahead.bad && ahead.len > 0) {
+      if (pages_b != ahead.b || ahead.t < pages_at || ahead.t >= pages_at + 32) {
+        pages_b = ahead.b;
+        pages_at = ahead.t;
+        const int key = (ahead.t + lane) * kTileKeys;  // 16 keys lie in one page
+        pages = key < ahead.len ? __ldg(a.block_table + ahead.b * a.table_stride + key / a.page_size) : 0;
+        if (pages < 0 || pages >= a.pages) {
+          report(a.status, MKB_SERVE_BAD_PAGE);
+          pages = -1;
         }
       }
-      cp_commit();
+      const int page = __shfl_sync(0xffffffffu, pages, ahead.t - pages_at);
+      const int slot = ahead.t * kTileKeys & (a.page_size - 1);
+      oob = page < 0;
+      if (lane == 0) {
+        uint8_t* const dst = mine + fill * kBytes;
+        uint64_t* const bar = &full[warp][fill];
+        const int at = page < 0 ? a.pages : page;  // (outside the pool: zeros)
+        mbar_arrive_expect_tx(bar, kBytes);
 #pragma unroll
-      for (int s = 0; s + 1 < kStages; ++s) ahead[s] = ahead[s + 1];
-      ahead[kStages - 1] = page_of(i + kStages);
-    };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) load(i);
+        for (int d = 0; d < D / 64; ++d) {
+          tc::tma_load_4d(dst + d * kHalf, &tk, 64 * d, slot, ahead.hk * g.k_head, at, bar);
+          tc::tma_load_4d(dst + kBytes / 2 + d * kHalf, &tv, 64 * d, slot, ahead.hk * g.v_head, at, bar);
+        }
+      }
+    } else if (lane == 0) {
+      mbar_arrive(&full[warp][fill]);  // nothing to bring
+    }
+    bad_pages = (bad_pages & ~(1u << load_bit)) | static_cast<uint32_t>(oob) << load_bit;
+    load_bit = (load_bit + 1) & 31;
+    if (++fill == g.stages) fill = 0;
+    ++ahead.t;
+  };
+#pragma unroll 1
+  for (int i = 0; i < g.stages - 1; ++i) load();
 
+  uint32_t phase = 0;
+  int stage = 0;
+  for (; open(cur); leave(cur)) {
+    if (cur.t >= cur.t_end) continue;
+    const int t0 = cur.t, t1 = cur.t_end, b = cur.b, hk = cur.hk, len = cur.len;
+    const int first_pos = len - a.q_len;  // position of the request's first new token
     // Q^T as the B operand: columns are rows of Q (row = token * group + head)
     uint32_t qf[kN][D / 16][2];
+    int lim[kN][2];  // of this lane's columns of S^T, rows 8 nn + 2 (lane % 4) + {0, 1}
+    float m[kN][2], l[kN][2], o[D / 16][kN][4];
 #pragma unroll
     for (int nn = 0; nn < kN; ++nn) {
       const int r = 8 * nn + lane / 4;
@@ -219,42 +275,59 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) attn_decode_kernel(const __
         qf[nn][kk][0] = live ? __ldg(q + 8 * kk + lane % 4) : 0;
         qf[nn][kk][1] = live ? __ldg(q + 8 * kk + 4 + lane % 4) : 0;
       }
-    }
-    // this lane's columns of S^T: rows 8 nn + 2 (lane % 4) + {0, 1}
-    int lim[kN][2];
-    float m[kN][2], l[kN][2], o[D / 16][kN][4];
-#pragma unroll
-    for (int nn = 0; nn < kN; ++nn)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int r = 8 * nn + 2 * (lane % 4) + e;
-        lim[nn][e] = r < g.rows ? first_pos + r / g.group : -1;
+        const int re = 8 * nn + 2 * (lane % 4) + e;
+        lim[nn][e] = re < g.rows ? min(first_pos + re / g.group, len - 1) : -1;
         m[nn][e] = -INFINITY;
         l[nn][e] = 0.f;
       }
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-      for (int nn = 0; nn < kN; ++nn)
+      for (int d = 0; d < D / 16; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[d][nn][e] = 0.f;
+    }
 
-    for (int i = 0; i < mine; ++i) {
-      load(i + kStages - 1);
-      cp_wait<kStages - 1>();
-      __syncwarp();
-      const uint32_t kt = ring + (i % kStages) * Shape::kStageBytes, vt = kt + Shape::kStageBytes / 2;
-      const int key = (t0 + warp + i * kDecWarps) * kTileKeys;
+    for (int t = t0; t < t1; ++t) {
+      load();
+      if (!dead)
+        for (int i = 0; !__all_sync(0xffffffffu, mbar_wait(&full[warp][stage], phase, kDecTryNs)); ++i)
+          if (i > kDecTries) {
+            err = 1;
+            dead = true;
+            break;
+          }
+      const uint32_t kt = ring + stage * kBytes, vt = kt + kBytes / 2;
+      const int key = t * kTileKeys;
+      if (key + kTileKeys > len) {  // past the last key a page holds anything: P = 0 must give 0
+        const int there = max(len - key, 0);
+        for (int i = lane; i < (kTileKeys - there) * (D / 8); i += 32)
+          *reinterpret_cast<uint4*>(mine + stage * kBytes + kBytes / 2 + (i / 8 % (D / 64)) * kHalf +
+                                    (there + i / (D / 8)) * 128 + (i % 8) * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_shared();
+        __syncwarp();
+      }
+      if (++stage == g.stages) {
+        stage = 0;
+        phase ^= 1;
+      }
       float s[kN][4] = {};
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {  // A: keys by dims
         uint32_t ka[4];
-        const int r = lane % 16, x = 2 * kk + lane / 16;
-        ldsm4(kt + r * (D * 2) + ((x ^ (r & 7)) << 4), ka);
+        const int r = lane % 16, x = 2 * (kk % 4) + lane / 16;
+        ldsm4(kt + kk / 4 * kHalf + r * 128 + ((x ^ (r & 7)) << 4), ka);
 #pragma unroll
         for (int nn = 0; nn < kN; ++nn) mma16816<T>(s[nn], ka, qf[nn][kk][0], qf[nn][kk][1]);
       }
       // s[nn][e], s[nn][2 + e]: keys lane / 4 and lane / 4 + 8, row 8 nn + 2 (lane % 4) + e
+      if (bad_pages >> bad_bit & 1u) {  // a page outside the pool: its keys are NaN
+#pragma unroll
+        for (int nn = 0; nn < kN; ++nn)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nn][e] = NAN;
+      }
+      bad_bit = (bad_bit + 1) & 31;
       uint32_t ph[kN][2], pl[kN][2];
 #pragma unroll
       for (int nn = 0; nn < kN; ++nn) {
@@ -262,8 +335,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) attn_decode_kernel(const __
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int j = key + lane / 4;
-          float x0 = j <= lim[nn][e] && j < len ? s[nn][e] * g.sl2 : -INFINITY;
-          float x1 = j + 8 <= lim[nn][e] && j + 8 < len ? s[nn][2 + e] * g.sl2 : -INFINITY;
+          const float x0 = j <= lim[nn][e] ? s[nn][e] * g.sl2 : -INFINITY;
+          const float x1 = j + 8 <= lim[nn][e] ? s[nn][2 + e] * g.sl2 : -INFINITY;
           float mx = fmaxf(x0, x1);
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
@@ -293,8 +366,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) attn_decode_kernel(const __
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {  // A: dims by keys, V transposed on the way
         uint32_t va[4];
-        const int r = lane % 8 + 8 * (lane / 16), x = 2 * d + (lane / 8) % 2;
-        ldsm4_t(vt + r * (D * 2) + ((x ^ (r & 7)) << 4), va);
+        const int r = lane % 8 + 8 * (lane / 16), x = 2 * (d % 4) + (lane / 8) % 2;
+        ldsm4_t(vt + d / 4 * kHalf + r * 128 + ((x ^ (r & 7)) << 4), va);
 #pragma unroll
         for (int nn = 0; nn < kN; ++nn) {
           mma16816<T>(o[d][nn], va, ph[nn][0], ph[nn][1]);
@@ -303,141 +376,201 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) attn_decode_kernel(const __
       }
       __syncwarp();  // the stage may be filled again
     }
-    cp_wait<0>();
 
-    // ---- the warps' shares -------------------------------------------------------------------
+    // ---- the end of a request's part ------------------------------------------------------
+    const bool wrong = cur.bad || dead;
+    if (cur.bad && lane == 0) report(a.status, MKB_SERVE_BAD_LENGTH);
+    const bool whole = t0 == 0 && t1 == cur.n;
+    const int which = t0 == 0;
+    uint32_t odd = 0;  // rows whose O is not finite
 #pragma unroll
     for (int nn = 0; nn < kN; ++nn)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) l[nn][e] += __shfl_xor_sync(0xffffffffu, l[nn][e], w);
-        if (lane < 4) {
-          red_m[warp][8 * nn + 2 * lane + e] = m[nn][e];
-          red_l[warp][8 * nn + 2 * lane + e] = l[nn][e];
-        }
-      }
-    if (threadIdx.x == 0) odd_rows = 0;
-    const bool page_out = __syncthreads_or(page_bad != 0);
-    float* buf = reinterpret_cast<float*>(smem);  // [warp][D][8 kN], over the ring
-#pragma unroll
-    for (int nn = 0; nn < kN; ++nn)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
+        if (wrong) l[nn][e] = NAN;
         const int r = 8 * nn + 2 * (lane % 4) + e;
-        float mm = -INFINITY;
+        float z = 0.f;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) mm = fmaxf(mm, red_m[w][r]);
-        const float f = ex2_approx(m[nn][e] - (mm == -INFINITY ? 0.f : mm));
+        for (int d = 0; d < D / 16; ++d) z = fmaf(o[d][nn][e], 0.f, fmaf(o[d][nn][2 + e], 0.f, z));
+        if (z != 0.f) odd |= 1u << r;
+        if (whole) {
+          if (r < g.rows) {
+            const int tok = r / g.group, h = hk * g.group + r - tok * g.group;
+            const bool zero = lim[nn][e] < 0 && !wrong;  // a row that sees no key
+            const float inv = 1.f / l[nn][e];
+            uint16_t* out = reinterpret_cast<uint16_t*>(static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.q_len + tok) * a.out_stride[0] +
+                                                        h * a.out_stride[1]);
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-          buf[(warp * D + 16 * d + lane / 4) * (8 * kN) + r] = o[d][nn][e] * f;
-          buf[(warp * D + 16 * d + 8 + lane / 4) * (8 * kN) + r] = o[d][nn][2 + e] * f;
+            for (int d = 0; d < D / 16; ++d) {
+              const uint32_t w2 = Pair<T>::put(o[d][nn][e] * inv, o[d][nn][2 + e] * inv);
+              out[16 * d + lane / 4] = zero ? 0 : static_cast<uint16_t>(w2);
+              out[16 * d + 8 + lane / 4] = zero ? 0 : static_cast<uint16_t>(w2 >> 16);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            if (r < g.cols) {
+              part_o[which][(16 * d + lane / 4) * g.cols + r] = o[d][nn][e];
+              part_o[which][(16 * d + 8 + lane / 4) * g.cols + r] = o[d][nn][2 + e];
+            }
+          }
+          if (lane < 4) {
+            part_m[warp][which][r] = m[nn][e];
+            part_l[warp][which][r] = l[nn][e];
+          }
         }
       }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == n;
-    const bool wrong = bad || page_out;
-    if (threadIdx.x == 0 && wrong) report(a.status, bad ? MKB_SERVE_BAD_LENGTH : MKB_SERVE_BAD_PAGE);
-    // (first part: slot 2 cta + 1, others: slot 2 cta)
-    const int slot = 2 * cta + (t0 == 0);
-    for (int i = threadIdx.x; i < D * 8 * kN; i += 32 * kDecWarps) {
-      const int r = i % (8 * kN);
-      if (r >= g.rows) continue;
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) v += buf[w * D * 8 * kN + i];
-      float mm = -INFINITY, ll = 0.f;
-#pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) mm = fmaxf(mm, red_m[w][r]);
-#pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) ll += red_l[w][r] * ex2_approx(red_m[w][r] - (mm == -INFINITY ? 0.f : mm));
-      if (wrong) ll = NAN;
-      if (a.q_len > 1 && v * 0.f != 0.f) atomicOr(&odd_rows, 1u << r);
-      if (whole) {
-        const int d = i / (8 * kN), tok = r / g.group, h = hk * g.group + r - tok * g.group;
-        const bool zero = first_pos + tok < 0 && !wrong;
-        T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.q_len + tok) * a.out_stride[0] + h * a.out_stride[1];
-        const uint32_t w2 = Pair<T>::put(zero ? 0.f : v / ll, 0.f);
-        reinterpret_cast<uint16_t*>(out)[d] = static_cast<uint16_t>(w2 & 0xffffu);
-      } else {
-        g.part[static_cast<size_t>(slot) * D * 16 + i] = v;
-        if (i < 8 * kN) {
-          g.stat[slot * 32 + r] = mm;
-          g.stat[slot * 32 + 16 + r] = ll;
-        }
-      }
+    if (!whole && lane == 0) {
+      part_pos[warp][which] = cur.pos;
+      part_at[warp][which][0] = b;
+      part_at[warp][which][1] = hk;
+      part_at[warp][which][2] = len;
+      part_at[warp][which][3] = cur.n;
     }
     // Where rows see different keys, V that is not finite reaches those that do not see it:
     // such rows are computed again key by key.
     if (a.q_len > 1) {
-      __syncthreads();
-      for (int r = warp; r < g.rows && !wrong; r += kDecWarps) {
-        if (!(odd_rows >> r & 1u)) continue;
+      odd = __reduce_or_sync(0xffffffffu, odd);
+      __syncwarp();
+      while (odd != 0) {
+        const int r = __ffs(odd) - 1;
+        odd &= odd - 1;
+        if (r >= g.rows || wrong) continue;
         const int tok = r / g.group, h = hk * g.group + r - tok * g.group;
-        constexpr int kPer = D / 32;
         float x[kPer], mm, ll;
         row_by_key<T, D, true>(a, g.sl2, b, 0, b * a.q_len + tok, h, hk, t0 * kTileKeys,
                                min(min(t1 * kTileKeys, len), first_pos + tok + 1), x, &mm, &ll);
+        T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.q_len + tok) * a.out_stride[0] + h * a.out_stride[1];
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           const int d = lane * kPer + i;
-          if (whole) {
-            T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.q_len + tok) * a.out_stride[0] + h * a.out_stride[1];
-            const uint32_t w2 = Pair<T>::put(first_pos + tok < 0 ? 0.f : x[i] / ll, 0.f);
-            reinterpret_cast<uint16_t*>(out)[d] = static_cast<uint16_t>(w2 & 0xffffu);
-          } else {
-            g.part[static_cast<size_t>(slot) * D * 16 + d * 8 * kN + r] = x[i];
-          }
+          if (whole) reinterpret_cast<uint16_t*>(out)[d] = static_cast<uint16_t>(Pair<T>::put(first_pos + tok < 0 ? 0.f : x[i] / ll, 0.f));
+          else part_o[which][d * g.cols + r] = x[i];
         }
         if (!whole && lane == 0) {
-          g.stat[slot * 32 + r] = mm;
-          g.stat[slot * 32 + 16 + r] = ll;
+          part_m[warp][which][r] = mm;
+          part_l[warp][which][r] = ll;
         }
       }
     }
-    if (!whole) {
-      int c0 = cta, c1 = cta;  // the CTAs of the request's first and last stretch for this KV head
-      while (cut(c0) > pos) --c0;
-      while (cut(c1 + 1) < pos + n) ++c1;
+  }
+  for (int i = 0; dead && i < 1000; ++i) __nanosleep(100000);  // (copies still in flight)
+  __syncthreads();
+  if (threadIdx.x == 0 && err) report(a.status, MKB_SERVE_TIMEOUT);
+
+  // ---- requests that several warps have parts of --------------------------------------------
+  for (int w0 = 0; w0 < 2 * kDecWarps;) {  // parts in order of their keys: warp w0 / 2, part w0 % 2
+    const int64_t pos = part_pos[w0 / 2][w0 % 2];
+    if (pos < 0) {
+      ++w0;
+      continue;
+    }
+    int w1 = w0 + 1;  // the parts of the same request and KV head: up to here
+    while (w1 < 2 * kDecWarps && (part_pos[w1 / 2][w1 % 2] == pos || part_pos[w1 / 2][w1 % 2] < 0)) ++w1;
+    const int* at = part_at[w0 / 2][w0 % 2];
+    const int b = at[0], hk = at[1], len = at[2], n = at[3];
+    // the weight of every part's rows, relative to the largest maximum: [part][row], sums in row 16 + r
+    float* const fac = fac_mem;
+    const bool begins = tile_at(cta_from, pos, n) == 0, ends = tile_at(cta_from + cta_units, pos, n) == n;
+    const bool here = begins && ends;  // all of it in this CTA
+    const int slot = 2 * cta + begins;
+    __syncthreads();
+    if (threadIdx.x < 16) {
+      const int r = threadIdx.x;
+      float mm = -INFINITY, ll = 0.f;
+      for (int w = w0; w < w1; ++w)
+        if (part_pos[w / 2][w % 2] == pos) mm = fmaxf(mm, part_m[w / 2][w % 2][r]);
+      const float ref = mm == -INFINITY ? 0.f : mm;
+      for (int w = w0; w < w1; ++w) {
+        const bool is = part_pos[w / 2][w % 2] == pos;
+        const float f = is ? ex2_approx(part_m[w / 2][w % 2][r] - ref) : 0.f;
+        if (is) ll += part_l[w / 2][w % 2][r] * f;
+        fac[w * 16 + r] = f;
+      }
+      const int tok = r / g.group;
+      fac[2 * kDecWarps * 16 + r] = len - a.q_len + tok < 0 && ll == ll ? 0.f : 1.f / ll;
+      if (!here && r < g.rows) {
+        g.stat[slot * 32 + r] = mm;
+        g.stat[slot * 32 + 16 + r] = ll;
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < D * g.cols; i += 32 * kDecWarps) {
+      const int r = i & (g.cols - 1);
+      if (r >= g.rows) continue;
+      float v = 0.f;
+      for (int w = w0; w < w1; ++w) {
+        if (part_pos[w / 2][w % 2] != pos) continue;
+        const uint8_t* base = smem + (w / 2) * g.warp_bytes + (w % 2 == 0 ? g.stages * kBytes : 0);
+        v += reinterpret_cast<const float*>(base)[i] * fac[w * 16 + r];
+      }
+      const int d = i / g.cols, tok = r / g.group, h = hk * g.group + r - tok * g.group;
+      if (here) {
+        T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.q_len + tok) * a.out_stride[0] + h * a.out_stride[1];
+        const float f = fac[2 * kDecWarps * 16 + r];
+        reinterpret_cast<uint16_t*>(out)[d] = static_cast<uint16_t>(Pair<T>::put(f == 0.f ? 0.f : v * f, 0.f));
+      } else {
+        g.part[static_cast<size_t>(slot) * D * 16 + i] = v;
+      }
+    }
+    if (!here) {
+      int c0 = cta, c1 = cta;  // the CTAs of its first and last part
+      while (tile_at(cut(c0), pos, n) > 0) --c0;
+      while (tile_at(cut(c1 + 1), pos, n) < n) ++c1;
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) flag = atomicInc(g.counters + c0, c1 - c0) == static_cast<uint32_t>(c1 - c0);
       __syncthreads();
       if (flag) {
         __threadfence();
-        for (int i = threadIdx.x; i < D * 8 * kN; i += 32 * kDecWarps) {
-          const int r = i % (8 * kN);
-          if (r >= g.rows) continue;
-          float mm = -INFINITY, ll = 0.f, v = 0.f;
-          for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, __ldcg(g.stat + (2 * c + (c == c0)) * 32 + r));
+        // as above, over the CTAs: a warp a row, a lane a part
+        for (int r = warp; r < g.rows; r += kDecWarps) {
+          float mm = -INFINITY, ll = 0.f;
+          for (int c = c0 + lane; c <= c1; c += 32) mm = fmaxf(mm, __ldcg(g.stat + (2 * c + (c == c0)) * 32 + r));
+#pragma unroll
+          for (int w = 16; w > 0; w >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, w));
           const float ref = mm == -INFINITY ? 0.f : mm;
+          for (int c = c0 + lane; c <= c1; c += 32) {
+            const float* st = g.stat + (2 * c + (c == c0)) * 32 + r;
+            ll += __ldcg(st + 16) * ex2_approx(__ldcg(st) - ref);
+          }
+#pragma unroll
+          for (int w = 16; w > 0; w >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, w);
+          if (lane == 0) {
+            fac[r] = ref;
+            fac[2 * kDecWarps * 16 + r] = len - a.q_len + r / g.group < 0 && ll == ll ? 0.f : 1.f / ll;
+          }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < D * g.cols; i += 32 * kDecWarps) {
+          const int r = i & (g.cols - 1);
+          if (r >= g.rows) continue;
+          float v = 0.f;
+#pragma unroll 4
           for (int c = c0; c <= c1; ++c) {
             const int s = 2 * c + (c == c0);
-            const float f = ex2_approx(__ldcg(g.stat + s * 32 + r) - ref);
-            ll += __ldcg(g.stat + s * 32 + 16 + r) * f;
-            v += __ldcg(g.part + static_cast<size_t>(s) * D * 16 + i) * f;
+            v += __ldcg(g.part + static_cast<size_t>(s) * D * 16 + i) * ex2_approx(__ldcg(g.stat + s * 32 + r) - fac[r]);
           }
-          const int d = i / (8 * kN), tok = r / g.group, h = hk * g.group + r - tok * g.group;
+          const int d = i / g.cols, tok = r / g.group, h = hk * g.group + r - tok * g.group;
           T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.q_len + tok) * a.out_stride[0] + h * a.out_stride[1];
-          const uint32_t w2 = Pair<T>::put(first_pos + tok < 0 ? 0.f : v / ll, 0.f);
-          reinterpret_cast<uint16_t*>(out)[d] = static_cast<uint16_t>(w2 & 0xffffu);
+          const float f = fac[2 * kDecWarps * 16 + r];
+          reinterpret_cast<uint16_t*>(out)[d] = static_cast<uint16_t>(Pair<T>::put(f == 0.f ? 0.f : v * f, 0.f));
         }
       }
     }
-    __syncthreads();  // the ring and the reductions are free again
-    // on to the next stretch
-    pos += n;
-    if (++hk == a.kv_heads) {
-      hk = 0;
-      if (++b < a.batch) n = dec_tiles(g, b, &len, &bad);
-    }
+    __syncthreads();  // fac is free again
+    w0 = w1;
   }
 }
 
 // ---- host side -----------------------------------------------------------------------
 
-int sm_count();  // mkb_attn_tc.cu
+int sm_count();  // these three: mkb_attn_tc.cu
+cudaError_t map_rows(CUtensorMap* m, int dtype, const void* base, int D, int rank, const uint64_t* dims,
+                     const int64_t* strides, const uint32_t* box);
 size_t counter_bytes();
 
 size_t decode_workspace(const mkb_attn_args& a) {
@@ -449,6 +582,8 @@ static cudaError_t decode_launch(const mkb_attn_args& a, cudaStream_t stream) {
   DecArgs g;
   g.a = a;
   g.sl2 = a.scale * 1.4426950408889634f;
+  g.k_head = a.k_stride[1] != 0;
+  g.v_head = a.v_stride[1] != 0;
   g.group = a.heads / a.kv_heads;
   g.rows = a.q_len * g.group;
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
@@ -456,23 +591,38 @@ static cudaError_t decode_launch(const mkb_attn_args& a, cudaStream_t stream) {
   g.counters = reinterpret_cast<uint32_t*>(ws);
   g.stat = reinterpret_cast<float*>(ws + counter_bytes());
   g.part = g.stat + 2 * static_cast<size_t>(sm_count()) * 32;
-  constexpr size_t ring = DecShape<D>::kSmem, sums = static_cast<size_t>(kDecWarps) * D * 8 * kN * 4;
-  constexpr size_t bytes = ring > sums ? ring : sums;
+  for (g.cols = 2; g.cols < g.rows;) g.cols *= 2;
+  // as many tiles of 128-wide (64-wide) heads as the part beside them leaves room for (a part
+  // is smaller than any of these rings, which the last one lies over)
+  g.stages = D == 64 ? (g.cols <= 8 ? kMaxStages : kMaxStages - 1) : g.cols <= 4 ? 3 : 2;
+  g.warp_bytes = (g.stages * kStageBytes<D> + D * g.cols * 4 + 1023) / 1024 * 1024;  // (swizzle atoms)
+  constexpr size_t most_bytes = 216 * 1024;
+  const size_t bytes = static_cast<size_t>(kDecWarps) * g.warp_bytes + 1024;
   static bool configured[64] = {false};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  CUtensorMap mk, mv;
+  const void* kb = a.pages > 0 ? a.k : a.q;  // an empty pool is never read: any address will do
+  const void* vb = a.pages > 0 ? a.v : a.q;
+  const uint64_t dims[3] = {static_cast<uint64_t>(a.page_size), static_cast<uint64_t>(a.kv_heads),
+                            static_cast<uint64_t>(a.pages)};
+  const int64_t ks[3] = {a.k_stride[2], a.k_stride[1], a.k_stride[0]};
+  const int64_t vs[3] = {a.v_stride[2], a.v_stride[1], a.v_stride[0]};
+  const uint32_t box[3] = {kTileKeys, 1, 1};
+  if ((e = map_rows(&mk, a.dtype, kb, D, 3, dims, ks, box)) != cudaSuccess) return e;
+  if ((e = map_rows(&mv, a.dtype, vb, D, 3, dims, vs, box)) != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(attn_decode_kernel<T, D, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    e = cudaFuncSetAttribute(attn_decode_kernel<T, D, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most_bytes));
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
   // a CTA for every SM that the tiles could keep busy
   const int64_t most = static_cast<int64_t>(a.batch) * a.kv_heads *
-                       (static_cast<int64_t>(a.table_width) * a.page_size / (kTileKeys * kDecTileMin) + 1);
+                       (static_cast<int64_t>(a.table_width) * a.page_size / (kTileKeys * kCtaTiles) + 1);
   const int grid = static_cast<int>(most < sm_count() ? most : sm_count());
-  return launch_early(attn_decode_kernel<T, D, kN>, grid, 32 * kDecWarps, bytes, stream, g);
+  return launch_early(attn_decode_kernel<T, D, kN>, grid, 32 * kDecWarps, bytes, stream, mk, mv, g);
 }
 
 // Few enough rows a KV head for one tile of columns.

@@ -137,12 +137,6 @@ __device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t ph, int* err, b
   }
 }
 
-__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
-      : "memory");
-}
 __device__ __forceinline__ void tma_store_3d(const void* src, const CUtensorMap* map, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];\n\t"
                "cp.async.bulk.commit_group;"
@@ -152,13 +146,6 @@ __device__ __forceinline__ void tma_store_3d(const void* src, const CUtensorMap*
 // this thread's stores: their shared memory has been read / they are done
 __device__ __forceinline__ void tma_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w),
-      "r"(smem_addr(bar))
-      : "memory");
-}
 
 // Descriptor of an operand whose contiguous dimension is N, written by TMA with the
 // 128-byte swizzle: 64 values of N a row, eight rows (of K) to an atom of 1024 bytes;
@@ -542,13 +529,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
 #pragma unroll
             for (int d = 0; d < D / 64; ++d)
-              tma_4d(sm.kv[s] + d * kHalf + lane * box * 128, map, 64 * d, at % a.page_size, head, page,
+              tc::tma_load_4d(sm.kv[s] + d * kHalf + lane * box * 128, map, 64 * d, at % a.page_size, head, page,
                      &sm.kv_full[s]);
           }
         } else if (lane == 0) {
 #pragma unroll
           for (int d = 0; d < D / 64; ++d)
-            tma_3d(sm.kv[s] + d * kHalf, map, 64 * d, p.first + key, head, &sm.kv_full[s]);
+            tc::tma_load_3d(sm.kv[s] + d * kHalf, map, 64 * d, p.first + key, head, &sm.kv_full[s]);
         }
       };
       const int kh = p.hk * g.k_head, vh = p.hk * g.v_head;
@@ -562,7 +549,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           mbar_arrive_expect_tx(&sm.q_full[t], g.tile_tokens * g.group * D * 2);
 #pragma unroll
           for (int d = 0; d < D / 64; ++d)
-            tma_3d(sm.q[t] + d * kHalf, &tq, 64 * d, p.hk * g.group, p.first + p.tok0 + (p.halves ? 0 : t * g.tile_tokens),
+            tc::tma_load_3d(sm.q[t] + d * kHalf, &tq, 64 * d, p.hk * g.group, p.first + p.tok0 + (p.halves ? 0 : t * g.tile_tokens),
                    &sm.q_full[t]);
         }
         __syncwarp();
@@ -1045,7 +1032,7 @@ static EncodeTiled encoder() {
 
 // Rows of 64 values (of D); the dimensions after the row's are `dims` with strides of
 // `strides` elements, a copy takes `box` of each. What lies outside reads as zeros.
-static cudaError_t map_rows(CUtensorMap* m, int dtype, const void* base, int D, int rank, const uint64_t* dims,
+cudaError_t map_rows(CUtensorMap* m, int dtype, const void* base, int D, int rank, const uint64_t* dims,
                             const int64_t* strides, const uint32_t* box) {
   const EncodeTiled enc = encoder();
   if (!enc) return cudaErrorNotSupported;

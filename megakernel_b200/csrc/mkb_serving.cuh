@@ -108,7 +108,10 @@ __device__ __noinline__ void row_by_key(const mkb_attn_args& a, float sl2, int b
     int64_t ko, vo;
     if (kPaged) {
       const int64_t page = a.block_table[b * a.table_stride + j / a.page_size], slot = j % a.page_size;
-      if (page < 0 || page >= a.pages) continue;  // reported; the row is NaN already
+      if (page < 0 || page >= a.pages) {  // reported already
+        l = NAN;
+        continue;
+      }
       ko = page * a.k_stride[0] + hk * a.k_stride[1] + slot * a.k_stride[2];
       vo = page * a.v_stride[0] + hk * a.v_stride[1] + slot * a.v_stride[2];
     } else {
