@@ -112,8 +112,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   __shared__ float part_m[kDecWarps][2][16], part_l[kDecWarps][2][16];
   __shared__ int64_t part_pos[kDecWarps][2];                   // the request's and KV head's place, -1: none
   __shared__ int part_at[kDecWarps][2][4];                     // b, hk, len, n
-  __shared__ float fac_mem[(2 * kDecWarps + 1) * 16];
-  __shared__ int flag, err;
+  __shared__ float fac[2 * kDecWarps][16], sum_m[2 * kDecWarps][16], sum_l[2 * kDecWarps][16];
+  __shared__ int flags[2][2], err;
   const mkb_attn_args& a = g.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   depend_launch();
@@ -135,15 +135,24 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   // ---- the work, and this warp's range of it ----------------------------------------------
   int len0 = 0;
   bool bad0 = false;
-  const int tiles0 = lane < a.batch ? dec_tiles(g, lane, &len0, &bad0) + 1 : 0;  // (a lane keeps its first request's)
-  int64_t total = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    int n = tiles0, x;
+  auto units = [&](int b, int* len, bool* bad) {
+    return b < a.batch ? static_cast<int64_t>(dec_tiles(g, b, len, bad) + 1) * a.kv_heads : 0;
+  };
+  auto upto = [&](int64_t x) {  // sums over the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    return x;
+  };
+  const int64_t units0 = units(lane, &len0, &bad0), upto0 = upto(units0);  // (a lane keeps its first request's)
+  int64_t total = __shfl_sync(0xffffffffu, upto0, 31);
+  for (int b0 = 32; b0 < a.batch; b0 += 32) {
+    int x;
     bool y;
-    if (b0 > 0) n = b0 + lane < a.batch ? dec_tiles(g, b0 + lane, &x, &y) + 1 : 0;
-    total += __reduce_add_sync(0xffffffffu, n);
+    total += __shfl_sync(0xffffffffu, upto(units(b0 + lane, &x, &y)), 31);
   }
-  total *= a.kv_heads;
   const int64_t heads = static_cast<int64_t>(a.batch) * a.kv_heads;
   const int ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x),
                                         total > heads * kLongTiles ? max(total / kCtaTiles, heads) : heads));
@@ -157,21 +166,18 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   ahead.b = a.batch;
   ahead.pos = 0;
   for (int b0 = 0; b0 < a.batch && from < to; b0 += 32) {
-    int t = tiles0, ln = len0;
+    int64_t own = units0, inc = upto0;
+    int ln = len0;
     bool bd = bad0;
-    if (b0 > 0) t = b0 + lane < a.batch ? dec_tiles(g, b0 + lane, &ln, &bd) + 1 : 0;
-    int64_t inc = static_cast<int64_t>(t) * a.kv_heads;
-    const int64_t own = inc;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += y;
+    if (b0 > 0) {
+      own = units(b0 + lane, &ln, &bd);
+      inc = upto(own);
     }
     const uint32_t who = __ballot_sync(0xffffffffu, from - ahead.pos < inc);
     if (who != 0) {
       const int src = __ffs(who) - 1;
       ahead.b = b0 + src;
-      ahead.n = __shfl_sync(0xffffffffu, t, src) - 1;
+      ahead.n = static_cast<int>(__shfl_sync(0xffffffffu, own, src) / a.kv_heads) - 1;
       ahead.len = __shfl_sync(0xffffffffu, ln, src);
       ahead.bad = __shfl_sync(0xffffffffu, static_cast<int>(bd), src) != 0;
       ahead.pos += __shfl_sync(0xffffffffu, inc - own, src);
@@ -461,108 +467,133 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   __syncthreads();
   if (threadIdx.x == 0 && err) report(a.status, MKB_SERVE_TIMEOUT);
 
+  // value i (a dim of a row) of a request: the sum v over the weights' sum
+  auto write_out = [&](int b, int hk, int len, int i, float v, float ll) {
+    const int r = i & (g.cols - 1), d = i / g.cols, tok = r / g.group, h = hk * g.group + r - tok * g.group;
+    const float x = len - a.q_len + tok < 0 && ll == ll ? 0.f : v / ll;  // (a row that sees no key is zero)
+    reinterpret_cast<uint16_t*>(static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.q_len + tok) * a.out_stride[0] +
+                                h * a.out_stride[1])[d] = static_cast<uint16_t>(Pair<T>::put(x, 0.f));
+  };
+
   // ---- requests that several warps have parts of --------------------------------------------
-  for (int w0 = 0; w0 < 2 * kDecWarps;) {  // parts in order of their keys: warp w0 / 2, part w0 % 2
-    const int64_t pos = part_pos[w0 / 2][w0 % 2];
-    if (pos < 0) {
-      ++w0;
-      continue;
+  // Part p = 2 warp + (0 or 1), in order of their keys; those of one request and KV head are
+  // neighbours. First every part's weight beside the largest maximum of its row, a lane a part:
+  constexpr int kParts = 2 * kDecWarps;
+  const int64_t my_pos = lane < kParts ? part_pos[lane / 2][lane % 2] : -1;
+  uint32_t same = 0;  // the parts that go with the lane's
+#pragma unroll
+  for (int j = 0; j < kParts; ++j) {
+    const int64_t x = __shfl_sync(0xffffffffu, my_pos, j);
+    if (my_pos >= 0 && x == my_pos) same |= 1u << j;
+  }
+  const uint32_t firsts = __ballot_sync(0xffffffffu, my_pos >= 0 && (same & ((1u << lane) - 1)) == 0);
+  if (firsts == 0) return;  // (the same for every warp)
+  for (int r = warp; r < g.rows; r += kDecWarps) {
+    const float m = my_pos >= 0 ? part_m[lane / 2][lane % 2][r] : -INFINITY;
+    float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+    for (int j = 0; j < kParts; ++j) {
+      const float x = __shfl_sync(0xffffffffu, m, j);
+      if (same >> j & 1u) mm = fmaxf(mm, x);
     }
-    int w1 = w0 + 1;  // the parts of the same request and KV head: up to here
-    while (w1 < 2 * kDecWarps && (part_pos[w1 / 2][w1 % 2] == pos || part_pos[w1 / 2][w1 % 2] < 0)) ++w1;
-    const int* at = part_at[w0 / 2][w0 % 2];
+    const float f = ex2_approx(m - (mm == -INFINITY ? 0.f : mm));
+    const float l = my_pos >= 0 ? part_l[lane / 2][lane % 2][r] * f : 0.f;
+#pragma unroll
+    for (int j = 0; j < kParts; ++j) {
+      const float x = __shfl_sync(0xffffffffu, l, j);
+      if (same >> j & 1u) ll += x;
+    }
+    if (lane < kParts) {
+      fac[lane][r] = f;
+      sum_m[lane][r] = mm;
+      sum_l[lane][r] = ll;
+    }
+  }
+  __syncthreads();
+  // then the sums: written out where the CTA has all of a request's keys, else left in memory
+  // (that can be the CTA's first and its last: `cross`)
+  int cross[2], crosses = 0;
+  for (uint32_t todo = firsts; todo != 0; todo &= todo - 1) {
+    const int p0 = __ffs(todo) - 1;
+    const uint32_t parts = __shfl_sync(0xffffffffu, same, p0);
+    const int64_t pos = part_pos[p0 / 2][p0 % 2];
+    const int* at = part_at[p0 / 2][p0 % 2];
     const int b = at[0], hk = at[1], len = at[2], n = at[3];
-    // the weight of every part's rows, relative to the largest maximum: [part][row], sums in row 16 + r
-    float* const fac = fac_mem;
-    const bool begins = tile_at(cta_from, pos, n) == 0, ends = tile_at(cta_from + cta_units, pos, n) == n;
-    const bool here = begins && ends;  // all of it in this CTA
+    const bool begins = tile_at(cta_from, pos, n) == 0, here = begins && tile_at(cta_from + cta_units, pos, n) == n;
     const int slot = 2 * cta + begins;
-    __syncthreads();
-    if (threadIdx.x < 16) {
-      const int r = threadIdx.x;
-      float mm = -INFINITY, ll = 0.f;
-      for (int w = w0; w < w1; ++w)
-        if (part_pos[w / 2][w % 2] == pos) mm = fmaxf(mm, part_m[w / 2][w % 2][r]);
-      const float ref = mm == -INFINITY ? 0.f : mm;
-      for (int w = w0; w < w1; ++w) {
-        const bool is = part_pos[w / 2][w % 2] == pos;
-        const float f = is ? ex2_approx(part_m[w / 2][w % 2][r] - ref) : 0.f;
-        if (is) ll += part_l[w / 2][w % 2][r] * f;
-        fac[w * 16 + r] = f;
+    for (int i = threadIdx.x; i < D * g.cols; i += 32 * kDecWarps) {
+      const int r = i & (g.cols - 1);
+      if (r >= g.rows) continue;
+      float v = 0.f;
+      for (uint32_t u = parts; u != 0; u &= u - 1) {
+        const int p = __ffs(u) - 1;
+        const uint8_t* base = smem + (p / 2) * g.warp_bytes + (p % 2 == 0 ? g.stages * kBytes : 0);
+        v += reinterpret_cast<const float*>(base)[i] * fac[p][r];
       }
-      const int tok = r / g.group;
-      fac[2 * kDecWarps * 16 + r] = len - a.q_len + tok < 0 && ll == ll ? 0.f : 1.f / ll;
-      if (!here && r < g.rows) {
-        g.stat[slot * 32 + r] = mm;
-        g.stat[slot * 32 + 16 + r] = ll;
+      if (here) write_out(b, hk, len, i, v, sum_l[p0][r]);
+      else g.part[static_cast<size_t>(slot) * D * 16 + i] = v;
+    }
+    if (!here) {
+      if (threadIdx.x < g.rows) {
+        g.stat[slot * 32 + threadIdx.x] = sum_m[p0][threadIdx.x];
+        g.stat[slot * 32 + 16 + threadIdx.x] = sum_l[p0][threadIdx.x];
+      }
+      cross[crosses++ & 1] = p0;
+    }
+  }
+  if (crosses == 0) return;
+  __threadfence();
+  __syncthreads();
+  for (int x = 0; x < crosses; ++x) {
+    const int p0 = cross[x], n = part_at[p0 / 2][p0 % 2][3];
+    const int64_t pos = part_pos[p0 / 2][p0 % 2];
+    if (threadIdx.x == 32 * x) {
+      int c0 = cta, c1 = cta;  // the CTAs of its first and last part
+      while (tile_at(cut(c0), pos, n) > 0) --c0;
+      while (tile_at(cut(c1 + 1), pos, n) < n) ++c1;
+      const bool last = atomicInc(g.counters + c0, c1 - c0) == static_cast<uint32_t>(c1 - c0);
+      flags[x][0] = last ? c0 : -1;
+      flags[x][1] = c1;
+    }
+  }
+  __syncthreads();
+  for (int x = 0; x < crosses; ++x) {
+    const int c0 = flags[x][0], c1 = flags[x][1], p0 = cross[x];
+    if (c0 < 0) continue;
+    __threadfence();
+    const int* at = part_at[p0 / 2][p0 % 2];
+    const int b = at[0], hk = at[1], len = at[2];
+    for (int r = warp; r < g.rows; r += kDecWarps) {  // a warp a row, a lane a CTA
+      float mm = -INFINITY, ll = 0.f;
+      for (int c = c0 + lane; c <= c1; c += 32) mm = fmaxf(mm, __ldcg(g.stat + (2 * c + (c == c0)) * 32 + r));
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, w));
+      const float ref = mm == -INFINITY ? 0.f : mm;
+      for (int c = c0 + lane; c <= c1; c += 32) {
+        const float* st = g.stat + (2 * c + (c == c0)) * 32 + r;
+        ll += __ldcg(st + 16) * ex2_approx(__ldcg(st) - ref);
+      }
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, w);
+      if (lane == 0) {
+        sum_m[p0][r] = ref;
+        sum_l[p0][r] = ll;
       }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < D * g.cols; i += 32 * kDecWarps) {
       const int r = i & (g.cols - 1);
       if (r >= g.rows) continue;
+      const float ref = sum_m[p0][r];
       float v = 0.f;
-      for (int w = w0; w < w1; ++w) {
-        if (part_pos[w / 2][w % 2] != pos) continue;
-        const uint8_t* base = smem + (w / 2) * g.warp_bytes + (w % 2 == 0 ? g.stages * kBytes : 0);
-        v += reinterpret_cast<const float*>(base)[i] * fac[w * 16 + r];
+#pragma unroll 8
+      for (int c = c0; c <= c1; ++c) {
+        const int s = 2 * c + (c == c0);
+        v += __ldcg(g.part + static_cast<size_t>(s) * D * 16 + i) * ex2_approx(__ldcg(g.stat + s * 32 + r) - ref);
       }
-      const int d = i / g.cols, tok = r / g.group, h = hk * g.group + r - tok * g.group;
-      if (here) {
-        T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.q_len + tok) * a.out_stride[0] + h * a.out_stride[1];
-        const float f = fac[2 * kDecWarps * 16 + r];
-        reinterpret_cast<uint16_t*>(out)[d] = static_cast<uint16_t>(Pair<T>::put(f == 0.f ? 0.f : v * f, 0.f));
-      } else {
-        g.part[static_cast<size_t>(slot) * D * 16 + i] = v;
-      }
+      write_out(b, hk, len, i, v, sum_l[p0][r]);
     }
-    if (!here) {
-      int c0 = cta, c1 = cta;  // the CTAs of its first and last part
-      while (tile_at(cut(c0), pos, n) > 0) --c0;
-      while (tile_at(cut(c1 + 1), pos, n) < n) ++c1;
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) flag = atomicInc(g.counters + c0, c1 - c0) == static_cast<uint32_t>(c1 - c0);
-      __syncthreads();
-      if (flag) {
-        __threadfence();
-        // as above, over the CTAs: a warp a row, a lane a part
-        for (int r = warp; r < g.rows; r += kDecWarps) {
-          float mm = -INFINITY, ll = 0.f;
-          for (int c = c0 + lane; c <= c1; c += 32) mm = fmaxf(mm, __ldcg(g.stat + (2 * c + (c == c0)) * 32 + r));
-#pragma unroll
-          for (int w = 16; w > 0; w >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, w));
-          const float ref = mm == -INFINITY ? 0.f : mm;
-          for (int c = c0 + lane; c <= c1; c += 32) {
-            const float* st = g.stat + (2 * c + (c == c0)) * 32 + r;
-            ll += __ldcg(st + 16) * ex2_approx(__ldcg(st) - ref);
-          }
-#pragma unroll
-          for (int w = 16; w > 0; w >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, w);
-          if (lane == 0) {
-            fac[r] = ref;
-            fac[2 * kDecWarps * 16 + r] = len - a.q_len + r / g.group < 0 && ll == ll ? 0.f : 1.f / ll;
-          }
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < D * g.cols; i += 32 * kDecWarps) {
-          const int r = i & (g.cols - 1);
-          if (r >= g.rows) continue;
-          float v = 0.f;
-#pragma unroll 4
-          for (int c = c0; c <= c1; ++c) {
-            const int s = 2 * c + (c == c0);
-            v += __ldcg(g.part + static_cast<size_t>(s) * D * 16 + i) * ex2_approx(__ldcg(g.stat + s * 32 + r) - fac[r]);
-          }
-          const int d = i / g.cols, tok = r / g.group, h = hk * g.group + r - tok * g.group;
-          T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.q_len + tok) * a.out_stride[0] + h * a.out_stride[1];
-          const float f = fac[2 * kDecWarps * 16 + r];
-          reinterpret_cast<uint16_t*>(out)[d] = static_cast<uint16_t>(Pair<T>::put(f == 0.f ? 0.f : v * f, 0.f));
-        }
-      }
-    }
-    __syncthreads();  // fac is free again
-    w0 = w1;
+    __syncthreads();
   }
 }
 
