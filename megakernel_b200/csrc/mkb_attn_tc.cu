@@ -28,12 +28,12 @@
 // moves P stays below 2^8, which FP32 sums and 16-bit P hold without loss. P is rounded
 // to the operands' 16-bit type, as the output is: the same relative error.
 //
-// Work: a piece is (request, KV head, two tiles); its weight is its keys and a fixed
-// part. The pieces' weights are laid end to end and cut into as many equal ranges as
-// there are CTAs; a cut inside a long enough piece splits its keys. Every part of a split
-// piece leaves its O, maximum and sum in memory, and the last part to be done adds them
-// up in order of their keys, so results do not depend on timing. Every CTA works its range
-// out for itself from the lengths: no list is written, nothing is asked of the host.
+// Work: a piece is (request, KV head, one or two tiles of rows, a range of key tiles).
+// Every CTA works the list out for itself from the lengths, the longest pieces first, and
+// takes the next one whenever its loads have run through the last (a counter in memory).
+// Rows whose keys are more than a fair share are split over several pieces; each leaves its
+// O, maximum and sum in memory, and the last one to be done adds them up in order of their
+// keys, so results do not depend on timing. Nothing is asked of the host.
 //
 // Masked places: scores are replaced, not added to. V rows past the request's last key
 // are cleared in shared memory. V that is not finite and stands where some row of the
@@ -56,10 +56,8 @@ constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 constexpr int kRows = 256, kKeys = 128;   // rows of a piece (two tiles), keys of a tile
 constexpr int kFirstKeys = 96;            // of a tile's weights, what the second product starts on
 constexpr int kHalf = 128 * 128;          // 16 KB: 128 rows x 64 values, 128-byte swizzle
-constexpr int kMinSplit = 6;              // key tiles of a piece below which it is not split
-constexpr int kMinPart = 2;               // key tiles of a part
-constexpr int kFixed = 256;               // a piece's fixed part, in keys (about what its start and end take)
-constexpr int kMinShare = 384;            // the least weight that is worth a CTA
+constexpr int kMinSplit = 6;              // key tiles (turns, of one tile's rows) below which rows are not split
+constexpr int kSortBatch = 128;           // requests up to which pieces are taken longest first
 constexpr int kTryNs = 20000, kTries = 50000;  // bound of every wait: about a second
 
 struct Piece {
@@ -71,8 +69,7 @@ struct Piece {
   int k0, total;    // first key tile, how many
   int n[2];         // those of tiles A and B
   int halves;       // A and B have the same rows, and every other key tile
-  int splits, split;  // parts of the piece, and which this is
-  int cta0;           // the CTA of its first part
+  int splits, split, slot;  // ranges of the rows' keys, which this is, where the first leaves its results
   int bad;
 };
 
@@ -112,11 +109,11 @@ struct TcArgs {
   int warp_tokens;      // tokens of a warp's 32 rows, 0 where they are not whole
   int box;              // keys of a TMA box
   int k_head, v_head;   // 0 where every KV head lies at the same place (stride 0), else 1
-  // Parts of split pieces: a CTA has at most one that begins a piece (slot 2 cta + 1) and
-  // one that does not (slot 2 cta).
-  uint32_t* counters;   // [ctas][2], of the piece that the CTA begins, by tile; zero between calls
-  float4* part;         // [2 ctas][D / 4][256]
-  float2* stat;         // [2 ctas][256]: maximum, sum
+  unsigned tile_mul;    // x / tile_tokens is x * tile_mul >> 32, or one less (0: tile_tokens is 1)
+  uint32_t* work;       // the next piece, CTAs that have finished; both zero between calls
+  uint32_t* counters;   // [slots][2], of the splits that are done, by tile; zero between calls
+  float4* part;         // [slots][D / 4][256]
+  float2* stat;         // [slots][256]: maximum, sum
 };
 
 // A warp's wait for a phase of a barrier. Bounded: each try suspends for 20 us at most.
@@ -276,11 +273,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// ---- the pieces, worked out by one warp ------------------------------------------------
+// ---- the list of pieces, worked out by one warp -------------------------------------
 
-// One request as the work sees it.
+// One request as the list sees it.
 struct Load {
-  int first, q, len, ctx, blocks, bad;
+  int first, q, len, ctx, tiles, bad;
 };
 template <bool kPaged>
 __device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
@@ -291,8 +288,7 @@ __device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
   l.len = kPaged ? max(__ldg(g.a.kv_lens + b), 0) : rq.n;
   l.bad = kPaged && static_cast<int64_t>(l.len) > static_cast<int64_t>(g.a.table_width) * g.a.page_size;
   l.ctx = l.len - l.q;
-  const unsigned span = 2 * g.tile_tokens;
-  l.blocks = static_cast<int>((static_cast<unsigned>(l.q) + span - 1) / span);
+  l.tiles = l.bad || l.q == 0 ? 0 : static_cast<int>((static_cast<unsigned>(l.len) + kKeys - 1) / kKeys);
   return l;
 }
 // key tiles that the first `toks` tokens of the request see
@@ -300,30 +296,30 @@ __device__ __forceinline__ int tiles_of(const Load& l, int toks) {
   const int keys = l.ctx + min(toks, l.q);
   return l.bad || keys <= 0 ? 0 : static_cast<int>((static_cast<unsigned>(keys) + kKeys - 1) / kKeys);
 }
-// Weight of a request's blocks [0, i) of one KV head; block i weighs kFixed + the keys
-// before the request's new tokens + (i + 1) span, where there are rows for one tile (its
-// keys then take half the time) kFixed + half of them. (`even`: each block the same.)
-__device__ __forceinline__ int64_t weight_to(const Load& l, int span, bool even, int i) {
-  const int64_t n = i;
-  if (even) return n;
-  if (2 * l.q <= span) return n * (kFixed + (max(l.ctx, 0) + span) / 2);
-  return n * (kFixed + max(l.ctx, 0)) + span * (n * (n + 1) / 2);
-}
-// Where the work is cut: what lies before CTA c's range. (Any function that all CTAs
-// agree on and that grows with c would do.)
-__device__ __forceinline__ int64_t cut_at(int64_t total, int ctas, double per, int c) {
-  return c >= ctas ? total : static_cast<int64_t>(per * c);
-}
-// A cut `y` into a piece of weight `w` as a key tile of its `n`, short ends left out. The
-// tiles of a piece that is split weigh at most 256 each, a range at least kMinShare: two
-// cuts of one piece never fall together, except at its ends.
-__device__ __forceinline__ int cut_tile(int64_t y, int64_t w, int n) {
-  if (y <= 0) return 0;
-  if (y >= w) return n;
-  if (n < kMinSplit || w > 256 * static_cast<int64_t>(n)) return 2 * y >= w ? n : 0;
-  const int t = static_cast<int>(static_cast<float>(y) / static_cast<float>(w) * n + 0.5f);
-  return t < kMinPart ? 0 : t > n - kMinPart ? n : t;
-}
+// Blocks of `span` tokens, `tiles` tiles of rows each (1 or 2).
+struct Blocks {
+  int tiles, span;
+  unsigned tile_mul;
+  __device__ __forceinline__ int over(unsigned x) const {  // x / span
+    const unsigned y = tiles == 2 ? x >> 1 : x;  // (span = tiles * tile_tokens)
+    if (tile_mul == 0) return y;
+    int i = __umulhi(y, tile_mul);
+    return i * (span >> (tiles - 1)) > y ? i - 1 : i;
+  }
+  __device__ __forceinline__ int of(const Load& l) const { return l.q > 0 ? over(l.q - 1) + 1 : 0; }
+  // turns that a block with n key tiles takes: rows for one tile take two at a time
+  __device__ __forceinline__ int turns(const Load& l, int n) const {
+    return tiles == 1 || 2 * l.q <= span ? (n + 1) / 2 : n;
+  }
+  // how many of the request's blocks take more than x turns (they come last)
+  __device__ __forceinline__ int above(const Load& l, int x) const {
+    if (x < 0) return of(l);
+    if (turns(l, l.tiles) <= x) return 0;
+    const int n = tiles == 1 || 2 * l.q <= span ? 2 * x : x;  // more than n key tiles
+    const int y = n * kKeys - l.ctx;                          // the first token that sees more (n < tiles: no overflow)
+    return y <= 0 ? of(l) : of(l) - over(y);
+  }
+};
 
 template <typename T, int D, bool kPaged>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -384,114 +380,127 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc::prefetch_tensormap(&tv);
       tc::prefetch_tensormap(&tq);
     }
-    const int kv_heads = a.kv_heads, span = 2 * g.tile_tokens;
+    const int kv_heads = a.kv_heads, grid = gridDim.x;
     auto request = [&](int b) { return b < 32 ? mine : load_of<kPaged>(g, b); };  // of lane b % 32
-    // all there is to do; pieces that are short and few have a CTA each
-    int64_t total = 0;
-    int pieces = 0, top = 0;
+    // pieces of more than x turns each, all requests
+    Blocks blocks = {2, 2 * g.tile_tokens, g.tile_mul};
+    int cap = 0x3fffffff;
+    auto splits_of = [&](const Load& l) {  // (rows that stand before position 0 have no keys to split)
+      const int n = blocks.turns(l, l.tiles);
+      return n > cap && l.ctx >= 0 ? (n + cap - 1) / cap : 1;
+    };
+    auto pieces_above = [&](int x) {
+      int n = 0;
+      for (int b = lane; b < a.batch; b += 32) {
+        const Load l = request(b);
+        const int sp = splits_of(l);
+        n += blocks.above(l, x * sp) * sp;
+      }
+      return __reduce_add_sync(0xffffffffu, n) * kv_heads;
+    };
+    // pairs of tiles, unless those are fewer than the CTAs: then single ones
+    if (pieces_above(-1) <= grid) blocks = {1, g.tile_tokens, g.tile_mul};
+    // a fair share of the turns; rows with more are split
+    float total = 0.f;
     for (int b = lane; b < a.batch; b += 32) {
-      const Load l = request(b);
-      total += weight_to(l, span, false, l.blocks);
-      pieces += l.blocks;
-      top = max(top, l.blocks > 0 ? tiles_of(l, l.q) : 0);
+      const Load l = request(b);  // (linear in the block)
+      const int n = blocks.turns(l, l.tiles);
+      total += 0.5f * (blocks.turns(l, tiles_of(l, blocks.span)) + n) * blocks.of(l);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    pieces = __reduce_add_sync(0xffffffffu, pieces) * kv_heads;
-    top = __reduce_max_sync(0xffffffffu, top);
-    const bool even = pieces <= static_cast<int>(gridDim.x) && top < kMinSplit;
-    total = even ? pieces : total * kv_heads;
-    const int ctas = even ? pieces : static_cast<int>(min(static_cast<int64_t>(gridDim.x), max(total / kMinShare, static_cast<int64_t>(1))));
-    const double per = static_cast<double>(total) / ctas;
-    const int cta = blockIdx.x;
-    const bool work = cta < ctas && total > 0;
-    const int64_t from = cut_at(total, ctas, per, cta), to_end = cut_at(total, ctas, per, cta + 1);
-    // the piece that `from` falls into
-    Load l = {};
-    int b = a.batch, hk = 0, blk = 0;
-    int64_t pos = 0;  // what lies before it
-    for (int b0 = 0; b0 < a.batch && work; b0 += 32) {
-      const Load x = b0 + lane < a.batch ? request(b0 + lane) : Load{};
-      const int64_t w = weight_to(x, span, even, x.blocks) * kv_heads;
-      int64_t inc = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += y;
-      }
-      const uint32_t who = __ballot_sync(0xffffffffu, from - pos < inc);
-      if (who != 0) {
-        const int src = __ffs(who) - 1;
-        b = b0 + src;
-        l.first = __shfl_sync(0xffffffffu, x.first, src);
-        l.q = __shfl_sync(0xffffffffu, x.q, src);
-        l.len = __shfl_sync(0xffffffffu, x.len, src);
-        l.bad = __shfl_sync(0xffffffffu, x.bad, src);
-        l.blocks = __shfl_sync(0xffffffffu, x.blocks, src);
-        l.ctx = l.len - l.q;
-        pos += __shfl_sync(0xffffffffu, inc - w, src);
-        const int64_t head = weight_to(l, span, even, l.blocks);
-        hk = static_cast<int>(static_cast<float>(from - pos) / static_cast<float>(head));
-        hk = max(min(hk, kv_heads - 1), 0);
-        while (hk > 0 && head * hk > from - pos) --hk;
-        while (hk + 1 < kv_heads && head * (hk + 1) <= from - pos) ++hk;
-        pos += head * hk;
-        const float r = static_cast<float>(from - pos), c = kFixed + max(l.ctx, 0) + 0.5f * span;
-        blk = even ? static_cast<int>(from - pos) : static_cast<int>((sqrtf(c * c + 2.f * span * r) - c) / span);
-        blk = max(min(blk, l.blocks - 1), 0);
-        while (blk > 0 && weight_to(l, span, even, blk) > from - pos) --blk;
-        while (blk + 1 < l.blocks && weight_to(l, span, even, blk + 1) <= from - pos) ++blk;
-        pos += weight_to(l, span, even, blk);
-        break;
-      }
-      pos += __shfl_sync(0xffffffffu, inc, 31);
+    cap = max(kMinSplit, static_cast<int>(fminf(total * kv_heads * 1.25f / grid, 1e9f)) + 1);
+    int top = 0;  // the most turns of a piece
+    for (int b = lane; b < a.batch; b += 32) {
+      const Load l = request(b);
+      const int sp = splits_of(l);
+      top = max(top, (blocks.turns(l, l.tiles) + sp - 1) / sp);
     }
+    top = __reduce_max_sync(0xffffffffu, top);
+    // longest first, unless every piece has a CTA of its own (or the list is long: even anyway)
+    const bool sorted = a.batch <= kSortBatch && pieces_above(-1) > grid;
     int slot = 0, k = 0, q_uses[2] = {0, 0};  // the ring's next slot, and how often it has gone round
     uint32_t round = 0;
     for (; !dead; ++k) {
       const int st = k & 1;
+      int want = blockIdx.x;
+      if (k > 0) {
+        if (lane == 0) want = grid + static_cast<int>(atomicAdd(g.work, 1u));
+        want = __shfl_sync(0xffffffffu, want, 0);
+      }
       Piece p;
       p.b = -1;
-      auto advance = [&](int64_t w) {  // on to the next piece
-        pos += w;
-        if (++blk < l.blocks) return;
-        blk = 0;
-        if (++hk < kv_heads) return;
-        hk = 0;
-        do {
-          if (++b < a.batch) l = load_of<kPaged>(g, b);
-        } while (b < a.batch && l.blocks == 0);
-      };
-      while (b < a.batch && pos < to_end) {
-        const int64_t w = weight_to(l, span, even, blk + 1) - weight_to(l, span, even, blk);
-        const int n = tiles_of(l, (blk + 1) * span), n1 = max(n, 1);  // (a piece without keys has its zeros to write)
-        const int k0 = cut_tile(from - pos, w, n1), k1 = cut_tile(to_end - pos, w, n1);
-        if (k0 < k1) {
-          p.b = b;
-          p.hk = hk;
-          p.first = l.first;
-          p.len = l.len;
-          p.ctx = l.ctx;
-          p.bad = l.bad;
-          p.tok0 = blk * span;
-          p.toks = min(l.q - p.tok0, span);
-          p.k0 = k0;
-          p.total = min(k1, n) - k0;
-          p.halves = p.toks <= g.tile_tokens;
-          p.n[0] = p.halves ? (p.total + 1) / 2 : max(min(tiles_of(l, p.tok0 + g.tile_tokens), k1) - k0, 0);
-          p.n[1] = p.halves ? p.total / 2 : p.total;
-          int c0 = cta, c1 = cta;  // the CTAs of its first and last part
-          if (k0 > 0)
-            while (cut_tile(cut_at(total, ctas, per, c0) - pos, w, n1) > 0) --c0;
-          if (k1 < n1)
-            while (cut_tile(cut_at(total, ctas, per, c1 + 1) - pos, w, n1) < n1) ++c1;
-          p.cta0 = c0;
-          p.splits = c1 - c0 + 1;
-          p.split = cta - c0;
-          if (l.bad && lane == 0) report(a.status, MKB_SERVE_BAD_LENGTH);
+      // the level (turns of a piece) that `want` falls into, and its place there
+      int lo = 0, r = want;
+      if (sorted) {
+        int hi = top;
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (pieces_above(mid) <= want) hi = mid;
+          else lo = mid + 1;
         }
-        if (p.b >= 0) break;
-        advance(w);
+        r = want - pieces_above(lo);
+      }
+      int slot_base = 0;
+      for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        const int b = b0 + lane;
+        Load l = {};
+        int above = 0, here = 0, slots = 0, sp = 1;
+        if (b < a.batch) {
+          l = request(b);
+          sp = splits_of(l);
+          if (sorted) above = blocks.above(l, lo * sp);
+          here = (sorted ? blocks.above(l, (lo - 1) * sp) - above : blocks.of(l)) * sp * kv_heads;
+          slots = sp > 1 ? blocks.of(l) * sp * kv_heads : 0;
+        }
+        int inc = here, sinc = slots;  // inclusive prefix sums
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, inc, o), y = __shfl_up_sync(0xffffffffu, sinc, o);
+          if (lane >= o) {
+            inc += x;
+            sinc += y;
+          }
+        }
+        const bool is_it = r >= inc - here && r < inc;
+        const uint32_t who = __ballot_sync(0xffffffffu, is_it);
+        if (who != 0) {
+          if (is_it) {
+            unsigned at = static_cast<unsigned>(r) - (inc - here);
+            p.b = b;
+            p.splits = sp;
+            p.split = 0;
+            if (sp > 1) {
+              p.split = at % static_cast<unsigned>(sp);
+              at /= static_cast<unsigned>(sp);
+            }
+            const unsigned i0 = at / static_cast<unsigned>(kv_heads);
+            p.hk = at - i0 * kv_heads;
+            const int i = blocks.of(l) - 1 - above - static_cast<int>(i0);  // longest first
+            p.first = l.first;
+            p.len = l.len;
+            p.ctx = l.ctx;
+            p.tok0 = i * blocks.span;
+            p.toks = min(l.q - p.tok0, blocks.span);
+            const int n = tiles_of(l, p.tok0 + p.toks), per = sp > 1 ? (n + sp - 1) / sp : n;
+            p.k0 = min(p.split * per, n);
+            const int k1 = min(p.k0 + per, n);
+            p.slot = slot_base + sinc - slots + (i * kv_heads + p.hk) * sp;
+            p.bad = l.bad;
+            p.total = k1 - p.k0;
+            p.halves = p.toks <= g.tile_tokens;
+            p.n[0] = p.halves ? (p.total + 1) / 2 : max(min(tiles_of(l, p.tok0 + g.tile_tokens), k1) - p.k0, 0);
+            p.n[1] = p.halves ? p.total / 2 : p.total;
+            if (l.bad) report(a.status, MKB_SERVE_BAD_LENGTH);
+          }
+          const int src = __ffs(who) - 1;
+          uint32_t* w = reinterpret_cast<uint32_t*>(&p);
+#pragma unroll
+          for (int i = 0; i < static_cast<int>(sizeof(Piece) / 4); ++i) w[i] = __shfl_sync(0xffffffffu, w[i], src);
+          break;
+        }
+        r -= __shfl_sync(0xffffffffu, inc, 31);
+        slot_base += __shfl_sync(0xffffffffu, sinc, 31);
       }
       if (k >= 2) wait_for(&sm.info_empty[st], ((k >> 1) - 1) & 1, &sm.err, dead);
       if (lane == 0) {
@@ -500,7 +509,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       __syncwarp();
       if (p.b < 0) break;
-      advance(weight_to(l, span, even, blk + 1) - weight_to(l, span, even, blk));
       // K(0), then K(j + 1) and V(j): the order in which the products take them
       const int n = p.total;
       auto load = [&](const CUtensorMap* map, int head, int j) {
@@ -559,6 +567,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         load(&tv, vh, j);
       }
     }
+    // the last CTA to have asked for its last piece puts the list back to its start
+    if (lane == 0 && atomicInc(g.work + 1, grid - 1) == static_cast<uint32_t>(grid - 1)) atomicExch(g.work, 0u);
     // after a stop, wait (bounded) for the copies still in flight before leaving
     if (sm.err) {
       int tries = 0;
@@ -860,7 +870,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       };
       const bool split = p.splits > 1;
       const int at = 128 * t + row_in;
-      auto slot_of = [&](int s) { return static_cast<size_t>(2 * (p.cta0 + s) + (s == 0)); };
+      auto slot_of = [&](int s) { return static_cast<size_t>(p.slot + s); };
       const size_t slot = slot_of(p.split);
       float4* part = g.part + slot * (D / 4) * kRows;
       uint64_t odd2 = 0;  // NaN once a value of O is not finite
@@ -958,7 +968,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tile_sync();
         if (threadIdx.x % 128 == 0)
           *reinterpret_cast<volatile int*>(&sm.last[t]) =
-              atomicInc(g.counters + 2 * p.cta0 + t, p.splits - 1) ==
+              atomicInc(g.counters + 2 * p.slot + t, p.splits - 1) ==
               static_cast<uint32_t>(p.splits - 1);
         tile_sync();
         if (*reinterpret_cast<volatile int*>(&sm.last[t]) != 0) {
@@ -1062,14 +1072,16 @@ int sm_count() {
 
 // Upper bound of the pieces of a call before any split, all KV heads.
 static int64_t tc_blocks(const mkb_attn_args& a) {
-  const int64_t span = 2 * (128 / (a.heads / a.kv_heads));
-  return (a.tokens / span + a.batch) * a.kv_heads;
+  return (a.tokens / (128 / (a.heads / a.kv_heads)) + a.batch) * static_cast<int64_t>(a.kv_heads);
 }
-// Counters (the place of both attention kernels', zero between calls), then two partial
-// results a CTA.
-size_t counter_bytes() { return (static_cast<size_t>(sm_count()) * 8 + 255) / 256 * 256; }
+// Partial results a call can leave. Rows are split only where their n turns are more than a
+// cap C >= 5/4 U / grid of all U turns, into at most 2 n / C ranges; a request's blocks grow
+// linearly, so that U counts at least half of n for each: at most 4 U / C < 4 grid.
+static size_t tc_slots() { return 4 * static_cast<size_t>(sm_count()); }
+// Counters (the place of both attention kernels', zero between calls), then partial results.
+size_t counter_bytes() { return (16 + tc_slots() * 8 + 255) / 256 * 256; }
 size_t tc_workspace(const mkb_attn_args& a) {
-  return counter_bytes() + 2 * static_cast<size_t>(sm_count()) * kRows * (static_cast<size_t>(a.head_dim) * 4 + 8);
+  return counter_bytes() + tc_slots() * kRows * (static_cast<size_t>(a.head_dim) * 4 + 8);
 }
 
 template <typename T, int D, bool kPaged>
@@ -1085,9 +1097,11 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   g.v_head = a.v_stride[1] != 0;
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   if (ws == nullptr) return cudaErrorInvalidValue;
-  g.counters = reinterpret_cast<uint32_t*>(ws);
+  g.tile_mul = g.tile_tokens > 1 ? static_cast<unsigned>((1ull << 32) / g.tile_tokens + 1) : 0;
+  g.work = reinterpret_cast<uint32_t*>(ws);
+  g.counters = g.work + 4;
   g.stat = reinterpret_cast<float2*>(ws + counter_bytes());
-  g.part = reinterpret_cast<float4*>(g.stat + 2 * static_cast<size_t>(sm_count()) * kRows);
+  g.part = reinterpret_cast<float4*>(g.stat + tc_slots() * kRows);
   CUtensorMap mk, mv, mq, mo;
   cudaError_t e;
   {
