@@ -399,7 +399,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       return __reduce_add_sync(0xffffffffu, n) * kv_heads;
     };
     // pairs of tiles, unless those are fewer than the CTAs: then single ones
-    if (pieces_above(-1) <= grid) blocks = {1, g.tile_tokens, g.tile_mul};
+    const int pairs = pieces_above(-1);
+    if (pairs <= grid) {  // (unless those would not all fit, and are too short to gain by it)
+      blocks = {1, g.tile_tokens, g.tile_mul};
+      int longest = 0;
+      for (int b = lane; b < a.batch; b += 32) longest = max(longest, request(b).tiles);
+      longest = __reduce_max_sync(0xffffffffu, longest);
+      if (longest < kMinSplit && pieces_above(-1) > grid) blocks = {2, 2 * g.tile_tokens, g.tile_mul};
+    }
     // a fair share of the turns; rows with more are split
     float total = 0.f;
     for (int b = lane; b < a.batch; b += 32) {
@@ -511,6 +518,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (p.b < 0) break;
       // K(0), then K(j + 1) and V(j): the order in which the products take them
       const int n = p.total;
+      int pages = 0, pages_at = 0, pages_end = 0;  // the lanes' pages: boxes of keys up to pages_end
       auto load = [&](const CUtensorMap* map, int head, int j) {
         const int s = slot;
         if (round > 0) wait_for(&sm.kv_empty[s], (round - 1) & 1, &sm.err, dead);
@@ -523,22 +531,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) mbar_arrive_expect_tx(&sm.kv_full[s], kTileBytes);
         __syncwarp();
         if (kPaged) {
+          // (a lane reads one entry of the table for several tiles to come: a lookup before every
+          // copy, of K and of V, is what such loads took longest over)
           const int box = g.box;
-          if (lane * box < kKeys) {
-            const int at = key + lane * box;
-            int page = a.pages;  // past the last key: outside the pool, which reads as zeros
+          const int box_log = 31 - __clz(box);
+          if (key + kKeys > pages_end) {
+            pages_at = max(key - kKeys, 0);  // (V follows a tile behind K)
+            pages_end = pages_at + 32 * box;
+            const int at = pages_at + lane * box;
+            pages = a.pages;  // past the last key: outside the pool, which reads as zeros
             if (at < p.len) {
-              page = __ldg(a.block_table + p.b * a.table_stride + at / a.page_size);
-              if (page < 0 || page >= a.pages) {
-                page = a.pages;
-                *reinterpret_cast<volatile int*>(&sm.piece[st].bad) = 1;
-                report(a.status, MKB_SERVE_BAD_PAGE);
-              }
+              pages = __ldg(a.block_table + p.b * a.table_stride + (at >> 31 - __clz(a.page_size)));
+              if (pages < 0 || pages >= a.pages) pages = -1;
+            }
+          }
+          int page = __shfl_sync(0xffffffffu, pages, ((key - pages_at >> box_log) + lane) & 31);
+          if (lane * box < kKeys) {
+            if (page < 0) {
+              page = a.pages;
+              *reinterpret_cast<volatile int*>(&sm.piece[st].bad) = 1;
+              report(a.status, MKB_SERVE_BAD_PAGE);
             }
 #pragma unroll
             for (int d = 0; d < D / 64; ++d)
-              tc::tma_load_4d(sm.kv[s] + d * kHalf + lane * box * 128, map, 64 * d, at % a.page_size, head, page,
-                     &sm.kv_full[s]);
+              tc::tma_load_4d(sm.kv[s] + d * kHalf + lane * box * 128, map, 64 * d, (key + lane * box) & (a.page_size - 1),
+                              head, page, &sm.kv_full[s]);
           }
         } else if (lane == 0) {
 #pragma unroll
