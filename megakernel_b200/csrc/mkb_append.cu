@@ -12,7 +12,10 @@
 // low half and the eight of the high half that RoPE pairs with them, so the rotation
 // needs no exchange, every access is 16 bytes, and the norm's sum is log2(D / 16)
 // shuffles. One block per token: its heads share the request, the page and the
-// cos / sin values.
+// cos / sin values. A block waits for one lookup after another (request, length, page,
+// tables), so blocks in flight carry the bandwidth: six of an SM at 80 registers, where
+// the compiler's own 111 left four. 16,000 tokens from FP32: 71 us, 5.7 TB/s of the 6.6
+// that a copy reaches (four blocks: 84 us; eight, with spills: 75).
 
 #include "mkb_serving.cuh"
 
@@ -21,8 +24,37 @@ namespace sv {
 
 constexpr int kAppendThreads = 128;
 
+// Eight values as they lie in memory.
+template <typename S>
+struct Raw8 {
+  uint4 v[sizeof(S) / 2];
+  __device__ __forceinline__ void load(const S* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(S)) / 2; ++i) v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void get(float x[8]) const {
+    if constexpr (sizeof(S) == 4) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        x[4 * i] = __uint_as_float(v[i].x);
+        x[4 * i + 1] = __uint_as_float(v[i].y);
+        x[4 * i + 2] = __uint_as_float(v[i].z);
+        x[4 * i + 3] = __uint_as_float(v[i].w);
+      }
+    } else {
+      const uint32_t w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = Pair<S>::get(w[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
+  }
+};
+
 template <typename S, typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const mkb_append_args a) {
+__global__ void __launch_bounds__(kAppendThreads, 6) append_kernel(const mkb_append_args a) {
   constexpr int kLanes = D / 16;                    // lanes of a head
   constexpr int kRows = kAppendThreads / kLanes;    // heads of a block at a time
   const int t = blockIdx.x;
@@ -33,13 +65,21 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const mkb_append
 
   depend_launch();
   depend_wait();
+  Raw8<S> lo, hi;  // the next head's values, asked for before anything else is known
+  auto fetch = [&](int row) {
+    if (row >= rows) return;
+    const S* src = static_cast<const S*>(a.qkv) + t * a.qkv_stride[0] + row * a.qkv_stride[1];
+    lo.load(src + d0);
+    hi.load(src + d1);
+  };
+  fetch(row0);
   const Request rq = request_at(a.cu_q, a.batch, a.q_len, a.tokens, t);
   const int b = rq.b, at = t - rq.first;
   const int pos = at >= 0 && at < rq.n ? a.kv_lens[b] - rq.n + at : -1;
   int64_t page = -1;
   uint32_t bad = 0;
   if (pos >= 0) {
-    const int entry = pos / a.page_size;
+    const int entry = pos >> (31 - __clz(a.page_size));
     if (pos >= a.rope_rows) {
       bad = MKB_SERVE_BAD_POSITION;
     } else if (entry >= a.table_width) {
@@ -51,7 +91,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const mkb_append
   }
   if (bad != 0 && threadIdx.x == 0) report(a.status, bad);
   const bool store = pos >= 0 && bad == 0;
-  const int64_t slot = pos % a.page_size;
+  const int64_t slot = pos & (a.page_size - 1);
 
   float cs[16], sn[16];
   if (store) {
@@ -80,11 +120,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const mkb_append
     const int row = r0 + row0;
     const bool live = row < rows;
     float x[16];
-    if (live) {
-      const S* src = static_cast<const S*>(a.qkv) + t * a.qkv_stride[0] + row * a.qkv_stride[1];
-      load8(src + d0, x);
-      load8(src + d1, x + 8);
-    }
+    lo.get(x);
+    hi.get(x + 8);
+    fetch(row + kRows);
     const bool is_v = row >= a.heads + a.kv_heads;
     const void* weight = row < a.heads ? a.q_norm : a.k_norm;
     if (a.q_norm != nullptr || a.k_norm != nullptr) {  // uniform: every lane takes the shuffles

@@ -998,31 +998,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             ll += x.y * ex2_approx(x.x - ref);
           }
           const float f0 = 1.f / ll;
+          // a row's whole D at once: the loads of a range are all in flight together
+          float o[D];
+#pragma unroll
+          for (int i = 0; i < D; ++i) o[i] = 0.f;
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            float o[32];
+          for (int s = 0; s < p.splits && live; ++s) {
+            const float w = __ldcg(g.stat + slot_of(s) * kRows + at).x;
+            const float4* x4 = g.part + slot_of(s) * (D / 4) * kRows + at;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0.f;
-#pragma unroll 2
-            for (int s = 0; s < p.splits && live; ++s) {
-              const float w = __ldcg(g.stat + slot_of(s) * kRows + at).x;
-              const float4* x4 = g.part + (slot_of(s) * (D / 4) + 8 * c) * kRows + at;
-              float4 x[8];
+            for (int h = 0; h < D / 64; ++h) {
+              float4 x[16];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) x[i] = __ldcg(x4 + i * kRows);
+              for (int i = 0; i < 16; ++i) x[i] = __ldcg(x4 + (16 * h + i) * kRows);
               if (w == -INFINITY) continue;  // that range holds no key this row sees
               const float f = ex2_approx(w - ref);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                o[4 * i] += f * x[i].x;
-                o[4 * i + 1] += f * x[i].y;
-                o[4 * i + 2] += f * x[i].z;
-                o[4 * i + 3] += f * x[i].w;
+              for (int i = 0; i < 16; ++i) {
+                o[64 * h + 4 * i] += f * x[i].x;
+                o[64 * h + 4 * i + 1] += f * x[i].y;
+                o[64 * h + 4 * i + 2] += f * x[i].z;
+                o[64 * h + 4 * i + 3] += f * x[i].w;
               }
             }
+          }
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
             uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = lim < 0 ? 0 : Pair<T>::put(o[2 * i] * f0, o[2 * i + 1] * f0);
+            for (int i = 0; i < 16; ++i) w[i] = lim < 0 ? 0 : Pair<T>::put(o[32 * c + 2 * i] * f0, o[32 * c + 2 * i + 1] * f0);
             emit(c, w);
           }
         }
