@@ -382,13 +382,51 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     const int kv_heads = a.kv_heads, grid = gridDim.x;
     auto request = [&](int b) { return b < 32 ? mine : load_of<kPaged>(g, b); };  // of lane b % 32
-    // pieces of more than x turns each, all requests
-    Blocks blocks = {2, 2 * g.tile_tokens, g.tile_mul};
-    int cap = 0x3fffffff;
-    auto splits_of = [&](const Load& l) {  // (rows that stand before position 0 have no keys to split)
+    // One pass over the requests: their blocks as pairs of tiles and as single ones, what
+    // those come to in turns (linear in the block), and the longest.
+    const Blocks pairs = {2, 2 * g.tile_tokens, g.tile_mul}, singles = {1, g.tile_tokens, g.tile_mul};
+    int n2 = 0, n1 = 0, longest = 0, top = 0;
+    float total2 = 0.f, total1 = 0.f;
+    for (int b = lane; b < a.batch; b += 32) {
+      const Load l = request(b);
+      const int b2 = pairs.of(l), b1 = singles.of(l), t2 = pairs.turns(l, l.tiles), t1 = singles.turns(l, l.tiles);
+      n2 += b2;
+      n1 += b1;
+      longest = max(longest, l.tiles);
+      top = max(top, t2);
+      total2 += 0.5f * (pairs.turns(l, tiles_of(l, pairs.span)) + t2) * b2;
+      total1 += 0.5f * (singles.turns(l, tiles_of(l, singles.span)) + t1) * b1;
+    }
+    n2 = __reduce_add_sync(0xffffffffu, n2) * kv_heads;
+    n1 = __reduce_add_sync(0xffffffffu, n1) * kv_heads;
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    // pairs of tiles; single ones where the pairs are fewer than the CTAs, unless the keys are
+    // few and not all of those would have a CTA either
+    const bool single = n2 <= grid && (longest >= kMinSplit || n1 <= grid);
+    const Blocks blocks = single ? singles : pairs;
+    float total = single ? total1 : total2;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    top = single ? (longest + 1) / 2 : __reduce_max_sync(0xffffffffu, top);
+    int count = single ? n1 : n2;  // of pieces
+    // a fair share of the turns; rows with more are split (but for those that stand before position 0)
+    const int cap = max(kMinSplit, static_cast<int>(fminf(total * kv_heads * 1.25f / grid, 1e9f)) + 1);
+    auto splits_of = [&](const Load& l) {
       const int n = blocks.turns(l, l.tiles);
       return n > cap && l.ctx >= 0 ? (n + cap - 1) / cap : 1;
     };
+    if (top > cap) {
+      top = count = 0;
+      for (int b = lane; b < a.batch; b += 32) {
+        const Load l = request(b);
+        const int sp = splits_of(l);
+        count += blocks.of(l) * sp;
+        top = max(top, (blocks.turns(l, l.tiles) + sp - 1) / sp);
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      count = __reduce_add_sync(0xffffffffu, count) * kv_heads;
+    }
+    // pieces of more than x turns each, all requests
     auto pieces_above = [&](int x) {
       int n = 0;
       for (int b = lane; b < a.batch; b += 32) {
@@ -398,34 +436,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       return __reduce_add_sync(0xffffffffu, n) * kv_heads;
     };
-    // pairs of tiles, unless those are fewer than the CTAs: then single ones
-    const int pairs = pieces_above(-1);
-    if (pairs <= grid) {  // (unless those would not all fit, and are too short to gain by it)
-      blocks = {1, g.tile_tokens, g.tile_mul};
-      int longest = 0;
-      for (int b = lane; b < a.batch; b += 32) longest = max(longest, request(b).tiles);
-      longest = __reduce_max_sync(0xffffffffu, longest);
-      if (longest < kMinSplit && pieces_above(-1) > grid) blocks = {2, 2 * g.tile_tokens, g.tile_mul};
-    }
-    // a fair share of the turns; rows with more are split
-    float total = 0.f;
-    for (int b = lane; b < a.batch; b += 32) {
-      const Load l = request(b);  // (linear in the block)
-      const int n = blocks.turns(l, l.tiles);
-      total += 0.5f * (blocks.turns(l, tiles_of(l, blocks.span)) + n) * blocks.of(l);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    cap = max(kMinSplit, static_cast<int>(fminf(total * kv_heads * 1.25f / grid, 1e9f)) + 1);
-    int top = 0;  // the most turns of a piece
-    for (int b = lane; b < a.batch; b += 32) {
-      const Load l = request(b);
-      const int sp = splits_of(l);
-      top = max(top, (blocks.turns(l, l.tiles) + sp - 1) / sp);
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
     // longest first, unless every piece has a CTA of its own (or the list is long: even anyway)
-    const bool sorted = a.batch <= kSortBatch && pieces_above(-1) > grid;
+    const bool sorted = a.batch <= kSortBatch && count > grid;
     int slot = 0, k = 0, q_uses[2] = {0, 0};  // the ring's next slot, and how often it has gone round
     uint32_t round = 0;
     for (; !dead; ++k) {
