@@ -310,8 +310,9 @@ void mkb_engine_destroy(mkb_engine* e);
  *
  * Lengths live on the device, so they are checked there: a page outside the pool,
  * more keys than the table has room for, or a position past the RoPE tables makes
- * the rows that need it NaN, touches no memory out of range, and is recorded in
- * *status (0 = ok; first code kept). */
+ * the rows that need it NaN (and may make other new rows of the same request NaN),
+ * touches no memory out of range, and is recorded in *status (0 = ok; first code
+ * kept). */
 enum { MKB_BF16 = 0, MKB_FP16 = 1, MKB_FP32 = 2 };
 enum {
   MKB_SERVE_BAD_PAGE = 1,      /* block_table names a page outside the pool */

@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
       if (lane == 0) {
         uint8_t* const dst = mine + fill * kBytes;
         uint64_t* const bar = &full[warp][fill];
-        const int at = page < 0 ? a.pages : page;  // (outside the pool: zeros)
+        const int at = page < 0 ? max(a.pages, 1) : page;  // (outside the pool and its map: zeros)
         mbar_arrive_expect_tx(bar, kBytes);
 #pragma unroll
         for (int d = 0; d < D / 64; ++d) {

@@ -530,6 +530,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (p.b < 0) break;
       // K(0), then K(j + 1) and V(j): the order in which the products take them
       const int n = p.total;
+      const int outside = max(a.pages, 1);  // (an empty pool's map has one page, that is never read)
       int pages = 0, pages_at = 0, pages_end = 0;  // the lanes' pages: boxes of keys up to pages_end
       auto load = [&](const CUtensorMap* map, int head, int j) {
         const int s = slot;
@@ -551,7 +552,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             pages_at = max(key - kKeys, 0);  // (V follows a tile behind K)
             pages_end = pages_at + 32 * box;
             const int at = pages_at + lane * box;
-            pages = a.pages;  // past the last key: outside the pool, which reads as zeros
+            pages = outside;  // past the last key: outside the pool, which reads as zeros
             if (at < p.len) {
               pages = __ldg(a.block_table + p.b * a.table_stride + (at >> 31 - __clz(a.page_size)));
               if (pages < 0 || pages >= a.pages) pages = -1;
@@ -560,7 +561,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           int page = __shfl_sync(0xffffffffu, pages, ((key - pages_at >> box_log) + lane) & 31);
           if (lane * box < kKeys) {
             if (page < 0) {
-              page = a.pages;
+              page = outside;
               *reinterpret_cast<volatile int*>(&sm.piece[st].bad) = 1;
               report(a.status, MKB_SERVE_BAD_PAGE);
             }

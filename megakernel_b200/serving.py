@@ -15,14 +15,14 @@ Without ``cu_q`` every request brings one token (``[batch, heads, dim]``) or ``n
 (``[batch, n, heads, dim]``). The cache is two pools ``[pages, kv_heads, page_size,
 dim]`` (any strides of whole 16 bytes, so another order of the dimensions is a
 permuted view), ``block_table[b]`` lists request ``b``'s pages and ``kv_lens[b]``
-counts its keys, the new tokens included. BF16 or FP16, heads of 64 or 128, any
-number of query heads per KV head, pages of a power of two of 16 keys or more.
+counts its keys, the new tokens included. BF16 or FP16, heads of 64 or 128, up
+to 128 query heads per KV head, pages of a power of two of 16 keys or more.
 
 A token sees the keys up to its own position; one that sees none gets zeros. What a
 page holds past a request's last key reaches no output. Calls run on the current
 stream, do not synchronise, and can be captured into a CUDA graph. Host-side misuse
 raises ``ValueError``; lengths and page numbers are read on the device, where a wrong
-one makes its rows NaN and is kept for :func:`serving_status`.
+one makes its request's new rows NaN, some or all, and is kept for :func:`serving_status`.
 
 There is no CPU or PyTorch fallback.
 """

@@ -317,6 +317,19 @@ def test_wrong_pages_and_lengths_are_reported():
         assert mk.serving_status()[0] == 2
 
 
+@pytest.mark.parametrize("new", [[1, 1, 1], [1, 40, 1]])
+def test_pool_without_pages(new):
+    """No page is inside it: requests with keys are reported, those without get zeros."""
+    pool = torch.empty((0, 2, 16, 128), dtype=BF, device=DEV)
+    table = torch.zeros((3, 4), dtype=torch.int32, device=DEV)
+    lens = torch.tensor([0, 50, 0], dtype=torch.int32, device=DEV)
+    q = rand(seeded(11), sum(new), 4, 128)
+    got = mk.paged_attention(q, pool, pool, table, lens, cu_of(new) if max(new) > 1 else None)
+    assert bool((got[0] == 0).all()) and bool((got[-1] == 0).all())
+    assert got[1:-1].isnan().all()
+    assert mk.serving_status()[0] == 1
+
+
 def test_paged_is_reproducible_across_streams_and_in_graphs():
     kv, new = [3000, 50, 7000, 1], [1, 30, 1, 1]
     c = Cache(kv, 8, 128, 16, seed=6)
