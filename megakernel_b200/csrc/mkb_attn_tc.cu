@@ -10,8 +10,9 @@
 // one only, A takes them with the even and B with the odd tiles of keys, and A adds the
 // two up in the end:
 //
-//   warp 9      which piece of work comes next; its Q, K and V tiles by TMA (128-byte
-//               swizzle; K and V through a ring, pages are boxes of page_size rows)
+//   warp 11     which piece of work comes next
+//   warp 9      its Q, K and V tiles by TMA (128-byte swizzle; K and V through a ring, pages
+//               are boxes of page_size rows)
 //   warps 8, 10 tcgen05.mma of tile A, B: S = Q K^T (Q and K in shared memory), O += P V with P from
 //               tensor memory and V as it lies, keys by dims (an MN-major operand: no
 //               transposed copy of V is made)
@@ -30,7 +31,7 @@
 //
 // Work: a piece is (request, KV head, one or two tiles of rows, a range of key tiles).
 // Every CTA works the list out for itself from the lengths, the longest pieces first, and
-// takes the next one whenever its loads have run through the last (a counter in memory).
+// takes the next one when the loads of the last are nearly through (a counter in memory).
 // Rows whose keys are more than a fair share are split over several pieces; each leaves its
 // O, maximum and sum in memory, and the last one to be done adds them up in order of their
 // keys, so results do not depend on timing. Nothing is asked of the host.
@@ -57,6 +58,7 @@ constexpr int kRows = 256, kKeys = 128;   // rows of a piece (two tiles), keys o
 constexpr int kFirstKeys = 96;            // of a tile's weights, what the second product starts on
 constexpr int kHalf = 128 * 128;          // 16 KB: 128 rows x 64 values, 128-byte swizzle
 constexpr int kMinSplit = 6;              // key tiles (turns, of one tile's rows) below which rows are not split
+constexpr int kAskTiles = 3;              // key tiles to load when a CTA asks for its next piece
 constexpr int kSortBatch = 128;           // requests up to which pieces are taken longest first
 constexpr int kTryNs = 20000, kTries = 50000;  // bound of every wait: about a second
 
@@ -89,7 +91,7 @@ struct TcSmem {
   uint8_t stage[8][32 * 128];                           // a warp's 32 rows x 64 values on their way out
   uint64_t kv_full[Shape::kSlots], kv_empty[Shape::kSlots];
   uint64_t q_full[2], q_empty[2], s_full[2], p_part[2], p_full[2], o_full[2];
-  uint64_t info_full[2], info_empty[2];
+  uint64_t info_full[2], info_empty[2], ask;
   uint64_t tile_bar[2];   // the four softmax warps of a tile
   uint64_t pair_full, pair_empty;
   float2 pair[128];       // maximum and sum of B's rows, where they are A's too
@@ -278,6 +280,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // One request as the list sees it.
 struct Load {
   int first, q, len, ctx, tiles, bad;
+  int blocks, turns, splits;  // its blocks of rows, the turns of the last of them, the ranges of each one's keys
 };
 template <bool kPaged>
 __device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
@@ -307,17 +310,17 @@ struct Blocks {
     return i * (span >> (tiles - 1)) > y ? i - 1 : i;
   }
   __device__ __forceinline__ int of(const Load& l) const { return l.q > 0 ? over(l.q - 1) + 1 : 0; }
-  // turns that a block with n key tiles takes: rows for one tile take two at a time
-  __device__ __forceinline__ int turns(const Load& l, int n) const {
-    return tiles == 1 || 2 * l.q <= span ? (n + 1) / 2 : n;
-  }
+  // rows for one tile take two key tiles at a time
+  __device__ __forceinline__ bool halves(const Load& l) const { return tiles == 1 || 2 * l.q <= span; }
+  // turns that a block with n key tiles takes
+  __device__ __forceinline__ int turns(const Load& l, int n) const { return halves(l) ? (n + 1) / 2 : n; }
   // how many of the request's blocks take more than x turns (they come last)
   __device__ __forceinline__ int above(const Load& l, int x) const {
-    if (x < 0) return of(l);
-    if (turns(l, l.tiles) <= x) return 0;
-    const int n = tiles == 1 || 2 * l.q <= span ? 2 * x : x;  // more than n key tiles
-    const int y = n * kKeys - l.ctx;                          // the first token that sees more (n < tiles: no overflow)
-    return y <= 0 ? of(l) : of(l) - over(y);
+    if (x < 0) return l.blocks;
+    if (l.turns <= x) return 0;
+    const int n = halves(l) ? 2 * x : x;  // more than n key tiles
+    const int y = n * kKeys - l.ctx;      // the first token that sees more (n < tiles: no overflow)
+    return y <= 0 ? l.blocks : l.blocks - over(y);
   }
 };
 
@@ -334,7 +337,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const mkb_attn_args& a = g.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   depend_launch();
-  // (a lane of the loading warp keeps its first request; the others are read again in every pass)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&sm.kv_full[s], 1);
@@ -349,8 +351,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&sm.o_full[t], 1);
       mbar_init(&sm.info_full[t], 1);
       mbar_init(&sm.tile_bar[t], 4);
-      mbar_init(&sm.info_empty[t], 10);  // eight softmax warps, two MMA warps
+      mbar_init(&sm.info_empty[t], 11);  // eight softmax warps, two MMA warps, the loading warp
     }
+    mbar_init(&sm.ask, 1);
     mbar_init(&sm.pair_full, 4);
     mbar_init(&sm.pair_empty, 4);
     sm.err = sm.turn = 0;
@@ -361,8 +364,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc::tmem_relinquish();
   }
   depend_wait();  // what came before in the stream is done: its results may be read
-  Load mine = {};
-  if (warp == 9 && lane < a.batch) mine = load_of<kPaged>(g, lane);
+  Load mine = {};  // (a lane keeps its first request; the others are read again in every pass)
+  if (warp == 11 && lane < a.batch) mine = load_of<kPaged>(g, lane);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -373,22 +376,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  if (warp == 9) {
-    // ---- the next piece, and its loads ------------------------------------------------
-    if (lane == 0) {
-      tc::prefetch_tensormap(&tk);
-      tc::prefetch_tensormap(&tv);
-      tc::prefetch_tensormap(&tq);
-    }
+  if (warp == 11) {
+    // ---- which piece comes next ----------------------------------------------------------
+    // (a warp of its own: working out a place in the list takes 3,000 cycles and more, which
+    // the loads of the next piece, 4,000 cycles late, do not get back)
     const int kv_heads = a.kv_heads, grid = gridDim.x;
-    auto request = [&](int b) { return b < 32 ? mine : load_of<kPaged>(g, b); };  // of lane b % 32
     // One pass over the requests: their blocks as pairs of tiles and as single ones, what
     // those come to in turns (linear in the block), and the longest.
     const Blocks pairs = {2, 2 * g.tile_tokens, g.tile_mul}, singles = {1, g.tile_tokens, g.tile_mul};
     int n2 = 0, n1 = 0, longest = 0, top = 0;
     float total2 = 0.f, total1 = 0.f;
     for (int b = lane; b < a.batch; b += 32) {
-      const Load l = request(b);
+      const Load l = b < 32 ? mine : load_of<kPaged>(g, b);
       const int b2 = pairs.of(l), b1 = singles.of(l), t2 = pairs.turns(l, l.tiles), t1 = singles.turns(l, l.tiles);
       n2 += b2;
       n1 += b1;
@@ -411,17 +410,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     int count = single ? n1 : n2;  // of pieces
     // a fair share of the turns; rows with more are split (but for those that stand before position 0)
     const int cap = max(kMinSplit, static_cast<int>(fminf(total * kv_heads * 1.25f / grid, 1e9f)) + 1);
-    auto splits_of = [&](const Load& l) {
-      const int n = blocks.turns(l, l.tiles);
-      return n > cap && l.ctx >= 0 ? (n + cap - 1) / cap : 1;
+    auto share = [&](Load& l) {
+      l.blocks = blocks.of(l);
+      l.turns = blocks.turns(l, l.tiles);
+      l.splits = l.turns > cap && l.ctx >= 0 ? static_cast<int>((static_cast<unsigned>(l.turns) + cap - 1) / cap) : 1;
     };
-    if (top > cap) {
+    share(mine);
+    auto request = [&](int b) {  // of lane b % 32
+      if (b < 32) return mine;
+      Load l = load_of<kPaged>(g, b);
+      share(l);
+      return l;
+    };
+    const bool any_split = top > cap;
+    if (any_split) {
       top = count = 0;
       for (int b = lane; b < a.batch; b += 32) {
         const Load l = request(b);
-        const int sp = splits_of(l);
-        count += blocks.of(l) * sp;
-        top = max(top, (blocks.turns(l, l.tiles) + sp - 1) / sp);
+        count += l.blocks * l.splits;
+        top = max(top, (l.turns + l.splits - 1) / l.splits);
       }
       top = __reduce_max_sync(0xffffffffu, top);
       count = __reduce_add_sync(0xffffffffu, count) * kv_heads;
@@ -429,105 +436,127 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // pieces of more than x turns each, all requests
     auto pieces_above = [&](int x) {
       int n = 0;
+#pragma unroll 1
       for (int b = lane; b < a.batch; b += 32) {
         const Load l = request(b);
-        const int sp = splits_of(l);
-        n += blocks.above(l, x * sp) * sp;
+        n += blocks.above(l, x * l.splits) * l.splits;
       }
       return __reduce_add_sync(0xffffffffu, n) * kv_heads;
     };
     // longest first, unless every piece has a CTA of its own (or the list is long: even anyway)
     const bool sorted = a.batch <= kSortBatch && count > grid;
-    int slot = 0, k = 0, q_uses[2] = {0, 0};  // the ring's next slot, and how often it has gone round
-    uint32_t round = 0;
-    for (; !dead; ++k) {
+    for (int k = 0; !dead; ++k) {
       const int st = k & 1;
       int want = blockIdx.x;
       if (k > 0) {
+        wait_for(&sm.ask, (k - 1) & 1, &sm.err, dead);
+        if (dead) break;
         if (lane == 0) want = grid + static_cast<int>(atomicAdd(g.work, 1u));
         want = __shfl_sync(0xffffffffu, want, 0);
       }
-      Piece p;
-      p.b = -1;
-      // the level (turns of a piece) that `want` falls into, and its place there
+      // the level (turns of a piece) that `want` falls into, and its place there; the next
+      // one wanted is never on a higher level
       int lo = 0, r = want;
-      if (sorted) {
-        int hi = top;
+      bool found = want < count;
+      if (sorted && found) {
+        int hi = top, at_hi = 0, n = 0;
         while (lo < hi) {
           const int mid = (lo + hi) / 2;
-          if (pieces_above(mid) <= want) hi = mid;
-          else lo = mid + 1;
+          if ((n = pieces_above(mid)) <= want) {
+            hi = mid;
+            at_hi = n;
+          } else {
+            lo = mid + 1;
+          }
         }
-        r = want - pieces_above(lo);
+        top = lo;
+        r = want - (at_hi > 0 ? at_hi : pieces_above(lo));
       }
+      if (k >= 2) wait_for(&sm.info_empty[st], ((k >> 1) - 1) & 1, &sm.err, dead);
+      Piece& p = sm.piece[st];
       int slot_base = 0;
-      for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      for (int b0 = 0; b0 < a.batch && found; b0 += 32) {
         const int b = b0 + lane;
         Load l = {};
         int above = 0, here = 0, slots = 0, sp = 1;
         if (b < a.batch) {
           l = request(b);
-          sp = splits_of(l);
+          sp = l.splits;
           if (sorted) above = blocks.above(l, lo * sp);
-          here = (sorted ? blocks.above(l, (lo - 1) * sp) - above : blocks.of(l)) * sp * kv_heads;
-          slots = sp > 1 ? blocks.of(l) * sp * kv_heads : 0;
+          here = (sorted ? blocks.above(l, (lo - 1) * sp) - above : l.blocks) * sp * kv_heads;
+          slots = sp > 1 ? l.blocks * sp * kv_heads : 0;
         }
         int inc = here, sinc = slots;  // inclusive prefix sums
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const int x = __shfl_up_sync(0xffffffffu, inc, o), y = __shfl_up_sync(0xffffffffu, sinc, o);
-          if (lane >= o) {
-            inc += x;
-            sinc += y;
+          const int x = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += x;
+        }
+        if (any_split) {
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, sinc, o);
+            if (lane >= o) sinc += y;
           }
         }
         const bool is_it = r >= inc - here && r < inc;
-        const uint32_t who = __ballot_sync(0xffffffffu, is_it);
-        if (who != 0) {
-          if (is_it) {
-            unsigned at = static_cast<unsigned>(r) - (inc - here);
-            p.b = b;
-            p.splits = sp;
-            p.split = 0;
-            if (sp > 1) {
-              p.split = at % static_cast<unsigned>(sp);
-              at /= static_cast<unsigned>(sp);
-            }
-            const unsigned i0 = at / static_cast<unsigned>(kv_heads);
-            p.hk = at - i0 * kv_heads;
-            const int i = blocks.of(l) - 1 - above - static_cast<int>(i0);  // longest first
-            p.first = l.first;
-            p.len = l.len;
-            p.ctx = l.ctx;
-            p.tok0 = i * blocks.span;
-            p.toks = min(l.q - p.tok0, blocks.span);
-            const int n = tiles_of(l, p.tok0 + p.toks), per = sp > 1 ? (n + sp - 1) / sp : n;
-            p.k0 = min(p.split * per, n);
-            const int k1 = min(p.k0 + per, n);
-            p.slot = slot_base + sinc - slots + (i * kv_heads + p.hk) * sp;
-            p.bad = l.bad;
-            p.total = k1 - p.k0;
-            p.halves = p.toks <= g.tile_tokens;
-            p.n[0] = p.halves ? (p.total + 1) / 2 : max(min(tiles_of(l, p.tok0 + g.tile_tokens), k1) - p.k0, 0);
-            p.n[1] = p.halves ? p.total / 2 : p.total;
-            if (l.bad) report(a.status, MKB_SERVE_BAD_LENGTH);
+        if (is_it) {
+          unsigned at = static_cast<unsigned>(r) - (inc - here), split = 0;
+          if (sp > 1) {
+            split = at % static_cast<unsigned>(sp);
+            at /= static_cast<unsigned>(sp);
           }
-          const int src = __ffs(who) - 1;
-          uint32_t* w = reinterpret_cast<uint32_t*>(&p);
-#pragma unroll
-          for (int i = 0; i < static_cast<int>(sizeof(Piece) / 4); ++i) w[i] = __shfl_sync(0xffffffffu, w[i], src);
-          break;
+          const unsigned i0 = at / static_cast<unsigned>(kv_heads);
+          const int hk = at - i0 * kv_heads, i = l.blocks - 1 - above - static_cast<int>(i0);  // longest first
+          const int tok0 = i * blocks.span, toks = min(l.q - tok0, blocks.span);
+          const int n = tiles_of(l, tok0 + toks);
+          const int per = sp > 1 ? static_cast<int>((static_cast<unsigned>(n) + sp - 1) / sp) : n;
+          const int k0 = min(static_cast<int>(split) * per, n), k1 = min(k0 + per, n), total = k1 - k0;
+          const bool halves = toks <= g.tile_tokens;
+          p.b = b;
+          p.hk = hk;
+          p.first = l.first;
+          p.tok0 = tok0;
+          p.toks = toks;
+          p.ctx = l.ctx;
+          p.len = l.len;
+          p.k0 = k0;
+          p.total = total;
+          p.n[0] = halves ? (total + 1) / 2 : max(min(tiles_of(l, tok0 + g.tile_tokens), k1) - k0, 0);
+          p.n[1] = halves ? total / 2 : total;
+          p.halves = halves;
+          p.splits = sp;
+          p.split = split;
+          p.slot = slot_base + sinc - slots + (i * kv_heads + hk) * sp;
+          p.bad = l.bad;
+          if (l.bad) report(a.status, MKB_SERVE_BAD_LENGTH);
         }
+        if (__any_sync(0xffffffffu, is_it)) break;
         r -= __shfl_sync(0xffffffffu, inc, 31);
         slot_base += __shfl_sync(0xffffffffu, sinc, 31);
+        found = b0 + 32 < a.batch;
       }
-      if (k >= 2) wait_for(&sm.info_empty[st], ((k >> 1) - 1) & 1, &sm.err, dead);
-      if (lane == 0) {
-        sm.piece[st] = p;
-        mbar_arrive(&sm.info_full[st]);
-      }
+      if (!found && lane == 0) p.b = -1;
       __syncwarp();
-      if (p.b < 0) break;
+      if (lane == 0) mbar_arrive(&sm.info_full[st]);
+      if (!found) break;
+    }
+    // the last CTA to have asked for its last piece puts the list back to its start
+    if (lane == 0 && atomicInc(g.work + 1, grid - 1) == static_cast<uint32_t>(grid - 1)) atomicExch(g.work, 0u);
+  } else if (warp == 9) {
+    // ---- the loads of a piece -----------------------------------------------------------------
+    if (lane == 0) {
+      tc::prefetch_tensormap(&tk);
+      tc::prefetch_tensormap(&tv);
+      tc::prefetch_tensormap(&tq);
+    }
+    int slot = 0, q_uses[2] = {0, 0};  // the ring's next slot, and how often it has gone round
+    uint32_t round = 0;
+    for (int k = 0; !dead; ++k) {
+      const int st = k & 1;
+      wait_for(&sm.info_full[st], (k >> 1) & 1, &sm.err, dead);
+      const Piece p = sm.piece[st];
+      if (p.b < 0 || dead) break;
       // K(0), then K(j + 1) and V(j): the order in which the products take them
       const int n = p.total;
       const int outside = max(a.pages, 1);  // (an empty pool's map has one page, that is never read)
@@ -593,12 +622,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
       }
       for (int j = 0; j < n && !dead; ++j) {
+        if (lane == 0 && j == max(n - kAskTiles, 0)) mbar_arrive(&sm.ask);
         if (j + 1 < n) load(&tk, kh, j + 1);
         load(&tv, vh, j);
       }
+      __syncwarp();
+      if (lane == 0) {
+        if (n == 0) mbar_arrive(&sm.ask);
+        mbar_arrive(&sm.info_empty[st]);
+      }
     }
-    // the last CTA to have asked for its last piece puts the list back to its start
-    if (lane == 0 && atomicInc(g.work + 1, grid - 1) == static_cast<uint32_t>(grid - 1)) atomicExch(g.work, 0u);
     // after a stop, wait (bounded) for the copies still in flight before leaving
     if (sm.err) {
       int tries = 0;
