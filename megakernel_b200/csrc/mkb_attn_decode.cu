@@ -32,9 +32,10 @@ namespace mkb {
 namespace sv {
 
 constexpr int kDecWarps = 8;
+constexpr int kDecRows = 8;      // rows of a KV head: the columns of one mma
 constexpr int kTileKeys = 16;    // keys of a tile: the rows of one mma
 constexpr int kCtaTiles = 16;    // tiles that are worth a CTA where few requests are long ...
-constexpr int kLongTiles = 48;   // ... which is what more tiles than this a request and KV head is
+constexpr int kLongTiles = 64;   // ... which is what more tiles than this a request and KV head is
 constexpr int kWholeTiles = 8;   // below this a request's tiles (of a KV head) stay with one warp
 constexpr int kDecTryNs = 20000, kDecTries = 50000;  // bound of a wait: about a second
 
@@ -44,16 +45,19 @@ struct DecArgs {
   int k_head, v_head;  // 0 where every KV head lies at the same place (stride 0), else 1
   int group, rows;     // query heads of a KV head; rows (q_len * group)
   int cols;            // rows up to a power of two: columns of a part
-  int stages;          // tiles of a warp's ring
-  int warp_bytes;      // a warp's shared memory: the ring, then the part that it does not begin
   uint32_t* counters;  // [ctas], zero between calls
-  float* part;         // [2 ctas][D][16] O^T, the maxima and sums in stat [2 ctas][2][16]
+  float* part;         // [2 ctas][D][cols] O^T, the maxima and sums in stat [2 ctas][2][kDecRows]
   float* stat;
 };
 
-constexpr int kMaxStages = 6;
 template <int D>
 constexpr int kStageBytes = kTileKeys * D * 2 * 2;  // K and V of a tile
+// Tiles of a warp's ring: 24 KB, which leaves room for a part beside each of the eight.
+template <int D>
+constexpr int kStages = 24 * 1024 / kStageBytes<D>;
+// A warp's shared memory: the ring, then the part that it does not begin.
+template <int D>
+constexpr int kWarpBytes = kStages<D> * kStageBytes<D> + D * kDecRows * 4;
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t r[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -99,33 +103,31 @@ struct Cursor {
   int64_t pos;
 };
 
-// kN: columns of 8 rows each (1 or 2)
-template <typename T, int D, int kN>
+template <typename T, int D>
 __global__ void __launch_bounds__(32 * kDecWarps, 1)
     attn_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                        const __grid_constant__ DecArgs g) {
   constexpr int kBytes = kStageBytes<D>, kHalf = kTileKeys * 128;  // (64 values of 16 keys)
-  constexpr int kPer = D / 32;
+  constexpr int kPer = D / 32, kRing = kStages<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kDecWarps][kMaxStages];
-  __shared__ float part_m[kDecWarps][2][16], part_l[kDecWarps][2][16];
+  __shared__ uint64_t full[kDecWarps][kRing];
+  __shared__ float part_m[kDecWarps][2][kDecRows], part_l[kDecWarps][2][kDecRows];
   __shared__ int64_t part_pos[kDecWarps][2];                   // the request's and KV head's place, -1: none
   __shared__ int part_at[kDecWarps][2][4];                     // b, hk, len, n
-  __shared__ float fac[2 * kDecWarps][16], sum_m[2 * kDecWarps][16], sum_l[2 * kDecWarps][16];
   __shared__ int flags[2][2], err;
   const mkb_attn_args& a = g.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   depend_launch();
-  uint8_t* const mine = smem + warp * g.warp_bytes;
+  uint8_t* const mine = smem + warp * kWarpBytes<D>;
   const uint32_t ring = smem_addr(mine);
   // parts: 0 goes on from the warp before, 1 begins here (and lies over the ring, at the end)
-  float* const part_o[2] = {reinterpret_cast<float*>(mine + g.stages * kBytes), reinterpret_cast<float*>(mine)};
+  float* const part_o[2] = {reinterpret_cast<float*>(mine + kRing * kBytes), reinterpret_cast<float*>(mine)};
   if (lane < 2) part_pos[warp][lane] = -1;
   if (lane == 0) {
     tc::prefetch_tensormap(&tk);
     tc::prefetch_tensormap(&tv);
-    for (int i = 0; i < g.stages; ++i) mbar_init(&full[warp][i], 1);
+    for (int i = 0; i < kRing; ++i) mbar_init(&full[warp][i], 1);
     fence_mbar_init();
   }
   if (threadIdx.x == 0) err = 0;
@@ -188,17 +190,24 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     }
     ahead.pos += __shfl_sync(0xffffffffu, inc, 31);
   }
-  // a cut at x as a tile of the request and KV head that c stands at
-  auto tile_at = [&](int64_t x, int64_t pos, int n) {
+  // a cut at x as a tile of the request and KV head that starts at pos; one between CTAs
+  // (every cut, where there is more than one of those a CTA) leaves short ones whole
+  auto tile_in = [&](int64_t x, int64_t pos, int n, bool whole) {
     const int64_t y = x - pos;
     if (y <= 0) return 0;
     if (y >= n + 1) return n;
-    if (n < kWholeTiles) return 2 * y >= n + 1 ? n : 0;
+    if (whole && n < kWholeTiles) return 2 * y >= n + 1 ? n : 0;
     return static_cast<int>(y) - 1;
   };
+  auto tile_at = [&](int64_t x, int64_t pos, int n) { return tile_in(x, pos, n, true); };
+  const bool many = heads > ctas;
   auto enter = [&](Cursor& c) {  // the part of c's tiles that is this warp's
     c.t = tile_at(from, c.pos, c.n);
     c.t_end = tile_at(to, c.pos, c.n);
+    if (many || c.n >= kWholeTiles) return;
+    const int lo = tile_at(cta_from, c.pos, c.n), hi = tile_at(cta_from + cta_units, c.pos, c.n);  // its CTA's part
+    if (from != cta_from) c.t = min(max(tile_in(from, c.pos, c.n, false), lo), hi);
+    if (to != cta_from + cta_units) c.t_end = min(max(tile_in(to, c.pos, c.n, false), lo), hi);
   };
   auto leave = [&](Cursor& c) {  // on to the next request and KV head
     c.pos += c.n + 1;
@@ -252,11 +261,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     }
     bad_pages = (bad_pages & ~(1u << load_bit)) | static_cast<uint32_t>(oob) << load_bit;
     load_bit = (load_bit + 1) & 31;
-    if (++fill == g.stages) fill = 0;
+    if (++fill == kRing) fill = 0;
     ++ahead.t;
   };
 #pragma unroll 1
-  for (int i = 0; i < g.stages - 1; ++i) load();
+  for (int i = 0; i < kRing - 1; ++i) load();
 
   uint32_t phase = 0;
   int stage = 0;
@@ -265,34 +274,31 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     const int t0 = cur.t, t1 = cur.t_end, b = cur.b, hk = cur.hk, len = cur.len;
     const int first_pos = len - a.q_len;  // position of the request's first new token
     // Q^T as the B operand: columns are rows of Q (row = token * group + head)
-    uint32_t qf[kN][D / 16][2];
-    int lim[kN][2];  // of this lane's columns of S^T, rows 8 nn + 2 (lane % 4) + {0, 1}
-    float m[kN][2], l[kN][2], o[D / 16][kN][4];
+    uint32_t qf[D / 16][2];
+    int lim[2];  // of this lane's columns of S^T, rows 2 (lane % 4) + {0, 1}
+    float m[2], l[2], o[D / 16][4];
+    const int r = lane / 4;
+    const bool live = r < g.rows;
+    const int tok = live ? r / g.group : 0, h = hk * g.group + (live ? r - tok * g.group : 0);
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q) +
+                                                          (static_cast<int64_t>(b) * a.q_len + tok) * a.q_stride[0] +
+                                                          h * a.q_stride[1]);
 #pragma unroll
-    for (int nn = 0; nn < kN; ++nn) {
-      const int r = 8 * nn + lane / 4;
-      const bool live = r < g.rows;
-      const int tok = live ? r / g.group : 0, h = hk * g.group + (live ? r - tok * g.group : 0);
-      const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q) +
-                                                            (static_cast<int64_t>(b) * a.q_len + tok) * a.q_stride[0] +
-                                                            h * a.q_stride[1]);
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        qf[nn][kk][0] = live ? __ldg(q + 8 * kk + lane % 4) : 0;
-        qf[nn][kk][1] = live ? __ldg(q + 8 * kk + 4 + lane % 4) : 0;
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int re = 8 * nn + 2 * (lane % 4) + e;
-        lim[nn][e] = re < g.rows ? min(first_pos + re / g.group, len - 1) : -1;
-        m[nn][e] = -INFINITY;
-        l[nn][e] = 0.f;
-      }
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[d][nn][e] = 0.f;
+    for (int kk = 0; kk < D / 16; ++kk) {
+      qf[kk][0] = live ? __ldg(q + 8 * kk + lane % 4) : 0;
+      qf[kk][1] = live ? __ldg(q + 8 * kk + 4 + lane % 4) : 0;
     }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int re = 2 * (lane % 4) + e;
+      lim[e] = re < g.rows ? min(first_pos + re / g.group, len - 1) : -1;
+      m[e] = -INFINITY;
+      l[e] = 0.f;
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
 
     for (int t = t0; t < t1; ++t) {
       load();
@@ -313,72 +319,61 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
         fence_proxy_async_shared();
         __syncwarp();
       }
-      if (++stage == g.stages) {
+      if (++stage == kRing) {
         stage = 0;
         phase ^= 1;
       }
-      float s[kN][4] = {};
+      float s[4] = {};
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {  // A: keys by dims
         uint32_t ka[4];
         const int r = lane % 16, x = 2 * (kk % 4) + lane / 16;
         ldsm4(kt + kk / 4 * kHalf + r * 128 + ((x ^ (r & 7)) << 4), ka);
-#pragma unroll
-        for (int nn = 0; nn < kN; ++nn) mma16816<T>(s[nn], ka, qf[nn][kk][0], qf[nn][kk][1]);
+        mma16816<T>(s, ka, qf[kk][0], qf[kk][1]);
       }
-      // s[nn][e], s[nn][2 + e]: keys lane / 4 and lane / 4 + 8, row 8 nn + 2 (lane % 4) + e
+      // s[e], s[2 + e]: keys lane / 4 and lane / 4 + 8, row 2 (lane % 4) + e
       if (bad_pages >> bad_bit & 1u) {  // a page outside the pool: its keys are NaN
 #pragma unroll
-        for (int nn = 0; nn < kN; ++nn)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[nn][e] = NAN;
+        for (int e = 0; e < 4; ++e) s[e] = NAN;
       }
       bad_bit = (bad_bit + 1) & 31;
-      uint32_t ph[kN][2], pl[kN][2];
+      float p[4];
 #pragma unroll
-      for (int nn = 0; nn < kN; ++nn) {
-        float p[4];
+      for (int e = 0; e < 2; ++e) {
+        const int j = key + lane / 4;
+        const float x0 = j <= lim[e] ? s[e] * g.sl2 : -INFINITY;
+        const float x1 = j + 8 <= lim[e] ? s[2 + e] * g.sl2 : -INFINITY;
+        float mx = fmaxf(x0, x1);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = key + lane / 4;
-          const float x0 = j <= lim[nn][e] ? s[nn][e] * g.sl2 : -INFINITY;
-          const float x1 = j + 8 <= lim[nn][e] ? s[nn][2 + e] * g.sl2 : -INFINITY;
-          float mx = fmaxf(x0, x1);
+        for (int w = 4; w < 32; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        const float mn = fmaxf(m[e], mx);
+        const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: weights of 0
+        const float sc = ex2_approx(m[e] - ref);
+        m[e] = mn;
+        p[e] = ex2_approx(x0 - ref);
+        p[2 + e] = ex2_approx(x1 - ref);
+        l[e] = l[e] * sc + (p[e] + p[2 + e]);  // of this lane's keys: added up at the end
+        if (__any_sync(0xffffffffu, sc != 1.f)) {
 #pragma unroll
-          for (int w = 4; w < 32; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-          const float mn = fmaxf(m[nn][e], mx);
-          const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: weights of 0
-          const float sc = ex2_approx(m[nn][e] - ref);
-          m[nn][e] = mn;
-          p[e] = ex2_approx(x0 - ref);
-          p[2 + e] = ex2_approx(x1 - ref);
-          l[nn][e] = l[nn][e] * sc + (p[e] + p[2 + e]);  // of this lane's keys: added up at the end
-          if (__any_sync(0xffffffffu, sc != 1.f)) {
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-              o[d][nn][e] *= sc;
-              o[d][nn][2 + e] *= sc;
-            }
+          for (int d = 0; d < D / 16; ++d) {
+            o[d][e] *= sc;
+            o[d][2 + e] *= sc;
           }
         }
-        // transposed into the B operand: keys down, rows across; high part and remainder
-        const uint32_t h0 = Pair<T>::put(p[0], p[1]), h1 = Pair<T>::put(p[2], p[3]);
-        const float2 f0 = Pair<T>::get(h0), f1 = Pair<T>::get(h1);
-        ph[nn][0] = transpose8x8(h0);
-        ph[nn][1] = transpose8x8(h1);
-        pl[nn][0] = transpose8x8(Pair<T>::put(p[0] - f0.x, p[1] - f0.y));
-        pl[nn][1] = transpose8x8(Pair<T>::put(p[2] - f1.x, p[3] - f1.y));
       }
+      // transposed into the B operand: keys down, rows across; high part and remainder
+      const uint32_t h0 = Pair<T>::put(p[0], p[1]), h1 = Pair<T>::put(p[2], p[3]);
+      const float2 f0 = Pair<T>::get(h0), f1 = Pair<T>::get(h1);
+      const uint32_t ph[2] = {transpose8x8(h0), transpose8x8(h1)};
+      const uint32_t pl[2] = {transpose8x8(Pair<T>::put(p[0] - f0.x, p[1] - f0.y)),
+                              transpose8x8(Pair<T>::put(p[2] - f1.x, p[3] - f1.y))};
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {  // A: dims by keys, V transposed on the way
         uint32_t va[4];
         const int r = lane % 8 + 8 * (lane / 16), x = 2 * (d % 4) + (lane / 8) % 2;
         ldsm4_t(vt + d / 4 * kHalf + r * 128 + ((x ^ (r & 7)) << 4), va);
-#pragma unroll
-        for (int nn = 0; nn < kN; ++nn) {
-          mma16816<T>(o[d][nn], va, ph[nn][0], ph[nn][1]);
-          mma16816<T>(o[d][nn], va, pl[nn][0], pl[nn][1]);
-        }
+        mma16816<T>(o[d], va, ph[0], ph[1]);
+        mma16816<T>(o[d], va, pl[0], pl[1]);
       }
       __syncwarp();  // the stage may be filled again
     }
@@ -390,45 +385,43 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     const int which = t0 == 0;
     uint32_t odd = 0;  // rows whose O is not finite
 #pragma unroll
-    for (int nn = 0; nn < kN; ++nn)
+    for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int w = 4; w < 32; w <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], w);
+      if (wrong) l[e] = NAN;
+      const int r = 2 * (lane % 4) + e;
+      float z = 0.f;
 #pragma unroll
-        for (int w = 4; w < 32; w <<= 1) l[nn][e] += __shfl_xor_sync(0xffffffffu, l[nn][e], w);
-        if (wrong) l[nn][e] = NAN;
-        const int r = 8 * nn + 2 * (lane % 4) + e;
-        float z = 0.f;
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d) z = fmaf(o[d][nn][e], 0.f, fmaf(o[d][nn][2 + e], 0.f, z));
-        if (z != 0.f) odd |= 1u << r;
-        if (whole) {
-          if (r < g.rows) {
-            const int tok = r / g.group, h = hk * g.group + r - tok * g.group;
-            const bool zero = lim[nn][e] < 0 && !wrong;  // a row that sees no key
-            const float inv = 1.f / l[nn][e];
-            uint16_t* out = reinterpret_cast<uint16_t*>(static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.q_len + tok) * a.out_stride[0] +
-                                                        h * a.out_stride[1]);
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-              const uint32_t w2 = Pair<T>::put(o[d][nn][e] * inv, o[d][nn][2 + e] * inv);
-              out[16 * d + lane / 4] = zero ? 0 : static_cast<uint16_t>(w2);
-              out[16 * d + 8 + lane / 4] = zero ? 0 : static_cast<uint16_t>(w2 >> 16);
-            }
-          }
-        } else {
+      for (int d = 0; d < D / 16; ++d) z = fmaf(o[d][e], 0.f, fmaf(o[d][2 + e], 0.f, z));
+      if (z != 0.f) odd |= 1u << r;
+      if (whole) {
+        if (r < g.rows) {
+          const int tok = r / g.group, h = hk * g.group + r - tok * g.group;
+          const bool zero = lim[e] < 0 && !wrong;  // a row that sees no key
+          const float inv = 1.f / l[e];
+          uint16_t* out = reinterpret_cast<uint16_t*>(static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.q_len + tok) * a.out_stride[0] +
+                                                      h * a.out_stride[1]);
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) {
-            if (r < g.cols) {
-              part_o[which][(16 * d + lane / 4) * g.cols + r] = o[d][nn][e];
-              part_o[which][(16 * d + 8 + lane / 4) * g.cols + r] = o[d][nn][2 + e];
-            }
-          }
-          if (lane < 4) {
-            part_m[warp][which][r] = m[nn][e];
-            part_l[warp][which][r] = l[nn][e];
+            const uint32_t w2 = Pair<T>::put(o[d][e] * inv, o[d][2 + e] * inv);
+            out[16 * d + lane / 4] = zero ? 0 : static_cast<uint16_t>(w2);
+            out[16 * d + 8 + lane / 4] = zero ? 0 : static_cast<uint16_t>(w2 >> 16);
           }
         }
+      } else {
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          if (r < g.cols) {
+            part_o[which][(16 * d + lane / 4) * g.cols + r] = o[d][e];
+            part_o[which][(16 * d + 8 + lane / 4) * g.cols + r] = o[d][2 + e];
+          }
+        }
+        if (lane < 4) {
+          part_m[warp][which][r] = m[e];
+          part_l[warp][which][r] = l[e];
+        }
       }
+    }
     if (!whole && lane == 0) {
       part_pos[warp][which] = cur.pos;
       part_at[warp][which][0] = b;
@@ -479,6 +472,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   // Part p = 2 warp + (0 or 1), in order of their keys; those of one request and KV head are
   // neighbours. First every part's weight beside the largest maximum of its row, a lane a part:
   constexpr int kParts = 2 * kDecWarps;
+  // (these lie over the first warp's ring, behind its part)
+  float(*const fac)[kDecRows] = reinterpret_cast<float(*)[kDecRows]>(smem + D * kDecRows * 4);
+  float(*const sum_m)[kDecRows] = fac + kParts;
+  float(*const sum_l)[kDecRows] = sum_m + kParts;
+  static_assert((D + 3 * kParts) * kDecRows * 4 <= kRing * kBytes, "room of the first warp's ring");
   const int64_t my_pos = lane < kParts ? part_pos[lane / 2][lane % 2] : -1;
   uint32_t same = 0;  // the parts that go with the lane's
 #pragma unroll
@@ -527,16 +525,16 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
       float v = 0.f;
       for (uint32_t u = parts; u != 0; u &= u - 1) {
         const int p = __ffs(u) - 1;
-        const uint8_t* base = smem + (p / 2) * g.warp_bytes + (p % 2 == 0 ? g.stages * kBytes : 0);
+        const uint8_t* base = smem + (p / 2) * kWarpBytes<D> + (p % 2 == 0 ? kRing * kBytes : 0);
         v += reinterpret_cast<const float*>(base)[i] * fac[p][r];
       }
       if (here) write_out(b, hk, len, i, v, sum_l[p0][r]);
-      else g.part[static_cast<size_t>(slot) * D * 16 + i] = v;
+      else g.part[static_cast<size_t>(slot) * D * kDecRows + i] = v;
     }
     if (!here) {
       if (threadIdx.x < g.rows) {
-        g.stat[slot * 32 + threadIdx.x] = sum_m[p0][threadIdx.x];
-        g.stat[slot * 32 + 16 + threadIdx.x] = sum_l[p0][threadIdx.x];
+        g.stat[slot * 2 * kDecRows + threadIdx.x] = sum_m[p0][threadIdx.x];
+        g.stat[(slot * 2 + 1) * kDecRows + threadIdx.x] = sum_l[p0][threadIdx.x];
       }
       cross[crosses++ & 1] = p0;
     }
@@ -565,13 +563,13 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     const int b = at[0], hk = at[1], len = at[2];
     for (int r = warp; r < g.rows; r += kDecWarps) {  // a warp a row, a lane a CTA
       float mm = -INFINITY, ll = 0.f;
-      for (int c = c0 + lane; c <= c1; c += 32) mm = fmaxf(mm, __ldcg(g.stat + (2 * c + (c == c0)) * 32 + r));
+      for (int c = c0 + lane; c <= c1; c += 32) mm = fmaxf(mm, __ldcg(g.stat + (2 * c + (c == c0)) * 2 * kDecRows + r));
 #pragma unroll
       for (int w = 16; w > 0; w >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, w));
       const float ref = mm == -INFINITY ? 0.f : mm;
       for (int c = c0 + lane; c <= c1; c += 32) {
-        const float* st = g.stat + (2 * c + (c == c0)) * 32 + r;
-        ll += __ldcg(st + 16) * ex2_approx(__ldcg(st) - ref);
+        const float* st = g.stat + (2 * c + (c == c0)) * 2 * kDecRows + r;
+        ll += __ldcg(st + kDecRows) * ex2_approx(__ldcg(st) - ref);
       }
 #pragma unroll
       for (int w = 16; w > 0; w >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, w);
@@ -589,7 +587,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
 #pragma unroll 8
       for (int c = c0; c <= c1; ++c) {
         const int s = 2 * c + (c == c0);
-        v += __ldcg(g.part + static_cast<size_t>(s) * D * 16 + i) * ex2_approx(__ldcg(g.stat + s * 32 + r) - ref);
+        v += __ldcg(g.part + static_cast<size_t>(s) * D * kDecRows + i) * ex2_approx(__ldcg(g.stat + s * 2 * kDecRows + r) - ref);
       }
       write_out(b, hk, len, i, v, sum_l[p0][r]);
     }
@@ -605,10 +603,10 @@ cudaError_t map_rows(CUtensorMap* m, int dtype, const void* base, int D, int ran
 size_t counter_bytes();
 
 size_t decode_workspace(const mkb_attn_args& a) {
-  return counter_bytes() + 2 * static_cast<size_t>(sm_count()) * (32 + static_cast<size_t>(a.head_dim) * 16) * 4;
+  return counter_bytes() + 2 * static_cast<size_t>(sm_count()) * (2 + static_cast<size_t>(a.head_dim)) * kDecRows * 4;
 }
 
-template <typename T, int D, int kN>
+template <typename T, int D>
 static cudaError_t decode_launch(const mkb_attn_args& a, cudaStream_t stream) {
   DecArgs g;
   g.a = a;
@@ -621,14 +619,10 @@ static cudaError_t decode_launch(const mkb_attn_args& a, cudaStream_t stream) {
   if (ws == nullptr) return cudaErrorInvalidValue;
   g.counters = reinterpret_cast<uint32_t*>(ws);
   g.stat = reinterpret_cast<float*>(ws + counter_bytes());
-  g.part = g.stat + 2 * static_cast<size_t>(sm_count()) * 32;
+  g.part = g.stat + 2 * static_cast<size_t>(sm_count()) * 2 * kDecRows;
   for (g.cols = 2; g.cols < g.rows;) g.cols *= 2;
-  // as many tiles of 128-wide (64-wide) heads as the part beside them leaves room for (a part
-  // is smaller than any of these rings, which the last one lies over)
-  g.stages = D == 64 ? (g.cols <= 8 ? kMaxStages : kMaxStages - 1) : g.cols <= 4 ? 3 : 2;
-  g.warp_bytes = (g.stages * kStageBytes<D> + D * g.cols * 4 + 1023) / 1024 * 1024;  // (swizzle atoms)
-  constexpr size_t most_bytes = 216 * 1024;
-  const size_t bytes = static_cast<size_t>(kDecWarps) * g.warp_bytes + 1024;
+  constexpr int bytes = kDecWarps * kWarpBytes<D> + 1024;
+  static_assert(kWarpBytes<D> % 1024 == 0, "swizzle atoms");
   static bool configured[64] = {false};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -645,7 +639,7 @@ static cudaError_t decode_launch(const mkb_attn_args& a, cudaStream_t stream) {
   if ((e = map_rows(&mv, a.dtype, vb, D, 3, dims, vs, box)) != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(attn_decode_kernel<T, D, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most_bytes));
+    e = cudaFuncSetAttribute(attn_decode_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
@@ -653,19 +647,17 @@ static cudaError_t decode_launch(const mkb_attn_args& a, cudaStream_t stream) {
   const int64_t most = static_cast<int64_t>(a.batch) * a.kv_heads *
                        (static_cast<int64_t>(a.table_width) * a.page_size / (kTileKeys * kCtaTiles) + 1);
   const int grid = static_cast<int>(most < sm_count() ? most : sm_count());
-  return launch_early(attn_decode_kernel<T, D, kN>, grid, 32 * kDecWarps, bytes, stream, mk, mv, g);
+  return launch_early(attn_decode_kernel<T, D>, grid, 32 * kDecWarps, bytes, stream, mk, mv, g);
 }
 
 // Few enough rows a KV head for one tile of columns.
 bool decode_fits(const mkb_attn_args& a) {
-  return a.cu_q == nullptr && static_cast<int64_t>(a.q_len) * (a.heads / a.kv_heads) <= 16;
+  return a.cu_q == nullptr && static_cast<int64_t>(a.q_len) * (a.heads / a.kv_heads) <= kDecRows;
 }
 
 template <typename T>
 static cudaError_t decode_type(const mkb_attn_args& a, cudaStream_t stream) {
-  const bool one = a.q_len * (a.heads / a.kv_heads) <= 8;
-  if (a.head_dim == 128) return one ? decode_launch<T, 128, 1>(a, stream) : decode_launch<T, 128, 2>(a, stream);
-  return one ? decode_launch<T, 64, 1>(a, stream) : decode_launch<T, 64, 2>(a, stream);
+  return a.head_dim == 128 ? decode_launch<T, 128>(a, stream) : decode_launch<T, 64>(a, stream);
 }
 
 cudaError_t attn_decode(const mkb_attn_args& a, cudaStream_t stream) {
