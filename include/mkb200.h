@@ -340,7 +340,8 @@ typedef struct mkb_attn_args {
   int table_width, pages, page_size; /* page_size a power of two, 16 or more */
   float scale;                 /* scores are scale * q.k */
   void* workspace;             /* device, mkb_attn_workspace_bytes(); zeroed once with
-                                  mkb_attn_workspace_reset and left zeroed by every call.
+                                  mkb_attn_workspace_reset and left ready for the next call
+                                  of any shape that fits.
                                   Calls that share one must not overlap in time. */
   uint32_t* status;            /* device uint32 or NULL */
 } mkb_attn_args;
@@ -382,8 +383,8 @@ cudaError_t mkb_paged_attention(const mkb_attn_args* a, cudaStream_t stream);
  * rotate-half RoPE at the token's position, q to q_out, k and v to the cache (k
  * also to k_out, packed). Two tokens at the same page and slot race. Asynchronous. */
 cudaError_t mkb_paged_append(const mkb_append_args* a, cudaStream_t stream);
-/* Bytes of workspace an attention call with these arguments needs (tokens, batch,
- * heads, kv_heads, head_dim and q_len / cu_q are read). */
+/* Bytes of workspace an attention call with these arguments needs on the current
+ * device (head_dim alone is read); 0 where there is no such call. */
 size_t mkb_attn_workspace_bytes(const mkb_attn_args* a);
 cudaError_t mkb_attn_workspace_reset(void* workspace, size_t bytes, cudaStream_t stream);
 

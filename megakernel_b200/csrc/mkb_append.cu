@@ -182,13 +182,6 @@ cudaError_t append_source(const mkb_append_args& a, cudaStream_t stream) {
   return append_dim<float, T>(a, stream);
 }
 
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-static bool strides_ok(const int64_t* s, int n) {
-  for (int i = 0; i < n; ++i)
-    if (s[i] < 0 || s[i] % 8) return false;
-  return true;
-}
-
 }  // namespace sv
 }  // namespace mkb
 

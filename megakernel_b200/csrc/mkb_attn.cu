@@ -13,13 +13,6 @@ cudaError_t attn_decode(const mkb_attn_args& a, cudaStream_t stream);  // mkb_at
 size_t decode_workspace(const mkb_attn_args& a);
 bool decode_fits(const mkb_attn_args& a);
 
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-static bool strides_ok(const int64_t* s, int n) {
-  for (int i = 0; i < n; ++i)
-    if (s[i] < 0 || s[i] % 8) return false;
-  return true;
-}
-
 // What both entry points refuse before a launch.
 static cudaError_t check_attn(const mkb_attn_args* a, bool paged) {
   if (a == nullptr || a->tokens < 0 || a->batch < 0) return cudaErrorInvalidValue;
@@ -61,6 +54,7 @@ static cudaError_t check_attn(const mkb_attn_args* a, bool paged) {
 extern "C" {
 
 size_t mkb_attn_workspace_bytes(const mkb_attn_args* a) {
+  if (a == nullptr || (a->head_dim != 64 && a->head_dim != 128)) return 0;
   // (their counters share their place: both leave them zero)
   const size_t t = mkb::sv::tc_workspace(*a), d = mkb::sv::decode_workspace(*a);
   return t > d ? t : d;
@@ -81,9 +75,12 @@ cudaError_t mkb_paged_attention(const mkb_attn_args* a, cudaStream_t stream) {
   using namespace mkb::sv;
   const cudaError_t e = check_attn(a, true);
   if (e != cudaSuccess || a->tokens == 0) return e;
-  // Up to 16 rows (new tokens x query heads of a KV head) known from the shapes alone: bytes
+  // Up to 8 rows (new tokens x query heads of a KV head) known from the shapes alone: bytes
   // bound the call, and the streaming kernel reads them fastest. More rows, or chunks of
-  // lengths that only the device knows: the tensor-core tiles.
+  // lengths that only the device knows: the tensor-core tiles. Streaming against tiles, heads
+  // 16 over 8 of 128: 48 requests of 1-4,096 keys, 2 rows 58 and 69 us, 8 rows 71 and 70 (16,
+  // with two columns of products: 100 and 71); three of 9,001-60,000 keys, 2 rows 78 and 99,
+  // 8 rows 90 and 93 (16: 112 and 93); one of 33 keys 7.5 and 9.2.
   return decode_fits(*a) ? attn_decode(*a, stream) : attn_tc(*a, true, stream);
 }
 }

@@ -3,14 +3,14 @@
 //   out_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = 2^(c q_i.k_j - m_i),  c = scale log2(e),  j <= pos(i)
 //
 // Every key and value is read once from memory and used for the handful of rows (new
-// tokens x the query heads that share the KV head, 16 at most) that need it: bytes bound
+// tokens x the query heads that share the KV head, 8 at most) that need it: bytes bound
 // this kernel, at 4 D bytes a key and KV head. TMA brings them into shared memory (a box
 // of 16 keys x 64 values, 128-byte swizzle, so that the matrix loads below meet no bank
 // twice), a ring of tiles per warp, with no barrier between warps.
 //
 // The products run on mma.sync m16n8k16 with the keys as the 16 rows of S^T = K Q^T and
-// the queries as its columns (8 or 16 of them), so that the tile is filled by keys however
-// few the queries are: S^T's accumulators, transposed by movmatrix, are the B operand of
+// the queries as its 8 columns, so that the tile is filled by keys however few the queries
+// are: S^T's accumulators, transposed by movmatrix, are the B operand of
 // O^T += V^T P^T, and V^T comes from V by ldmatrix.trans. P enters as a 16-bit high part
 // and the remainder: memory leaves time for the second product, and P then costs no
 // precision.
@@ -22,6 +22,11 @@
 // leave O, maximum and sum in shared memory, where the CTA adds them up at its end; those
 // that go on in another CTA, in memory, where the last CTA to be done adds them up in
 // order of their keys.
+//
+// 48 requests of 1-4,096 keys, 16 heads over 8 of 128: 58 us for 273 MB. While it streams it
+// reads 6.2 TB/s of the 6.6 that a copy reaches, with 192 KB of copies in flight an SM (tiles
+// of 16 keys keep a ring a warp in that); 4 us pass before the first tile is there (launch,
+// lengths, page table, one after another) and 2 after the last (sums over warps and CTAs).
 
 #include <cmath>
 
@@ -34,9 +39,18 @@ namespace sv {
 constexpr int kDecWarps = 8;
 constexpr int kDecRows = 8;      // rows of a KV head: the columns of one mma
 constexpr int kTileKeys = 16;    // keys of a tile: the rows of one mma
-constexpr int kCtaTiles = 16;    // tiles that are worth a CTA where few requests are long ...
-constexpr int kLongTiles = 64;   // ... which is what more tiles than this a request and KV head is
-constexpr int kWholeTiles = 8;   // below this a request's tiles (of a KV head) stay with one warp
+// A CTA for every request and KV head, unless those have more than kLongTiles tiles on
+// average: then one for every kCtaTiles, as far as there are SMs. (8 requests of 700 keys: 13.0
+// us, spread out further 17.6, the sums over CTAs cost more than the keys; one of 4,000: 18.7
+// spread out, 40.7 not. With 64 tiles a CTA that one takes 23.7; with 4, 18.8, and one of 900
+// keys 17.2 instead of 16.0.)
+constexpr int kCtaTiles = 16;
+constexpr int kLongTiles = 64;
+// Below kWholeTiles a request's tiles of a KV head stay together: in one warp, or in one CTA
+// where there are enough of those for each. (256 requests of 100 keys: 32.3 us, 41.1 when they
+// are cut anywhere; 48 of 1-4,096 keys: 58.1, 58.8 cut anywhere, 59.8 with 32 tiles. One of 33
+// keys: 7.4, 8.1 in one warp.)
+constexpr int kWholeTiles = 8;
 constexpr int kDecTryNs = 20000, kDecTries = 50000;  // bound of a wait: about a second
 
 struct DecArgs {

@@ -19,10 +19,17 @@
 //   warps 0-3   softmax of tile A, a thread per row: S out of tensor memory, running
 //   warps 4-7   maximum and sum in FP32 registers, P into tensor memory; tile B
 //
-// While one tile's softmax runs, the tensor core works on the other's products. (P in
-// columns of its own, so that the next S need not wait for it, leaves room for 80 keys a
-// tile only; both tiles' softmax then run at once and hold each other up: 2,330 cycles a
-// pair of 128 x 80 tiles.)
+// While one tile's softmax runs, the tensor core works on the other's products. Tensor core
+// (4 D cycles a 128 x 128 tile: 1,024 at D = 128) and exponentials (1,024: 16 a cycle and SM)
+// bound a pair of tiles at 2,048 cycles each; the chain of one tile (load 215, maximum 450,
+// weights 1,450, the rest of PV and the next S 1,100) makes it 3,250. 15,999 tokens, 16 heads
+// over 8 of 128: 820 us, 1,280 TFLOP/s (of 1,640 that a library GEMM reaches), both units 63 %
+// busy; 980 us once the power limit holds the clock (1,070 of 1,370 TFLOP/s).
+// What did not shorten the chain: P in columns of its own, so that the next S need not wait
+// for it (80 keys a tile at D = 128: 2,330 cycles a pair; both tiles' softmax then run at
+// once); the next S in halves, the upper one while the weights are worked out (3-10 % slower:
+// 64 columns cost the tensor core three quarters of 128); S read twice, 32 columns at a time
+// (5-25 % slower); part of the exponentials as polynomials (no gain).
 //
 // The running maximum that P is relative to moves only when a row's grows by more than 8
 // (a factor 256): O, in tensor memory, is then rescaled by the softmax warps; between
@@ -55,11 +62,18 @@ constexpr int kTcThreads = 384;
 // that hold 128 scores a thread (2 x 128 x 208 + 128 x 88 = 384 x 168).
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 constexpr int kRows = 256, kKeys = 128;   // rows of a piece (two tiles), keys of a tile
-constexpr int kFirstKeys = 96;            // of a tile's weights, what the second product starts on
+constexpr int kFirstKeys = 96;            // of a tile's weights, what the second product starts on (2 x 4,096
+                                          // tokens: 123 us; 126 with 64)
 constexpr int kHalf = 128 * 128;          // 16 KB: 128 rows x 64 values, 128-byte swizzle
-constexpr int kMinSplit = 6;              // key tiles (turns, of one tile's rows) below which rows are not split
-constexpr int kAskTiles = 3;              // key tiles to load when a CTA asks for its next piece
-constexpr int kSortBatch = 128;           // requests up to which pieces are taken longest first
+// Key tiles (turns, of one tile's rows) below which rows are not split: 1,200 tokens take 20.3
+// us, with 3 35.8, with 12 24.8.
+constexpr int kMinSplit = 6;
+// Key tiles still to load when a CTA asks for its next piece: 12 prompts of 1-1,411 tokens take
+// 35.4 us, with 8 37.3 (pieces are taken too long before their turn).
+constexpr int kAskTiles = 3;
+// Requests up to which pieces are taken longest first: 28 decoding and two chunks 71.6 us, as
+// they come 76.4; 200 prompts of 30-930 tokens 516 us, as they come 463.
+constexpr int kSortBatch = 128;
 constexpr int kTryNs = 20000, kTries = 50000;  // bound of every wait: about a second
 
 struct Piece {
@@ -378,8 +392,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == 11) {
     // ---- which piece comes next ----------------------------------------------------------
-    // (a warp of its own: working out a place in the list takes 3,000 cycles and more, which
-    // the loads of the next piece, 4,000 cycles late, do not get back)
+    // (a warp of its own: the place in the list takes 5,000 cycles to work out, and the loads
+    // of the next piece came that much late: 12 prompts of 1-1,411 tokens 37.7 us, now 35.3)
     const int kv_heads = a.kv_heads, grid = gridDim.x;
     // One pass over the requests: their blocks as pairs of tiles and as single ones, what
     // those come to in turns (linear in the block), and the longest.
@@ -400,7 +414,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     n1 = __reduce_add_sync(0xffffffffu, n1) * kv_heads;
     longest = __reduce_max_sync(0xffffffffu, longest);
     // pairs of tiles; single ones where the pairs are fewer than the CTAs, unless the keys are
-    // few and not all of those would have a CTA either
+    // few and not all of those would have a CTA either (1,200 tokens 20.3 us, in pairs 29.5)
     const bool single = n2 <= grid && (longest >= kMinSplit || n1 <= grid);
     const Blocks blocks = single ? singles : pairs;
     float total = single ? total1 : total2;
@@ -408,7 +422,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     top = single ? (longest + 1) / 2 : __reduce_max_sync(0xffffffffu, top);
     int count = single ? n1 : n2;  // of pieces
-    // a fair share of the turns; rows with more are split (but for those that stand before position 0)
+    // a fair share of the turns and a quarter; rows with more are split (but for those that stand
+    // before position 0). 12 prompts of 1-1,411 tokens: 35.7 us, at the bare share 52.5.
     const int cap = max(kMinSplit, static_cast<int>(fminf(total * kv_heads * 1.25f / grid, 1e9f)) + 1);
     auto share = [&](Load& l) {
       l.blocks = blocks.of(l);

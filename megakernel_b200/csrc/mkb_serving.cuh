@@ -167,6 +167,14 @@ cudaError_t launch_early(void (*kernel)(P...), int grid, int threads, size_t sme
   return cudaLaunchKernelEx(&c, kernel, std::forward<A>(args)...);
 }
 
+// ---- host: what the entry points check ---------------------------------------------------
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool strides_ok(const int64_t* s, int n) {  // (whole 16 bytes of the 16-bit types)
+  for (int i = 0; i < n; ++i)
+    if (s[i] < 0 || s[i] % 8) return false;
+  return true;
+}
+
 // Records the first error of a launch.
 __device__ __forceinline__ void report(uint32_t* status, uint32_t code) {
   if (status != nullptr) atomicCAS(status, 0u, code);
