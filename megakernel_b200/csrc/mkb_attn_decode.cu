@@ -259,16 +259,12 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
       const int page = __shfl_sync(0xffffffffu, pages, ahead.t - pages_at);
       const int slot = ahead.t * kTileKeys & (a.page_size - 1);
       oob = page < 0;
-      if (lane == 0) {
-        uint8_t* const dst = mine + fill * kBytes;
-        uint64_t* const bar = &full[warp][fill];
-        const int at = page < 0 ? max(a.pages, 1) : page;  // (outside the pool and its map: zeros)
-        mbar_arrive_expect_tx(bar, kBytes);
-#pragma unroll
-        for (int d = 0; d < D / 64; ++d) {
-          tc::tma_load_4d(dst + d * kHalf, &tk, 64 * d, slot, ahead.hk * g.k_head, at, bar);
-          tc::tma_load_4d(dst + kBytes / 2 + d * kHalf, &tv, 64 * d, slot, ahead.hk * g.v_head, at, bar);
-        }
+      uint64_t* const bar = &full[warp][fill];
+      const int at = oob ? max(a.pages, 1) : page;  // (outside the pool and its map: zeros)
+      if (lane == 0) mbar_arrive_expect_tx(bar, kBytes);
+      __syncwarp();
+      if (lane < 2) {  // K and V
+        tc::tma_load_5d(mine + fill * kBytes + lane * (kBytes / 2), lane ? &tv : &tk, 0, slot, 0, ahead.hk * (lane ? g.v_head : g.k_head), at, bar);
       }
     } else if (lane == 0) {
       mbar_arrive(&full[warp][fill]);  // nothing to bring
@@ -644,13 +640,15 @@ static cudaError_t decode_launch(const mkb_attn_args& a, cudaStream_t stream) {
   CUtensorMap mk, mv;
   const void* kb = a.pages > 0 ? a.k : a.q;  // an empty pool is never read: any address will do
   const void* vb = a.pages > 0 ? a.v : a.q;
-  const uint64_t dims[3] = {static_cast<uint64_t>(a.page_size), static_cast<uint64_t>(a.kv_heads),
+  // (a row's blocks of 64 values are a dimension of their own: one copy brings them all, block
+  // by block)
+  const uint64_t dims[4] = {static_cast<uint64_t>(a.page_size), D / 64, static_cast<uint64_t>(a.kv_heads),
                             static_cast<uint64_t>(a.pages)};
-  const int64_t ks[3] = {a.k_stride[2], a.k_stride[1], a.k_stride[0]};
-  const int64_t vs[3] = {a.v_stride[2], a.v_stride[1], a.v_stride[0]};
-  const uint32_t box[3] = {kTileKeys, 1, 1};
-  if ((e = map_rows(&mk, a.dtype, kb, D, 3, dims, ks, box)) != cudaSuccess) return e;
-  if ((e = map_rows(&mv, a.dtype, vb, D, 3, dims, vs, box)) != cudaSuccess) return e;
+  const int64_t ks[4] = {a.k_stride[2], 64, a.k_stride[1], a.k_stride[0]};
+  const int64_t vs[4] = {a.v_stride[2], 64, a.v_stride[1], a.v_stride[0]};
+  const uint32_t box[4] = {kTileKeys, D / 64, 1, 1};
+  if ((e = map_rows(&mk, a.dtype, kb, 64, 4, dims, ks, box)) != cudaSuccess) return e;
+  if ((e = map_rows(&mv, a.dtype, vb, 64, 4, dims, vs, box)) != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
     e = cudaFuncSetAttribute(attn_decode_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);

@@ -650,7 +650,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // after a stop, wait (bounded) for the copies still in flight before leaving
     if (sm.err) {
       int tries = 0;
-      for (int s = 0; s < kSlots; ++s) {  // its last use: in this round, or in the one before
+      for (int s = 0; s < kSlots; ++s) {  // its last use: in this lap, or in the one before
         const uint32_t r = s < slot ? round : round - 1;
         while ((s < slot || round > 0) && !mbar_wait(&sm.kv_full[s], r & 1, kTryNs) && ++tries < kTries) {
         }
@@ -1128,8 +1128,8 @@ cudaError_t map_rows(CUtensorMap* m, int dtype, const void* base, int D, int ran
                             const int64_t* strides, const uint32_t* box) {
   const EncodeTiled enc = encoder();
   if (!enc) return cudaErrorNotSupported;
-  cuuint64_t gd[4] = {static_cast<cuuint64_t>(D)}, gs[3];
-  cuuint32_t bx[4] = {64, 1, 1, 1}, es[4] = {1, 1, 1, 1};
+  cuuint64_t gd[5] = {static_cast<cuuint64_t>(D)}, gs[4];
+  cuuint32_t bx[5] = {64, 1, 1, 1, 1}, es[5] = {1, 1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) {
     gd[i + 1] = dims[i] > 0 ? dims[i] : 1;
     // a stride of 0 (one element, or the same place for all) is never stepped along
