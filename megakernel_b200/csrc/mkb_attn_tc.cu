@@ -124,6 +124,8 @@ struct TcArgs {
   int group_mul;        // r / group = r * group_mul >> 16 for r < 128
   int warp_tokens;      // tokens of a warp's 32 rows, 0 where they are not whole
   int box;              // keys of a TMA box
+  int folded;           // pages and KV heads are one dimension of the maps: see tc_launch
+  int kx[3], vx[3];     // ... and lie there at page * [0] + head * [1], outside at [2]
   int k_head, v_head;   // 0 where every KV head lies at the same place (stride 0), else 1
   unsigned tile_mul;    // x / tile_tokens is x * tile_mul >> 32, or one less (0: tile_tokens is 1)
   uint32_t* work;       // the next piece, CTAs that have finished; both zero between calls
@@ -162,13 +164,13 @@ __device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.w
 
 // Descriptor of an operand whose contiguous dimension is N, written by TMA with the
 // 128-byte swizzle: 64 values of N a row, eight rows (of K) to an atom of 1024 bytes;
-// `n_bytes` between 64-value blocks of N (leading offset), 1024 between atoms of K
+// `n_bytes` between 64-value blocks of N (leading offset), `k_bytes` between atoms of K
 // (stride offset).
-__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t n_bytes) {
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t n_bytes, uint32_t k_bytes) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((addr >> 4) & 0x3fffu);
   d |= static_cast<uint64_t>((n_bytes >> 4) & 0x3fffu) << 16;
-  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(k_bytes >> 4) << 32;
   d |= static_cast<uint64_t>(1u) << 46;
   d |= static_cast<uint64_t>(2u) << 61;
   return d;
@@ -574,7 +576,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (p.b < 0 || dead) break;
       // K(0), then K(j + 1) and V(j): the order in which the products take them
       const int n = p.total;
-      const int outside = max(a.pages, 1);  // (an empty pool's map has one page, that is never read)
       int pages = 0, pages_at = 0, pages_end = 0;  // the lanes' pages: boxes of keys up to pages_end
       auto load = [&](const CUtensorMap* map, int head, int j) {
         const int s = slot;
@@ -596,23 +597,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             pages_at = max(key - kKeys, 0);  // (V follows a tile behind K)
             pages_end = pages_at + 32 * box;
             const int at = pages_at + lane * box;
-            pages = outside;  // past the last key: outside the pool, which reads as zeros
+            pages = -2;  // past the last key: outside the pool, which reads as zeros
             if (at < p.len) {
               pages = __ldg(a.block_table + p.b * a.table_stride + (at >> 31 - __clz(a.page_size)));
               if (pages < 0 || pages >= a.pages) pages = -1;
             }
           }
-          int page = __shfl_sync(0xffffffffu, pages, ((key - pages_at >> box_log) + lane) & 31);
+          const int page = __shfl_sync(0xffffffffu, pages, ((key - pages_at >> box_log) + lane) & 31);
           if (lane * box < kKeys) {
-            if (page < 0) {
-              page = outside;
+            if (page == -1) {
               *reinterpret_cast<volatile int*>(&sm.piece[st].bad) = 1;
               report(a.status, MKB_SERVE_BAD_PAGE);
             }
+            const int at = (key + lane * box) & (a.page_size - 1);
+            if (g.folded) {
+              const int* x = map == &tk ? g.kx : g.vx;
+              tc::tma_load_5d(sm.kv[s] + lane * box * D * 2, map, 0, 0, 0, at >> 3, page < 0 ? x[2] : page * x[0] + p.hk * x[1],
+                              &sm.kv_full[s]);
+            } else {
 #pragma unroll
-            for (int d = 0; d < D / 64; ++d)
-              tc::tma_load_4d(sm.kv[s] + d * kHalf + lane * box * 128, map, 64 * d, (key + lane * box) & (a.page_size - 1),
-                              head, page, &sm.kv_full[s]);
+              for (int d = 0; d < D / 64; ++d)
+                tc::tma_load_4d(sm.kv[s] + d * kHalf + lane * box * 128, map, 64 * d, at, head,
+                                page < 0 ? max(a.pages, 1) : page, &sm.kv_full[s]);
+            }
           }
         } else if (lane == 0) {
 #pragma unroll
@@ -662,8 +669,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else if (warp == 8 || warp == 10) {
     // ---- the products of a tile -------------------------------------------------------------------
     constexpr uint32_t id_s = idesc16<T>(128, kKeys, false), id_o = idesc16<T>(128, D, true);
-    const uint64_t dq0 = tc::desc_sw128(smem_addr(sm.q[0])), dk0 = tc::desc_sw128(smem_addr(sm.kv[0]));
-    const uint64_t dv0 = desc_mn_sw128(smem_addr(sm.kv[0]), kHalf);
+    // K and V lie block of 64 values by block, all keys of a block one after another; where
+    // they are folded, eight keys by eight, and in each the blocks
+    const bool folded = kPaged && uniform(g.folded) != 0;
+    const int block = folded ? 1024 : kHalf, row = folded ? D * 2 : 128;  // bytes between blocks; of a key
+    const uint64_t dq0 = tc::desc_sw128(smem_addr(sm.q[0]));
+    const uint64_t dk0 = tc::desc_sw128(smem_addr(sm.kv[0])) + (static_cast<uint64_t>(8 * row - 1024 >> 4) << 32);
+    const uint64_t dv0 = desc_mn_sw128(smem_addr(sm.kv[0]), block, 8 * row);
     const uint32_t leader = elect_one();
     const int t = uniform((warp - 8) >> 1);
     const uint32_t ts = tbase + 128 * t, to_ = tbase + Shape::kO + D * t;
@@ -682,8 +694,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint64_t dk = tc::desc_advance(dk0, s * kTileBytes);
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t off = (kk >> 2) * kHalf + (kk & 3) * 32;
-        mma_ss(leader, ts, tc::desc_advance(dq, off), tc::desc_advance(dk, off), id_s, kk != 0);
+        mma_ss(leader, ts, tc::desc_advance(dq, (kk >> 2) * kHalf + (kk & 3) * 32),
+               tc::desc_advance(dk, (kk >> 2) * block + (kk & 3) * 32), id_s, kk != 0);
       }
       commit(leader, &sm.s_full[t]);  // covers O as well: S(j + 1) seen means PV(j) done
     };
@@ -732,7 +744,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int d = 0; d < D / 64; ++d)
               for (int c = lane; c < chunks; c += 32)
-                reinterpret_cast<uint4*>(sm.kv[slot] + d * kHalf + valid * 128)[c] = make_uint4(0, 0, 0, 0);
+                reinterpret_cast<uint4*>(sm.kv[slot] + (valid + c / 8 >> 3) * 8 * row + d * block + (valid + c / 8 & 7) * 128)[c % 8] =
+                    make_uint4(0, 0, 0, 0);
             fence_proxy_async_shared();
             __syncwarp();
           }
@@ -752,13 +765,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tc::fence_after_sync();
 #pragma unroll
           for (int kk = 0; kk < kFirstKeys / 16; ++kk)  // O (+)= P V
-            mma_ts(leader, to_, ts + 8 * kk, tc::desc_advance(dv, kk * 2048), id_o, (j - from | kk) != 0);
+            mma_ts(leader, to_, ts + 8 * kk, tc::desc_advance(dv, 16 * kk * row), id_o, (j - from | kk) != 0);
           wait_for(&sm.p_full[t], p_ph, &sm.err, dead);
           p_ph ^= 1;
           tc::fence_after_sync();
 #pragma unroll
           for (int kk = kFirstKeys / 16; kk < kKeys / 16; ++kk)
-            mma_ts(leader, to_, ts + 8 * kk, tc::desc_advance(dv, kk * 2048), id_o, 1u);
+            mma_ts(leader, to_, ts + 8 * kk, tc::desc_advance(dv, 16 * kk * row), id_o, 1u);
           if (j == last) commit(leader, &sm.o_full[t]);
           done += step;
         }
@@ -1202,7 +1215,50 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   const uint32_t kbox[3] = {static_cast<uint32_t>(g.box), 1, 1};
   const void *kb = a.k, *vb = a.v;
   if (kPaged && a.pages == 0) kb = vb = a.q;  // an empty pool is never read: any address will do
-  if (kPaged) {
+  // What a copy of a page's keys costs is the copy (80 cycles of the loading warp, and a tile has
+  // 128 / page_size of them), so one brings all blocks of 64 values: keys are groups of eight, a
+  // key of a group, blocks and groups three dimensions, laid down as the products' operands want
+  // them. That leaves one of a map's five for page and KV head, which are folded: where one of
+  // their strides is a multiple of the other. (28 requests decoding and two chunks, pages of 16:
+  // 64 us, 71 by a copy a block.)
+  g.folded = kPaged;
+  uint64_t fold_dim[2];
+  int64_t fold_stride[2];
+  for (int i = 0; i < 2 && kPaged; ++i) {
+    const int64_t *st = i ? a.v_stride : a.k_stride, ps = st[0], hs = a.kv_heads > 1 ? st[1] : 0;
+    int64_t page_x = 1, head_x = 0, unit = ps;
+    if (hs > 0 && a.pages <= 1) {
+      page_x = 0, head_x = 1, unit = hs;
+    } else if (hs > 0 && ps % hs == 0) {
+      page_x = ps / hs, head_x = 1, unit = hs;
+    } else if (hs > 0 && hs % ps == 0) {
+      head_x = hs / ps;
+    } else if (hs > 0) {
+      g.folded = 0;
+    }
+    const int64_t pages = a.pages > 0 ? a.pages : 1;
+    if (page_x > INT32_MAX / pages || head_x > INT32_MAX / a.kv_heads) {
+      g.folded = 0;
+      continue;
+    }
+    const int64_t end = (pages - 1) * page_x + (a.kv_heads - 1) * head_x + 1;
+    if (end > INT32_MAX) g.folded = 0;
+    int* const x = i ? g.vx : g.kx;
+    x[0] = static_cast<int>(page_x);
+    x[1] = static_cast<int>(head_x);
+    x[2] = static_cast<int>(end);
+    fold_dim[i] = static_cast<uint64_t>(end);
+    fold_stride[i] = unit;
+  }
+  if (kPaged && g.folded) {
+    const uint32_t box[4] = {8, D / 64, static_cast<uint32_t>(g.box / 8), 1};
+    for (int i = 0; i < 2; ++i) {
+      const int64_t slot = i ? a.v_stride[2] : a.k_stride[2];
+      const uint64_t dims[4] = {8, D / 64, static_cast<uint64_t>(a.page_size / 8), fold_dim[i]};
+      const int64_t strides[4] = {slot, 64, 8 * slot, fold_stride[i]};
+      if ((e = map_rows(i ? &mv : &mk, a.dtype, i ? vb : kb, 64, 4, dims, strides, box)) != cudaSuccess) return e;
+    }
+  } else if (kPaged) {
     const uint64_t dims[3] = {static_cast<uint64_t>(a.page_size), static_cast<uint64_t>(a.kv_heads),
                               static_cast<uint64_t>(a.pages)};
     const int64_t ks[3] = {a.k_stride[2], a.k_stride[1], a.k_stride[0]};

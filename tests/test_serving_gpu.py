@@ -217,6 +217,28 @@ def test_pages_and_layouts(page, layout):
     check(mk.paged_attention(q[last], c.kc, c.vc, c.table, c.lens), *c.want(q[last], [1] * 5), BF)
 
 
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 128), (6, 3, 64)])
+@pytest.mark.parametrize("gaps", [(0, 24), (40, 0), (8, 8)])
+def test_pages_and_heads_with_gaps(gaps, hq, hk, d, page):
+    """Page and KV head strides of which neither is a multiple of the other (or one is)."""
+    new, kv = [1, 90, 200, 1], [1, 333, 200, 700]
+    c = Cache(kv, hk, d, page, seed=page)
+    q = rand(seeded(12), sum(new), hq, d, scale=2.0)
+    want = c.want(q, new)
+    pool = c.kc.shape[0]
+    hs = page * d + gaps[0]
+    ps = hk * hs + gaps[1]
+    caches = []
+    for x in (c.kc, c.vc):
+        store = torch.full((pool * ps,), math.nan, dtype=BF, device=DEV)
+        caches.append(torch.as_strided(store, (pool, hk, page, d), (ps, hs, d, 1)))
+        caches[-1].copy_(x)
+    check(mk.paged_attention(q, *caches, c.table, c.lens, cu_of(new)), *want, BF)
+    one = [1] * 4
+    check(mk.paged_attention(q[:4], *caches, c.table, c.lens), *c.want(q[:4], one), BF)
+
+
 @pytest.mark.parametrize("kv", [[1], [5000], [1, 9000, 2], [257] * 70, [int(1.13 ** i) for i in range(2, 66)]])
 @pytest.mark.parametrize("hq,hk", [(16, 8), (2, 1), (5, 1)])
 def test_decode_lengths(kv, hq, hk):
