@@ -75,12 +75,9 @@ cudaError_t mkb_paged_attention(const mkb_attn_args* a, cudaStream_t stream) {
   using namespace mkb::sv;
   const cudaError_t e = check_attn(a, true);
   if (e != cudaSuccess || a->tokens == 0) return e;
-  // Up to 8 rows (new tokens x query heads of a KV head) known from the shapes alone: bytes
-  // bound the call, and the streaming kernel reads them fastest. More rows, or chunks of
-  // lengths that only the device knows: the tensor-core tiles. Streaming against tiles, heads
-  // 16 over 8 of 128: 48 requests of 1-4,096 keys, 2 rows 58 and 69 us, 8 rows 71 and 70 (16,
-  // with two columns of products: 100 and 71); three of 9,001-60,000 keys, 2 rows 78 and 99,
-  // 8 rows 90 and 93 (16: 112 and 93); one of 33 keys 7.5 and 9.2.
+  // Few rows known from the shapes alone: bytes bound the call, and the streaming kernel reads
+  // them fastest (both sides measured: decode_fits). More rows, or chunks of lengths that only
+  // the device knows: the tensor-core tiles.
   return decode_fits(*a) ? attn_decode(*a, stream) : attn_tc(*a, true, stream);
 }
 }

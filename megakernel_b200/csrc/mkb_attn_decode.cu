@@ -662,9 +662,19 @@ static cudaError_t decode_launch(const mkb_attn_args& a, cudaStream_t stream) {
   return launch_early(attn_decode_kernel<T, D>, grid, 32 * kDecWarps, bytes, stream, mk, mv, g);
 }
 
-// Few enough rows a KV head for one tile of columns.
+// Rows (new tokens x query heads of a KV head) known from the shapes alone, and few: up to 4;
+// up to 8 where there are few requests and KV heads, whose keys have to be shared out over the
+// SMs. This kernel against the tensor-core tiles, heads 16 over 8 of 128 unless named:
+//   2 rows: 48 requests of 1-4,096 keys 58 and 66 us, 9,001-60,000 keys 78 and 95, 33 keys 7.3 and 9.2
+//   8 rows: 48 requests 71 and 66, four of 300-1,000 keys 25 and 17 (heads 16 over 2: 36 and 32 for
+//           the 48); 9,001-60,000 keys 89 and 90, one of 33 keys 8.6 and 9.3, heads 16 over 2 and
+//           500-30,000 keys 42 and 54
+//   16 rows, by two columns of products: 48 requests 100 and 71
 bool decode_fits(const mkb_attn_args& a) {
-  return a.cu_q == nullptr && static_cast<int64_t>(a.q_len) * (a.heads / a.kv_heads) <= kDecRows;
+  if (a.cu_q != nullptr) return false;
+  const int64_t rows = static_cast<int64_t>(a.q_len) * (a.heads / a.kv_heads);
+  const int64_t most = static_cast<int64_t>(a.batch) * a.kv_heads * 6 <= sm_count() ? kDecRows : kDecRows / 2;
+  return rows <= most;
 }
 
 template <typename T>

@@ -71,8 +71,8 @@ constexpr int kMinSplit = 6;
 // Key tiles still to load when a CTA asks for its next piece: 12 prompts of 1-1,411 tokens take
 // 35.4 us, with 8 37.3 (pieces are taken too long before their turn).
 constexpr int kAskTiles = 3;
-// Requests up to which pieces are taken longest first: 28 decoding and two chunks 71.6 us, as
-// they come 76.4; 200 prompts of 30-930 tokens 516 us, as they come 463.
+// Requests up to which pieces are taken longest first: 28 decoding and two chunks 62.3 us, as
+// they come 68.2; 200 prompts of 30-930 tokens 516 us, as they come 463.
 constexpr int kSortBatch = 128;
 constexpr int kTryNs = 20000, kTries = 50000;  // bound of every wait: about a second
 
@@ -1227,7 +1227,7 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   // key of a group, blocks and groups three dimensions, laid down as the products' operands want
   // them. That leaves one of a map's five for page and KV head, which are folded: where one of
   // their strides is a multiple of the other. (28 requests decoding and two chunks, pages of 16:
-  // 64 us, 71 by a copy a block.)
+  // 62.3 us, 73.5 by a copy a block; four chunks of 512, pages of 32: 44.5, 47.8.)
   g.folded = kPaged;
   uint64_t fold_dim[2];
   int64_t fold_stride[2];
