@@ -40,7 +40,7 @@ constexpr int kDecWarps = 8;
 constexpr int kDecRows = 8;      // rows of a KV head: the columns of one mma
 constexpr int kTileKeys = 16;    // keys of a tile: the rows of one mma
 // A CTA for every request and KV head, unless those have more than kLongTiles tiles on
-// average: then one for every kCtaTiles, as far as there are SMs. (8 requests of 700 keys: 13.0
+// average: then one for every kCtaTiles, as far as there are SMs. (8 requests of 700 keys: 12.4
 // us, spread out further 17.6, the sums over CTAs cost more than the keys; one of 4,000: 18.7
 // spread out, 40.7 not. With 64 tiles a CTA that one takes 23.7; with 4, 18.8, and one of 900
 // keys 17.2 instead of 16.0.)
@@ -666,7 +666,7 @@ static cudaError_t decode_launch(const mkb_attn_args& a, cudaStream_t stream) {
 // up to 8 where there are few requests and KV heads, whose keys have to be shared out over the
 // SMs. This kernel against the tensor-core tiles, heads 16 over 8 of 128 unless named:
 //   2 rows: 48 requests of 1-4,096 keys 58 and 66 us, 9,001-60,000 keys 78 and 95, 33 keys 7.3 and 9.2
-//   8 rows: 48 requests 71 and 66, four of 300-1,000 keys 25 and 17 (heads 16 over 2: 36 and 32 for
+//   8 rows: 48 requests 71 and 66, four of 300-1,000 keys 26 and 17 (heads 16 over 2: 36 and 32 for
 //           the 48); 9,001-60,000 keys 89 and 90, one of 33 keys 8.6 and 9.3, heads 16 over 2 and
 //           500-30,000 keys 42 and 54
 //   16 rows, by two columns of products: 48 requests 100 and 71
