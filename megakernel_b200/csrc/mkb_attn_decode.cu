@@ -333,14 +333,16 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
         stage = 0;
         phase ^= 1;
       }
-      float s[4] = {};
+      float s[4] = {}, s1[4] = {};  // (two sums: half the chain)
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {  // A: keys by dims
         uint32_t ka[4];
         const int r = lane % 16, x = 2 * (kk % 4) + lane / 16;
         ldsm4(kt + kk / 4 * kHalf + r * 128 + ((x ^ (r & 7)) << 4), ka);
-        mma16816<T>(s, ka, qf[kk][0], qf[kk][1]);
+        mma16816<T>(kk & 1 ? s1 : s, ka, qf[kk][0], qf[kk][1]);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += s1[e];
       // s[e], s[2 + e]: keys lane / 4 and lane / 4 + 8, row 2 (lane % 4) + e
       if (bad_pages >> bad_bit & 1u) {  // a page outside the pool: its keys are NaN
 #pragma unroll
@@ -488,12 +490,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   float(*const sum_l)[kDecRows] = sum_m + kParts;
   static_assert((D + 3 * kParts) * kDecRows * 4 <= kRing * kBytes, "room of the first warp's ring");
   const int64_t my_pos = lane < kParts ? part_pos[lane / 2][lane % 2] : -1;
-  uint32_t same = 0;  // the parts that go with the lane's
-#pragma unroll
-  for (int j = 0; j < kParts; ++j) {
-    const int64_t x = __shfl_sync(0xffffffffu, my_pos, j);
-    if (my_pos >= 0 && x == my_pos) same |= 1u << j;
-  }
+  // the parts that go with the lane's
+  const uint32_t same = __match_any_sync(0xffffffffu, static_cast<unsigned long long>(my_pos)) & (my_pos >= 0 ? ~0u : 0u);
   const uint32_t firsts = __ballot_sync(0xffffffffu, my_pos >= 0 && (same & ((1u << lane) - 1)) == 0);
   if (firsts == 0) return;  // (the same for every warp)
   for (int r = warp; r < g.rows; r += kDecWarps) {
