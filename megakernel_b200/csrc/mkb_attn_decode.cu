@@ -103,25 +103,6 @@ __device__ __forceinline__ void mma16816(float c[4], const uint32_t a[4], uint32
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Whether one of these eight values is not finite: 0 * x + n is NaN then.
-template <typename T>
-__device__ __forceinline__ uint32_t odd8(const uint4& u, uint32_t n) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (Pair<T>::kDtype == MKB_BF16)
-      asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(n) : "r"(w[i]), "r"(0u));
-    else
-      asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(n) : "r"(w[i]), "r"(0u));
-  }
-  return n;
-}
-template <typename T>
-__device__ __forceinline__ bool finite(uint16_t v) {
-  constexpr uint32_t kExp = Pair<T>::kDtype == MKB_BF16 ? 0x7f80u : 0x7c00u;
-  return (v & kExp) != kExp;
-}
-
 // Tiles of a request (one for a request without keys: its zeros have to be written).
 __device__ __forceinline__ int dec_tiles(const DecArgs& g, int b, int* len_out, bool* bad_out) {
   const int len = max(__ldg(g.a.kv_lens + b), 0);

@@ -44,9 +44,15 @@
 // keys, so results do not depend on timing. Nothing is asked of the host.
 //
 // Masked places: scores are replaced, not added to. V rows past the request's last key
-// are cleared in shared memory. V that is not finite and stands where some row of the
-// tile does not look reaches that row as 0 * inf = NaN: a row whose O is not finite is
-// computed again key by key, over the keys it sees.
+// are cleared in shared memory. V that is not finite and stands where some row does not
+// look would reach that row as 0 * inf = NaN. That can happen only in the key tiles that the
+// piece's first row does not see in full (its last three at most): the warp that issues the
+// product looks those over while it waits for P, and where it finds such a value clears it;
+// the softmax warps then add it to the rows that see it, as it is. What every row of the
+// piece sees goes through the product: a weight that rounds to 0 makes NaN of an infinity.
+// (Looking over takes instructions from the softmax warps: 12 prompts of 1-1,411 tokens 36.3 us,
+// 34.7 without; 2,049, 1,000 and 4,097 tokens of 64-wide FP16 118.8, 117.1; two of 4,096 125.3,
+// 123.0. 15,999 tokens 802 us; with NaN in all of the first key 834, all of V infinite 1,381.)
 
 #include <cmath>
 #include <cuda.h>
@@ -76,6 +82,9 @@ constexpr int kAskTiles = 3;
 constexpr int kSortBatch = 128;
 constexpr int kTryNs = 20000, kTries = 50000;  // bound of every wait: about a second
 
+// A page or length is wrong; values of V that are not finite were cleared in the piece's tiles.
+constexpr int kBad = 1, kOdd = 2;
+
 struct Piece {
   int b;            // request, -1: no more work
   int hk;
@@ -86,7 +95,7 @@ struct Piece {
   int n[2];         // those of tiles A and B
   int halves;       // A and B have the same rows, and every other key tile
   int splits, split, slot;  // ranges of the rows' keys, which this is, where the first leaves its results
-  int bad;
+  int flags;        // of kBad, kOdd
 };
 
 template <int D>
@@ -285,12 +294,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // ---- the list of pieces, worked out by one warp -------------------------------------
 
 // One request as the list sees it.
@@ -545,7 +548,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           p.splits = sp;
           p.split = split;
           p.slot = slot_base + sinc - slots + (i * kv_heads + hk) * sp;
-          p.bad = l.bad;
+          p.flags = l.bad ? kBad : 0;
           if (l.bad) report(a.status, MKB_SERVE_BAD_LENGTH);
         }
         if (__any_sync(0xffffffffu, is_it)) break;
@@ -606,7 +609,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int page = __shfl_sync(0xffffffffu, pages, ((key - pages_at >> box_log) + lane) & 31);
           if (lane * box < kKeys) {
             if (page == -1) {
-              *reinterpret_cast<volatile int*>(&sm.piece[st].bad) = 1;
+              atomicOr(&sm.piece[st].flags, kBad);
               report(a.status, MKB_SERVE_BAD_PAGE);
             }
             const int at = (key + lane * box) & (a.page_size - 1);
@@ -708,6 +711,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int step = uniform(sm.piece[st].halves) ? 2 : 1, from = step == 2 ? t : 0;  // its key tiles
       const int last = from + step * (mine_n - 1);                                     // (below `from`: none)
       const int left = uniform(sm.piece[st].len) - uniform(sm.piece[st].k0) * kKeys;  // keys from the first tile on
+      // the first tile of keys that the piece's first row does not see in full
+      const int sees = uniform(sm.piece[st].ctx) + uniform(sm.piece[st].tok0) + 1;
+      const int look = sees < uniform(sm.piece[st].len) ? max(sees / kKeys, 0) - uniform(sm.piece[st].k0) : 0x7fffffff;
       const bool stop = uniform(sm.piece[st].b) < 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.info_empty[st]);
@@ -753,6 +759,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               for (int c = lane; c < chunks; c += 32)
                 reinterpret_cast<uint4*>(sm.kv[slot] + (valid + c / 8 >> 3) * 8 * row + d * block + (valid + c / 8 & 7) * 128)[c % 8] =
                     make_uint4(0, 0, 0, 0);
+            fence_proxy_async_shared();
+            __syncwarp();
+          }
+          if (__builtin_expect(j >= look, 0)) {  // V that is not finite (both warps, side by side, to the same end)
+            uint8_t* const v = sm.kv[slot];
+            const int groups = (min(valid, kKeys) + 7) / 8;  // of eight keys
+            uint32_t x[D / 32] = {}, any = 0;
+#pragma unroll 2
+            for (int i = 0; i < groups; ++i) {
+#pragma unroll
+              for (int d = 0; d < D / 32; ++d)
+                x[d] = odd8<T>(reinterpret_cast<const uint4*>(v + 8 * row * i + block * (d / 2))[32 * (d % 2) + lane], x[d]);
+            }
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) any |= x[d];
+            if (__builtin_expect(__any_sync(0xffffffffu, any != 0), 0)) {
+              if (lane == 0) atomicOr(&sm.piece[st].flags, kOdd);
+              __threadfence_block();
+              __syncwarp();
+#pragma unroll 1
+              for (int i = lane; i < kTileBytes / 2; i += 32) {
+                uint16_t* const y = reinterpret_cast<uint16_t*>(v) + i;
+                if (!finite<T>(*y)) *y = 0;
+              }
+            }
             fence_proxy_async_shared();
             __syncwarp();
           }
@@ -932,16 +963,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         l = l * own + x.y * other;
         m = mm;
       }
-      const bool bad = *reinterpret_cast<volatile int*>(&sm.piece[st].bad) != 0;
+      const int flags = *reinterpret_cast<volatile int*>(&sm.piece[st].flags);
+      const bool bad = (flags & kBad) != 0, odd = (flags & kOdd) != 0;
       release();
       const int k_end = min(p.len, (p.k0 + p.total) * kKeys);
       constexpr int kPer = D / 32;
       uint8_t* stage = sm.stage[warp];
       // Rows on their way out, 32 values at a time (a small loop: this code is not in the
       // instruction cache when a piece ends): 64 values of all 32 rows of the warp by a TMA
-      // store where they are whole tokens of the request, else a thread its own row
+      // store where they are whole tokens of the request (and final), else a thread its own row
       const int tok_w = tok_t + g.warp_tokens * (warp & 3);
-      const bool whole = g.warp_tokens > 0 && tok_w + g.warp_tokens <= p.tok0 + p.toks;
+      const bool whole = g.warp_tokens > 0 && tok_w + g.warp_tokens <= p.tok0 + p.toks && !odd;
       auto emit = [&](int c, const uint32_t* w) {  // values 32 c .. + 31 of every row, packed
         if (!whole) {
           if (live) {
@@ -971,7 +1003,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       auto slot_of = [&](int s) { return static_cast<size_t>(p.slot + s); };
       const size_t slot = slot_of(p.split);
       float4* part = g.part + slot * (D / 4) * kRows;
-      uint64_t odd2 = 0;  // NaN once a value of O is not finite
       // no weights at all (every score -inf) are no mean; a row that sees no key is zero
       const bool zero = lim < 0 && !bad, zeros = __any_sync(0xffffffffu, zero);
       const float inv = bad || m == -INFINITY ? NAN : 1.f / l;
@@ -1000,8 +1031,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int i = 0; i < 16; ++i)
             o2[i] = fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), other2, fma2(o2[i], own2, 0));
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) odd2 = fma2(o2[i], 0, odd2);
         if (split) {  // one of several ranges of keys: left for whoever comes last
           if (live) {
 #pragma unroll
@@ -1023,41 +1052,38 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           emit(c, x);
         }
       }
-      const float2 oddf = unpack2(odd2);
-      const float odd = oddf.x + oddf.y;
       if (pair) {
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.pair_empty);
       }
       if (split && live) g.stat[slot * kRows + at] = make_float2(m, bad ? NAN : l);
-      // the rows of the warp whose O is not finite, key by key
-      uint32_t todo = __ballot_sync(0xffffffffu, odd != 0.f && live && lim >= 0 && !bad);
-      if (todo != 0) {
-        if (lane == 0) tma_store_done();
-        __syncwarp();
-      }
+      // the values of V that were cleared, to the warp's rows that see them
+      __syncwarp();
+      if (odd && !bad) {
+        int key = max(p.k0 * kKeys, max(p.ctx + p.tok0 + 1, 0) / kKeys * kKeys);
+        float z[kPer] = {};  // (rows come in the order of their tokens: each sees what the one before saw)
 #pragma unroll 1
-      while (todo != 0) {
-        const int r = __ffs(todo) - 1, rt = 32 * (warp & 3) + r, tok = rt * g.group_mul >> 16;
-        const int head = p.hk * g.group + rt - tok * g.group;
-        todo &= todo - 1;
-        float o[kPer], ms, ls;
-        row_by_key<T, D, kPaged>(a, g.sl2, p.b, p.first, p.first + tok_t + tok, head, p.hk, p.k0 * kKeys,
-                                 min(k_end, p.ctx + tok_t + tok + 1), o, &ms, &ls);
-        if (split) {
+        for (int r = 0; r < 32; ++r) {
+          const int rt = 32 * (warp & 3) + r, tok = rt * g.group_mul >> 16;
+          if (rt >= g.tile_tokens * g.group || tok_t + tok >= p.tok0 + p.toks) break;
+          const int end = min(k_end, p.ctx + tok_t + tok + 1);
+          if (key < end) {
+            sum_odd<T, D, kPaged>(a, p.b, p.first, p.hk, key, end, z);
+            key = end;
+          }
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
             const int d = lane * kPer + i;
-            reinterpret_cast<float*>(part + (d / 4) * kRows + 128 * t + rt)[d % 4] = o[i];
+            if (z[i] == 0.f) continue;
+            if (split) {
+              reinterpret_cast<float*>(part + (d / 4) * kRows + 128 * t + rt)[d % 4] += z[i];
+            } else {
+              T* const o = static_cast<T*>(a.out) + (p.first + tok_t + tok) * a.out_stride[0] +
+                           (p.hk * g.group + rt - tok * g.group) * a.out_stride[1] + d;
+              *o = static_cast<T>(static_cast<float>(*o) + z[i]);
+            }
           }
-          if (lane == 0) g.stat[slot * kRows + 128 * t + rt] = make_float2(ms, ls);
-        } else {
-          uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (p.first + tok_t + tok) * a.out_stride[0] +
-                                                      head * a.out_stride[1]) + lane * (kPer / 2);
-          const float f = 1.f / ls;
-#pragma unroll
-          for (int i = 0; i < kPer / 2; ++i) dst[i] = Pair<T>::put(o[2 * i] * f, o[2 * i + 1] * f);
         }
       }
       __syncwarp();

@@ -91,58 +91,52 @@ __device__ __forceinline__ Request request_at(const int* __restrict__ cu, int ba
   return request_rows(cu, cu == nullptr ? t / q_len : request_of(cu, batch, t), q_len, tokens);
 }
 
-// One row, key by key: what a row comes to where a product over a whole tile would bring
-// in values that are not finite from places the row does not see (0 * inf). Warp-wide;
-// keys [begin, end) of request b; the lane holds dims [lane * D / 32, + D / 32) of O,
-// relative to maximum m (in units of log2; sl2 = scale * log2(e)).
-template <typename T, int D, bool kPaged>
-__device__ __noinline__ void row_by_key(const mkb_attn_args& a, float sl2, int b, int first, int token, int h, int hk,
-                                        int begin, int end, float* o, float* m_out, float* l_out) {
-  const int lane = threadIdx.x & 31;
-  constexpr int kPer = D / 32;
-  const T* q = static_cast<const T*>(a.q) + token * a.q_stride[0] + h * a.q_stride[1];
-  float m = -INFINITY, l = 0.f;
+// ---- V that is not finite -------------------------------------------------------------
+// A product over a whole tile would bring it into rows that do not see it (0 * inf = NaN),
+// so it is cleared there and added to the rows that do.
+
+// Whether one of these eight values is not finite: 0 * x + n is NaN then.
+template <typename T>
+__device__ __forceinline__ uint32_t odd8(const uint4& u, uint32_t n) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-  for (int j = begin; j < end; ++j) {
-    int64_t ko, vo;
-    if (kPaged) {
-      const int64_t page = a.block_table[b * a.table_stride + j / a.page_size], slot = j % a.page_size;
-      if (page < 0 || page >= a.pages) {  // reported already
-        l = NAN;
-        continue;
-      }
-      ko = page * a.k_stride[0] + hk * a.k_stride[1] + slot * a.k_stride[2];
-      vo = page * a.v_stride[0] + hk * a.v_stride[1] + slot * a.v_stride[2];
-    } else {
-      ko = static_cast<int64_t>(first + j) * a.k_stride[0] + hk * a.k_stride[1];
-      vo = static_cast<int64_t>(first + j) * a.v_stride[0] + hk * a.v_stride[1];
-    }
-    const uint32_t* k2 = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.k) + ko);
-    const uint32_t* v2 = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.v) + vo);
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPer / 2; ++i) {
-      const float2 x = Pair<T>::get(reinterpret_cast<const uint32_t*>(q)[lane * (kPer / 2) + i]);
-      const float2 y = Pair<T>::get(k2[lane * (kPer / 2) + i]);
-      s += x.x * y.x + x.y * y.y;
-    }
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= sl2;
-    const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
-    const float sc = ex2_approx(m - ref), w = ex2_approx(s - ref);
-    l = l * sc + w;
-#pragma unroll
-    for (int i = 0; i < kPer / 2; ++i) {
-      const float2 y = Pair<T>::get(v2[lane * (kPer / 2) + i]);
-      o[2 * i] = o[2 * i] * sc + w * y.x;
-      o[2 * i + 1] = o[2 * i + 1] * sc + w * y.y;
-    }
-    m = mn;
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (Pair<T>::kDtype == MKB_BF16)
+      asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(n) : "r"(w[i]), "r"(0u));
+    else
+      asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(n) : "r"(w[i]), "r"(0u));
   }
-  *m_out = m;
-  *l_out = l;
+  return n;
+}
+template <typename T>
+__device__ __forceinline__ bool finite(uint16_t v) {
+  constexpr uint32_t kExp = Pair<T>::kDtype == MKB_BF16 ? 0x7f80u : 0x7c00u;
+  return (v & kExp) != kExp;
+}
+
+// Adds to z what of V's values at keys [begin, end) of request b is not finite. Warp-wide;
+// the lane holds dims [lane * D / 32, + D / 32).
+template <typename T, int D, bool kPaged>
+__device__ __noinline__ void sum_odd(const mkb_attn_args& a, int b, int first, int hk, int begin, int end, float* z) {
+  constexpr int kPer = D / 32;
+  const int lane = threadIdx.x & 31;
+#pragma unroll 4
+  for (int j = begin; j < end; ++j) {
+    int64_t vo = static_cast<int64_t>(first + j) * a.v_stride[0];
+    if (kPaged) {
+      const int64_t page = a.block_table[b * a.table_stride + j / a.page_size];
+      if (page < 0 || page >= a.pages) continue;  // (reported by the loads)
+      vo = page * a.v_stride[0] + j % a.page_size * a.v_stride[2];
+    }
+    const uint32_t* v = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.v) + vo + hk * a.v_stride[1]);
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i) {
+      const uint32_t u = v[lane * (kPer / 2) + i];
+      const float2 f = Pair<T>::get(u);
+      if (!finite<T>(u & 0xffffu)) z[2 * i] += f.x;
+      if (!finite<T>(u >> 16)) z[2 * i + 1] += f.y;
+    }
+  }
 }
 
 // ---- early launch ----------------------------------------------------------------------

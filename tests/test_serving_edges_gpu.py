@@ -95,3 +95,97 @@ def test_decode_of_several_tokens_with_values_that_some_do_not_see(n):
     q = rand(seeded(22), len(kv), n, 16, 128)
     got = mk.paged_attention(q, c.kc, c.vc, c.table, c.lens)
     check_any(got.flatten(0, 1), *want_of(c, q.flatten(0, 1), [n] * len(kv)), BF)
+
+
+def spoil(v, at):
+    """Values at (key, head, dim) of v, in place."""
+    for key, head, dim, value in at:
+        v[key, head, dim] = value
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("hq,hk,d", [(16, 8, 128), (8, 8, 64), (6, 2, 128), (16, 1, 64), (128, 1, 128)])
+@pytest.mark.parametrize("lens", [[300, 1, 70], [1000, 255, 130], [2, 3, 129, 64]])
+def test_prompts_with_values_that_some_rows_do_not_see(lens, hq, hk, d, dtype):
+    """At the first and last key, at both sides of a tile's border, of both signs in a column."""
+    q, k, v = prompts(lens, hq, hk, d, dtype, seed=len(lens), spread=0.25)
+    at = 0
+    for n in lens:
+        keys = sorted({0, 1, 63, 64, 127, 128, 200, n // 2, n - 2, n - 1} & set(range(n)))
+        spoil(v[at:at + n], [(j, i % hk, (7 * i) % d, (INF, -INF, NAN)[i % 3]) for i, j in enumerate(keys)])
+        spoil(v[at:at + n], [(n // 3, 0, 1, INF), (2 * n // 3, 0, 1, -INF)])
+        at += n
+    got = mk.prompt_attention(q, k, v, cu_of(lens))
+    want, at = [], 0
+    for n in lens:
+        want.append(attend_any(q[at:at + n], k[at:at + n], v[at:at + n]))
+        at += n
+    check_any(got, torch.cat([a for a, _ in want]), torch.cat([b for _, b in want]), dtype)
+
+
+@pytest.mark.parametrize("hq,hk,d,page", [(16, 8, 128, 16), (4, 2, 64, 32), (14, 2, 128, 128)])
+@pytest.mark.parametrize("new,kv", [([70, 1, 5], [200, 64, 5]), ([130], [9000]), ([300, 40], [4000, 12000]),
+                                    ([1, 2], [20000, 30]), ([20, 9], [7, 0])])
+def test_chunks_with_values_that_some_rows_do_not_see(new, kv, hq, hk, d, page):
+    """Over pages: whole rows, rows whose keys are split, and tokens that stand before position 0."""
+    c = Cache(kv, hk, d, page, seed=len(new))
+    for b, m in enumerate(kv):
+        for i, j in enumerate(sorted({0, m // 2, m - 1, m - 2, m - 5, m - 69, m - 130} & set(range(m)))):
+            plant(c, b, j, i % hk, (5 * i) % d, (INF, -INF, NAN)[i % 3])
+            plant(c, b, j, 0, d - 1, (INF, -INF)[i % 2])
+    q = rand(seeded(23), sum(new), hq, d, scale=0.25)
+    got = mk.paged_attention(q, c.kc, c.vc, c.table, c.lens, cu_of(new))
+    want, at = [], 0
+    for b, n in enumerate(new):
+        m, blind = kv[b], max(0, n - kv[b])
+        zero = torch.zeros((blind, hq, d), dtype=torch.float64, device=DEV)
+        o, size = attend_any(q[at + blind:at + n], c.k[b], c.v[b]) if m else (zero[:0], zero[:0])
+        want += [(zero, zero), (o, size)]
+        at += n
+    check_any(got, torch.cat([a for a, _ in want]), torch.cat([b for _, b in want]), BF)
+
+
+def elapsed(call, n=3):
+    call()
+    best = INF
+    for _ in range(n):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        call()
+        end.record()
+        end.synchronize()
+        best = min(best, start.elapsed_time(end))
+    return best
+
+
+def test_values_that_are_not_finite_cost_little():
+    """A NaN that every row sees is no reason to look at any row again; one that only some see
+    takes a look at the few keys they differ in. A pass over all keys of every row, key by key,
+    takes a hundred times as long."""
+    n = 4000
+    q, k, v = prompts([n], 16, 8, 128, seed=5, spread=0.25)
+    cu = cu_of([n])
+    clean = elapsed(lambda: mk.prompt_attention(q, k, v, cu))
+    v[0] = NAN
+    got = mk.prompt_attention(q, k, v, cu)
+    assert got.isnan().all()
+    assert elapsed(lambda: mk.prompt_attention(q, k, v, cu)) < 4 * clean
+    v[:] = INF
+    assert (mk.prompt_attention(q, k, v, cu) == INF).all()
+    assert elapsed(lambda: mk.prompt_attention(q, k, v, cu)) < 20 * clean
+    assert mk.serving_status() == (0, "ok")
+
+
+@pytest.mark.parametrize("new,kv", [([1, 1, 1], [300, 5000, 40]), ([90, 1, 700], [300, 5000, 700])])
+def test_output_in_place_of_q(new, kv):
+    """Every row of q is read before its row of the output is written, whatever V holds."""
+    c = Cache(kv, 2, 128, 16, seed=9)
+    plant(c, 0, kv[0] - 1, 0, 3, INF)
+    plant(c, 2, kv[2] // 2, 1, 4, NAN)
+    q = rand(seeded(24), sum(new), 16, 128, scale=0.25)
+    cu = cu_of(new) if max(new) > 1 else None
+    want = mk.paged_attention(q, c.kc, c.vc, c.table, c.lens, cu)
+    check_any(want, *want_of(c, q, new), BF)
+    got = mk.paged_attention(q, c.kc, c.vc, c.table, c.lens, cu, out=q)
+    assert got.data_ptr() == q.data_ptr()
+    assert torch.equal(got.nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
