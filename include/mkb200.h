@@ -387,6 +387,12 @@ cudaError_t mkb_paged_append(const mkb_append_args* a, cudaStream_t stream);
  * device (head_dim alone is read); 0 where there is no such call. */
 size_t mkb_attn_workspace_bytes(const mkb_attn_args* a);
 cudaError_t mkb_attn_workspace_reset(void* workspace, size_t bytes, cudaStream_t stream);
+/* Every wait inside the attention kernels is bounded (1 s at most). Where one expires the
+ * call ends with MKB_SERVE_TIMEOUT in *status: each of its rows is right or NaN, and the
+ * workspace is ready for the next call. Testing: in the calls that follow, CTA `cta` (-2:
+ * every one, -1: none) loads the first `from` pieces of its work and no more, so that its
+ * waits expire. */
+void mkb_attn_withhold(int cta, int from);
 
 /* ---- schedule introspection (host only, no GPU needed) ------------------------ */
 /* out[0..13] = qa, qb, in_bc, h, c, oa, ob, ja, jb, da, db, va, vb, group_size. */

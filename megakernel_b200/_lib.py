@@ -182,6 +182,7 @@ SIGNATURES = [
     ("mkb_paged_append", c_int, [POINTER(AppendArgs), c_void_p]),
     ("mkb_attn_workspace_bytes", c_size_t, [POINTER(AttnArgs)]),
     ("mkb_attn_workspace_reset", c_int, [c_void_p, c_size_t, c_void_p]),
+    ("mkb_attn_withhold", None, [c_int, c_int]),
     ("mkb_plan_query", c_int, [c_int, c_int, POINTER(c_int32)]),
     ("mkb_plan_query_tp", c_int, [c_int, c_int, c_int, c_int, POINTER(c_int32)]),
     ("mkb_qkv_global_row", c_int, [c_int, c_int, c_int]),

@@ -1,5 +1,6 @@
 // The attention entry points: what they refuse, and which kernel runs.
 
+#include <atomic>
 #include <cmath>
 
 #include "mkb_serving.cuh"
@@ -12,6 +13,9 @@ size_t tc_workspace(const mkb_attn_args& a);
 cudaError_t attn_decode(const mkb_attn_args& a, cudaStream_t stream);  // mkb_attn_decode.cu
 size_t decode_workspace(const mkb_attn_args& a);
 bool decode_fits(const mkb_attn_args& a);
+
+static std::atomic<Withheld> g_withheld{Withheld{-1, 0}};
+Withheld withheld() { return g_withheld.load(std::memory_order_relaxed); }
 
 // What both entry points refuse before a launch.
 static cudaError_t check_attn(const mkb_attn_args* a, bool paged) {
@@ -63,6 +67,8 @@ size_t mkb_attn_workspace_bytes(const mkb_attn_args* a) {
 cudaError_t mkb_attn_workspace_reset(void* workspace, size_t bytes, cudaStream_t stream) {
   return cudaMemsetAsync(workspace, 0, bytes, stream);
 }
+
+void mkb_attn_withhold(int cta, int from) { mkb::sv::g_withheld.store({cta, from}); }
 
 cudaError_t mkb_prompt_attention(const mkb_attn_args* a, cudaStream_t stream) {
   using namespace mkb::sv;

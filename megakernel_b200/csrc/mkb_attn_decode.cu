@@ -54,7 +54,7 @@ constexpr int kLongTiles = 64;
 // are cut anywhere; 48 of 1-4,096 keys: 58.1, 58.8 cut anywhere, 59.8 with 32 tiles. One of 33
 // keys: 7.4, 8.1 in one warp.)
 constexpr int kWholeTiles = 8;
-constexpr int kDecTryNs = 20000, kDecTries = 50000;  // bound of a wait: about a second
+constexpr int kDecTryNs = 20000, kDecTries = 50000;  // bound of a wait: a second at most (0.2 s)
 
 struct DecArgs {
   mkb_attn_args a;
@@ -65,6 +65,7 @@ struct DecArgs {
   uint32_t* counters;  // [ctas], zero between calls
   float* part;         // [2 ctas][D][cols] O^T, the maxima and sums in stat [2 ctas][2][kDecRows]
   float* stat;
+  Withheld withheld;   // testing: a CTA that loads nothing
 };
 
 template <int D>
@@ -238,7 +239,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   enter(ahead);
   Cursor cur = ahead;
 
-  bool dead = false;             // a wait has expired: nothing is loaded or waited for any more
+  bool dead = false;             // a wait has expired: nothing is waited for any more
+  bool stop = g.withheld.here(); // ... nor loaded
   int fill = 0;                  // the ring's next stage to load
   int pages = 0, pages_at = -1;  // the lanes' pages of tiles pages_at .. + 31 of request pages_b
   int pages_b = -1;
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   int load_bit = 0, bad_bit = 0;
   auto load = [&]() {
     while (open(ahead) && ahead.t >= ahead.t_end) leave(ahead);
-    if (dead || !open(ahead)) return;
+    if (stop || !open(ahead)) return;
     bool oob = false;
     if (!ahead.bad && ahead.len > 0) {
       if (pages_b != ahead.b || ahead.t < pages_at || ahead.t >= pages_at + 32) {
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
         for (int i = 0; !__all_sync(0xffffffffu, mbar_wait(&full[warp][stage], phase, kDecTryNs)); ++i)
           if (i > kDecTries) {
             err = 1;
-            dead = true;
+            dead = stop = true;
             break;
           }
       const uint32_t kt = ring + stage * kBytes, vt = kt + kBytes / 2;
@@ -628,6 +630,7 @@ static cudaError_t decode_launch(const mkb_attn_args& a, cudaStream_t stream) {
   g.v_head = a.v_stride[1] != 0;
   g.group = a.heads / a.kv_heads;
   g.rows = a.q_len * g.group;
+  g.withheld = withheld();
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   if (ws == nullptr) return cudaErrorInvalidValue;
   g.counters = reinterpret_cast<uint32_t*>(ws);

@@ -80,7 +80,7 @@ constexpr int kAskTiles = 3;
 // Requests up to which pieces are taken longest first: 28 decoding and two chunks 62.3 us, as
 // they come 68.2; 200 prompts of 30-930 tokens 516 us, as they come 463.
 constexpr int kSortBatch = 128;
-constexpr int kTryNs = 20000, kTries = 50000;  // bound of every wait: about a second
+constexpr int kTryNs = 20000, kTries = 50000;  // bound of every wait: a second at most (tries end sooner: 0.2 s)
 
 // A page or length is wrong; values of V that are not finite were cleared in the piece's tiles.
 constexpr int kBad = 1, kOdd = 2;
@@ -119,8 +119,12 @@ struct TcSmem {
   uint64_t pair_full, pair_empty;
   float2 pair[128];       // maximum and sum of B's rows, where they are A's too
   Piece piece[2];
+  Piece lost;             // taken off the list after a stop
   uint32_t tmem_base;
   int err;
+  int handed, open, pending;  // pieces given out; after a stop: the list goes on, with this one if not -1
+  int left[8];            // the first piece that a softmax warp has not finished
+  int counted[2];         // pieces up to the last split one that a tile has counted
   int last[2];
   int turn;               // turns of A's products issued so far
 };
@@ -141,11 +145,15 @@ struct TcArgs {
   uint32_t* counters;   // [slots][2], of the splits that are done, by tile; zero between calls
   float4* part;         // [slots][D / 4][256]
   float2* stat;         // [slots][256]: maximum, sum
+  Withheld withheld;    // testing: a CTA that stops loading
 };
 
 // A warp's wait for a phase of a barrier. Bounded: each try suspends for 20 us at most.
-// Once one has expired (here or in another warp) the warp is `dead`: it runs through what
-// is left of its part without waiting, so that nothing depends on the state of a lane.
+// Once one has expired (here or in another warp) the warp is `dead`: it waits for nothing and
+// issues nothing any more, makes the rows it is at NaN and leaves. What
+// the CTA was given and has not finished, and the rest of the list, are then made NaN too and
+// counted where others count on them (clean_up): every row of the call is right or NaN, and the
+// counters are zero after it.
 // (Short on purpose: the loops of the softmax warps fill the instruction caches, and what
 // the other warps run between two MMAs is fetched anew every time.)
 __device__ __forceinline__ void wait_for(uint64_t* bar, uint32_t ph, int* err, bool& dead) {
@@ -343,6 +351,241 @@ struct Blocks {
   }
 };
 
+// The rows of a piece that is not to be worked out any more: NaN. Where they are one of several
+// ranges of keys, this one is NaN for whoever adds them up, and counted: `count` has a bit for
+// each tile that has not been. Warp-wide.
+template <typename T, int D>
+__device__ __noinline__ void void_piece(const TcArgs& g, const Piece& p, int count) {
+  const mkb_attn_args& a = g.a;
+  const int lane = threadIdx.x & 31;
+  constexpr int kLanes = D / 8;  // of a row
+  for (int i = lane / kLanes; i < p.toks * g.group; i += 32 / kLanes) {
+    const int tok = i / g.group;
+    T* const out = static_cast<T*>(a.out) + (p.first + p.tok0 + tok) * a.out_stride[0] +
+                   (p.hk * g.group + i - tok * g.group) * a.out_stride[1];
+    reinterpret_cast<uint4*>(out)[lane % kLanes] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+  }
+  if (p.splits == 1) return;
+  for (int t = 0; t < (p.halves ? 1 : 2); ++t) {
+    if (!(count >> t & 1)) continue;
+    float2* const stat = g.stat + static_cast<size_t>(p.slot + p.split) * kRows + 128 * t;
+    for (int i = lane; i < 128; i += 32) stat[i] = make_float2(0.f, NAN);
+    __threadfence();
+    __syncwarp();
+    if (lane == 0) atomicInc(g.counters + 2 * p.slot + t, p.splits - 1);
+  }
+}
+
+// Which piece comes next, worked out by one warp: handed to the CTA's other warps or, after a
+// stop (kDrain), taken off the list and made NaN. `mine` is the lane's first request.
+template <typename T, int D, bool kPaged, bool kDrain>
+__device__ __forceinline__ void hand_out(const TcArgs& g, TcSmem<D>& sm, Load mine, bool& dead) {
+  // (a warp of its own: the place in the list takes 5,000 cycles to work out, and the loads
+  // of the next piece came that much late: 12 prompts of 1-1,411 tokens 37.7 us, now 35.3)
+  const mkb_attn_args& a = g.a;
+  const int lane = threadIdx.x & 31, kv_heads = a.kv_heads, grid = gridDim.x;
+  // One pass over the requests: their blocks as pairs of tiles and as single ones, what
+  // those come to in turns (linear in the block), and the longest.
+  const Blocks pairs = {2, 2 * g.tile_tokens, g.tile_mul}, singles = {1, g.tile_tokens, g.tile_mul};
+  int n2 = 0, n1 = 0, longest = 0, top = 0;
+  float total2 = 0.f, total1 = 0.f;
+  for (int b = lane; b < a.batch; b += 32) {
+    const Load l = b < 32 ? mine : load_of<kPaged>(g, b);
+    const int b2 = pairs.of(l), b1 = singles.of(l), t2 = pairs.turns(l, l.tiles), t1 = singles.turns(l, l.tiles);
+    n2 += b2;
+    n1 += b1;
+    longest = max(longest, l.tiles);
+    top = max(top, t2);
+    total2 += 0.5f * (pairs.turns(l, tiles_of(l, pairs.span)) + t2) * b2;
+    total1 += 0.5f * (singles.turns(l, tiles_of(l, singles.span)) + t1) * b1;
+  }
+  n2 = __reduce_add_sync(0xffffffffu, n2) * kv_heads;
+  n1 = __reduce_add_sync(0xffffffffu, n1) * kv_heads;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  // pairs of tiles; single ones where the pairs are fewer than the CTAs, unless the keys are
+  // few and not all of those would have a CTA either (1,200 tokens 20.3 us, in pairs 29.5)
+  const bool single = n2 <= grid && (longest >= kMinSplit || n1 <= grid);
+  const Blocks blocks = single ? singles : pairs;
+  float total = single ? total1 : total2;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  top = single ? (longest + 1) / 2 : __reduce_max_sync(0xffffffffu, top);
+  int count = single ? n1 : n2;  // of pieces
+  // a fair share of the turns and a quarter; rows with more are split (but for those that stand
+  // before position 0). 12 prompts of 1-1,411 tokens: 35.7 us, at the bare share 52.5.
+  const int cap = max(kMinSplit, static_cast<int>(fminf(total * kv_heads * 1.25f / grid, 1e9f)) + 1);
+  auto share = [&](Load& l) {
+    l.blocks = blocks.of(l);
+    l.turns = blocks.turns(l, l.tiles);
+    l.splits = l.turns > cap && l.ctx >= 0 ? static_cast<int>((static_cast<unsigned>(l.turns) + cap - 1) / cap) : 1;
+  };
+  share(mine);
+  auto request = [&](int b) {  // of lane b % 32
+    if (b < 32) return mine;
+    Load l = load_of<kPaged>(g, b);
+    share(l);
+    return l;
+  };
+  const bool any_split = top > cap;
+  if (any_split) {
+    top = count = 0;
+    for (int b = lane; b < a.batch; b += 32) {
+      const Load l = request(b);
+      count += l.blocks * l.splits;
+      top = max(top, (l.turns + l.splits - 1) / l.splits);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    count = __reduce_add_sync(0xffffffffu, count) * kv_heads;
+  }
+  // pieces of more than x turns each, all requests
+  auto pieces_above = [&](int x) {
+    int n = 0;
+#pragma unroll 1
+    for (int b = lane; b < a.batch; b += 32) {
+      const Load l = request(b);
+      n += blocks.above(l, x * l.splits) * l.splits;
+    }
+    return __reduce_add_sync(0xffffffffu, n) * kv_heads;
+  };
+  // longest first, unless every piece has a CTA of its own (or the list is long: even anyway)
+  const bool sorted = a.batch <= kSortBatch && count > grid;
+  int k = 0, pending = kDrain ? sm.pending : blockIdx.x;  // (-1: none)
+  for (;; ++k) {
+    const int st = k & 1;
+    int want = pending;
+    if (kDrain ? k > 0 || want < 0 : k > 0) {
+      pending = -1;
+      if (!kDrain) wait_for(&sm.ask, (k - 1) & 1, &sm.err, dead);
+      if (!kDrain && dead) break;
+      if (lane == 0) want = grid + static_cast<int>(atomicAdd(g.work, 1u));
+      want = __shfl_sync(0xffffffffu, want, 0);
+    }
+    // the level (turns of a piece) that `want` falls into, and its place there; the next
+    // one wanted is never on a higher level
+    int lo = 0, r = want;
+    bool found = want < count;
+    if (sorted && found) {
+      int hi = top, at_hi = 0, n = 0;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if ((n = pieces_above(mid)) <= want) {
+          hi = mid;
+          at_hi = n;
+        } else {
+          lo = mid + 1;
+        }
+      }
+      top = lo;
+      r = want - (at_hi > 0 ? at_hi : pieces_above(lo));
+    }
+    if (!kDrain && k >= 2) {
+      wait_for(&sm.info_empty[st], ((k >> 1) - 1) & 1, &sm.err, dead);
+      if (dead) {
+        pending = want;
+        break;
+      }
+    }
+    Piece& p = kDrain ? sm.lost : sm.piece[st];
+    int slot_base = 0;
+    for (int b0 = 0; b0 < a.batch && found; b0 += 32) {
+      const int b = b0 + lane;
+      Load l = {};
+      int above = 0, here = 0, slots = 0, sp = 1;
+      if (b < a.batch) {
+        l = request(b);
+        sp = l.splits;
+        if (sorted) above = blocks.above(l, lo * sp);
+        here = (sorted ? blocks.above(l, (lo - 1) * sp) - above : l.blocks) * sp * kv_heads;
+        slots = sp > 1 ? l.blocks * sp * kv_heads : 0;
+      }
+      int inc = here, sinc = slots;  // inclusive prefix sums
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      if (any_split) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, sinc, o);
+          if (lane >= o) sinc += y;
+        }
+      }
+      const bool is_it = r >= inc - here && r < inc;
+      if (is_it) {
+        unsigned at = static_cast<unsigned>(r) - (inc - here), split = 0;
+        if (sp > 1) {
+          split = at % static_cast<unsigned>(sp);
+          at /= static_cast<unsigned>(sp);
+        }
+        const unsigned i0 = at / static_cast<unsigned>(kv_heads);
+        const int hk = at - i0 * kv_heads, i = l.blocks - 1 - above - static_cast<int>(i0);  // longest first
+        const int tok0 = i * blocks.span, toks = min(l.q - tok0, blocks.span);
+        const int n = tiles_of(l, tok0 + toks);
+        const int per = sp > 1 ? static_cast<int>((static_cast<unsigned>(n) + sp - 1) / sp) : n;
+        const int k0 = min(static_cast<int>(split) * per, n), k1 = min(k0 + per, n), total = k1 - k0;
+        const bool halves = toks <= g.tile_tokens;
+        p.b = b;
+        p.hk = hk;
+        p.first = l.first;
+        p.tok0 = tok0;
+        p.toks = toks;
+        p.ctx = l.ctx;
+        p.len = l.len;
+        p.k0 = k0;
+        p.total = total;
+        p.n[0] = halves ? (total + 1) / 2 : max(min(tiles_of(l, tok0 + g.tile_tokens), k1) - k0, 0);
+        p.n[1] = halves ? total / 2 : total;
+        p.halves = halves;
+        p.splits = sp;
+        p.split = split;
+        p.slot = slot_base + sinc - slots + (i * kv_heads + hk) * sp;
+        p.flags = l.bad ? kBad : 0;
+        if (l.bad) report(a.status, MKB_SERVE_BAD_LENGTH);
+      }
+      if (__any_sync(0xffffffffu, is_it)) break;
+      r -= __shfl_sync(0xffffffffu, inc, 31);
+      slot_base += __shfl_sync(0xffffffffu, sinc, 31);
+      found = b0 + 32 < a.batch;
+    }
+    if (!kDrain) {
+      if (!found && lane == 0) p.b = -1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.info_full[st]);
+    }
+    if (!found) break;
+    if (kDrain) {
+      __syncwarp();
+      void_piece<T, D>(g, p, 3);
+      __syncwarp();
+    }
+  }
+  if (!kDrain && lane == 0) {
+    sm.handed = k;
+    sm.open = dead;
+    sm.pending = pending;
+  }
+  if (!kDrain && dead) return;  // (the rest of the list after the CTA's other warps)
+  // the last CTA to have asked for its last piece puts the list back to its start
+  if (lane == 0 && atomicInc(g.work + 1, grid - 1) == static_cast<uint32_t>(grid - 1)) atomicExch(g.work, 0u);
+}
+// What a CTA leaves that has stopped: the last two pieces that it was given, as far as they
+// are not finished, and the rest of the list. Warp-wide.
+template <typename T, int D, bool kPaged>
+__device__ __noinline__ void clean_up(const TcArgs& g, TcSmem<D>& sm) {
+  const int lane = threadIdx.x & 31;
+  for (int k = max(sm.handed - 2, 0); k < sm.handed; ++k) {
+    if (__any_sync(0xffffffffu, lane < 8 && sm.left[lane & 7] <= k))
+      void_piece<T, D>(g, sm.piece[k & 1], (sm.counted[0] <= k) | (sm.counted[1] <= k) << 1);
+    __syncwarp();
+  }
+  if (!sm.open) return;
+  Load mine = {};
+  if (lane < g.a.batch) mine = load_of<kPaged>(g, lane);
+  bool dead = true;
+  hand_out<T, D, kPaged, true>(g, sm, mine, dead);
+}
+
 template <typename T, int D, bool kPaged>
 __global__ void __launch_bounds__(kTcThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -375,6 +618,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_init(&sm.ask, 1);
     mbar_init(&sm.pair_full, 4);
     mbar_init(&sm.pair_empty, 4);
+    for (int w = 0; w < 8; ++w) sm.left[w] = 0x7fffffff;
+    sm.counted[0] = sm.counted[1] = 0;
     sm.err = sm.turn = 0;
     fence_mbar_init();
   }
@@ -396,173 +641,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == 11) {
-    // ---- which piece comes next ----------------------------------------------------------
-    // (a warp of its own: the place in the list takes 5,000 cycles to work out, and the loads
-    // of the next piece came that much late: 12 prompts of 1-1,411 tokens 37.7 us, now 35.3)
-    const int kv_heads = a.kv_heads, grid = gridDim.x;
-    // One pass over the requests: their blocks as pairs of tiles and as single ones, what
-    // those come to in turns (linear in the block), and the longest.
-    const Blocks pairs = {2, 2 * g.tile_tokens, g.tile_mul}, singles = {1, g.tile_tokens, g.tile_mul};
-    int n2 = 0, n1 = 0, longest = 0, top = 0;
-    float total2 = 0.f, total1 = 0.f;
-    for (int b = lane; b < a.batch; b += 32) {
-      const Load l = b < 32 ? mine : load_of<kPaged>(g, b);
-      const int b2 = pairs.of(l), b1 = singles.of(l), t2 = pairs.turns(l, l.tiles), t1 = singles.turns(l, l.tiles);
-      n2 += b2;
-      n1 += b1;
-      longest = max(longest, l.tiles);
-      top = max(top, t2);
-      total2 += 0.5f * (pairs.turns(l, tiles_of(l, pairs.span)) + t2) * b2;
-      total1 += 0.5f * (singles.turns(l, tiles_of(l, singles.span)) + t1) * b1;
-    }
-    n2 = __reduce_add_sync(0xffffffffu, n2) * kv_heads;
-    n1 = __reduce_add_sync(0xffffffffu, n1) * kv_heads;
-    longest = __reduce_max_sync(0xffffffffu, longest);
-    // pairs of tiles; single ones where the pairs are fewer than the CTAs, unless the keys are
-    // few and not all of those would have a CTA either (1,200 tokens 20.3 us, in pairs 29.5)
-    const bool single = n2 <= grid && (longest >= kMinSplit || n1 <= grid);
-    const Blocks blocks = single ? singles : pairs;
-    float total = single ? total1 : total2;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    top = single ? (longest + 1) / 2 : __reduce_max_sync(0xffffffffu, top);
-    int count = single ? n1 : n2;  // of pieces
-    // a fair share of the turns and a quarter; rows with more are split (but for those that stand
-    // before position 0). 12 prompts of 1-1,411 tokens: 35.7 us, at the bare share 52.5.
-    const int cap = max(kMinSplit, static_cast<int>(fminf(total * kv_heads * 1.25f / grid, 1e9f)) + 1);
-    auto share = [&](Load& l) {
-      l.blocks = blocks.of(l);
-      l.turns = blocks.turns(l, l.tiles);
-      l.splits = l.turns > cap && l.ctx >= 0 ? static_cast<int>((static_cast<unsigned>(l.turns) + cap - 1) / cap) : 1;
-    };
-    share(mine);
-    auto request = [&](int b) {  // of lane b % 32
-      if (b < 32) return mine;
-      Load l = load_of<kPaged>(g, b);
-      share(l);
-      return l;
-    };
-    const bool any_split = top > cap;
-    if (any_split) {
-      top = count = 0;
-      for (int b = lane; b < a.batch; b += 32) {
-        const Load l = request(b);
-        count += l.blocks * l.splits;
-        top = max(top, (l.turns + l.splits - 1) / l.splits);
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      count = __reduce_add_sync(0xffffffffu, count) * kv_heads;
-    }
-    // pieces of more than x turns each, all requests
-    auto pieces_above = [&](int x) {
-      int n = 0;
-#pragma unroll 1
-      for (int b = lane; b < a.batch; b += 32) {
-        const Load l = request(b);
-        n += blocks.above(l, x * l.splits) * l.splits;
-      }
-      return __reduce_add_sync(0xffffffffu, n) * kv_heads;
-    };
-    // longest first, unless every piece has a CTA of its own (or the list is long: even anyway)
-    const bool sorted = a.batch <= kSortBatch && count > grid;
-    for (int k = 0; !dead; ++k) {
-      const int st = k & 1;
-      int want = blockIdx.x;
-      if (k > 0) {
-        wait_for(&sm.ask, (k - 1) & 1, &sm.err, dead);
-        if (dead) break;
-        if (lane == 0) want = grid + static_cast<int>(atomicAdd(g.work, 1u));
-        want = __shfl_sync(0xffffffffu, want, 0);
-      }
-      // the level (turns of a piece) that `want` falls into, and its place there; the next
-      // one wanted is never on a higher level
-      int lo = 0, r = want;
-      bool found = want < count;
-      if (sorted && found) {
-        int hi = top, at_hi = 0, n = 0;
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if ((n = pieces_above(mid)) <= want) {
-            hi = mid;
-            at_hi = n;
-          } else {
-            lo = mid + 1;
-          }
-        }
-        top = lo;
-        r = want - (at_hi > 0 ? at_hi : pieces_above(lo));
-      }
-      if (k >= 2) wait_for(&sm.info_empty[st], ((k >> 1) - 1) & 1, &sm.err, dead);
-      Piece& p = sm.piece[st];
-      int slot_base = 0;
-      for (int b0 = 0; b0 < a.batch && found; b0 += 32) {
-        const int b = b0 + lane;
-        Load l = {};
-        int above = 0, here = 0, slots = 0, sp = 1;
-        if (b < a.batch) {
-          l = request(b);
-          sp = l.splits;
-          if (sorted) above = blocks.above(l, lo * sp);
-          here = (sorted ? blocks.above(l, (lo - 1) * sp) - above : l.blocks) * sp * kv_heads;
-          slots = sp > 1 ? l.blocks * sp * kv_heads : 0;
-        }
-        int inc = here, sinc = slots;  // inclusive prefix sums
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int x = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += x;
-        }
-        if (any_split) {
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, sinc, o);
-            if (lane >= o) sinc += y;
-          }
-        }
-        const bool is_it = r >= inc - here && r < inc;
-        if (is_it) {
-          unsigned at = static_cast<unsigned>(r) - (inc - here), split = 0;
-          if (sp > 1) {
-            split = at % static_cast<unsigned>(sp);
-            at /= static_cast<unsigned>(sp);
-          }
-          const unsigned i0 = at / static_cast<unsigned>(kv_heads);
-          const int hk = at - i0 * kv_heads, i = l.blocks - 1 - above - static_cast<int>(i0);  // longest first
-          const int tok0 = i * blocks.span, toks = min(l.q - tok0, blocks.span);
-          const int n = tiles_of(l, tok0 + toks);
-          const int per = sp > 1 ? static_cast<int>((static_cast<unsigned>(n) + sp - 1) / sp) : n;
-          const int k0 = min(static_cast<int>(split) * per, n), k1 = min(k0 + per, n), total = k1 - k0;
-          const bool halves = toks <= g.tile_tokens;
-          p.b = b;
-          p.hk = hk;
-          p.first = l.first;
-          p.tok0 = tok0;
-          p.toks = toks;
-          p.ctx = l.ctx;
-          p.len = l.len;
-          p.k0 = k0;
-          p.total = total;
-          p.n[0] = halves ? (total + 1) / 2 : max(min(tiles_of(l, tok0 + g.tile_tokens), k1) - k0, 0);
-          p.n[1] = halves ? total / 2 : total;
-          p.halves = halves;
-          p.splits = sp;
-          p.split = split;
-          p.slot = slot_base + sinc - slots + (i * kv_heads + hk) * sp;
-          p.flags = l.bad ? kBad : 0;
-          if (l.bad) report(a.status, MKB_SERVE_BAD_LENGTH);
-        }
-        if (__any_sync(0xffffffffu, is_it)) break;
-        r -= __shfl_sync(0xffffffffu, inc, 31);
-        slot_base += __shfl_sync(0xffffffffu, sinc, 31);
-        found = b0 + 32 < a.batch;
-      }
-      if (!found && lane == 0) p.b = -1;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.info_full[st]);
-      if (!found) break;
-    }
-    // the last CTA to have asked for its last piece puts the list back to its start
-    if (lane == 0 && atomicInc(g.work + 1, grid - 1) == static_cast<uint32_t>(grid - 1)) atomicExch(g.work, 0u);
+    hand_out<T, D, kPaged, false>(g, sm, mine, dead);
   } else if (warp == 9) {
     // ---- the loads of a piece -----------------------------------------------------------------
     if (lane == 0) {
@@ -577,6 +656,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       wait_for(&sm.info_full[st], (k >> 1) & 1, &sm.err, dead);
       const Piece p = sm.piece[st];
       if (p.b < 0 || dead) break;
+      if (g.withheld.here() && k >= g.withheld.from) break;
       // K(0), then K(j + 1) and V(j): the order in which the products take them
       const int n = p.total;
       int pages = 0, pages_at = 0, pages_end = 0;  // the lanes' pages: boxes of keys up to pages_end
@@ -714,16 +794,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // the first tile of keys that the piece's first row does not see in full
       const int sees = uniform(sm.piece[st].ctx) + uniform(sm.piece[st].tok0) + 1;
       const int look = sees < uniform(sm.piece[st].len) ? max(sees / kKeys, 0) - uniform(sm.piece[st].k0) : 0x7fffffff;
-      const bool stop = uniform(sm.piece[st].b) < 0;
+      const bool end = uniform(sm.piece[st].b) < 0;
+      if (dead) break;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.info_empty[st]);
-      if (stop || dead) break;
+      if (end) break;
       if (n == 0) continue;
       if (mine_n > 0) {
         wait_for(&sm.q_full[t], q_ph, &sm.err, dead);
         q_ph ^= 1;
       }
       wait_for(&sm.kv_full[slot], ring, &sm.err, dead);
+      if (dead) break;
       int todo = from, done = from;  // the next tile of scores, of outputs
       auto maybe_scores = [&](int j, int s) {
         if (j != todo || j > last) return;
@@ -746,10 +828,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // pages: 28 requests decoding and two chunks 62.5 us, 64.4 in order; prompts lose 1 %)
         const bool mine = j == done && j <= last, early = kPaged && !mine && j + 1 < n;
         if (early) {
+          if (dead) break;
           maybe_scores(j + 1, sk);
           commit(leader, &sm.kv_empty[sk]);
         }
         wait_for(&sm.kv_full[slot], ring, &sm.err, dead);  // V(j)
+        if (dead) break;
         if (mine) {
           const int valid = left - j * kKeys;
           if (valid < kKeys) {  // rows past the last key: whatever lies there, P = 0 must give 0 (both warps clear them)
@@ -800,11 +884,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             dead = __any_sync(0xffffffffu, dead);
           }
           wait_for(&sm.p_part[t], p_ph, &sm.err, dead);
+          if (dead) break;
           tc::fence_after_sync();
 #pragma unroll
           for (int kk = 0; kk < kFirstKeys / 16; ++kk)  // O (+)= P V
             mma_ts(leader, to_, ts + 8 * kk, tc::desc_advance(dv, 16 * kk * row), id_o, (j - from | kk) != 0);
           wait_for(&sm.p_full[t], p_ph, &sm.err, dead);
+          if (dead) break;
           p_ph ^= 1;
           tc::fence_after_sync();
 #pragma unroll
@@ -841,10 +927,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       wait_for(&sm.tile_bar[t], t_ph, &sm.err, dead);
       t_ph ^= 1;
     };
+    int k = 0;
 #pragma unroll 1
-    for (int k = 0; !dead; ++k) {
+    for (; !dead; ++k) {
       const int st = k & 1;
       wait_for(&sm.info_full[st], (k >> 1) & 1, &sm.err, dead);
+      if (dead) break;
       const Piece p = sm.piece[st];
       auto release = [&]() {
         __syncwarp();
@@ -864,6 +952,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 1
       for (int j = 0; j < n; ++j) {
         wait_for(&sm.s_full[t], s_ph, &sm.err, dead);
+        if (dead) break;
         s_ph ^= 1;
         tc::fence_after_sync();
         uint32_t sr[kKeys];
@@ -964,7 +1053,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         m = mm;
       }
       const int flags = *reinterpret_cast<volatile int*>(&sm.piece[st].flags);
-      const bool bad = (flags & kBad) != 0, odd = (flags & kOdd) != 0;
+      const bool bad = (flags & kBad) != 0 || dead, odd = (flags & kOdd) != 0;
       release();
       const int k_end = min(p.len, (p.k0 + p.total) * kKeys);
       constexpr int kPer = D / 32;
@@ -1090,12 +1179,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (split) {
         __threadfence();
         tile_sync();
-        if (threadIdx.x % 128 == 0)
+        if (threadIdx.x % 128 == 0 && !dead) {
           *reinterpret_cast<volatile int*>(&sm.last[t]) =
               atomicInc(g.counters + 2 * p.slot + t, p.splits - 1) ==
               static_cast<uint32_t>(p.splits - 1);
+          sm.counted[t] = k + 1;
+        }
         tile_sync();
-        if (*reinterpret_cast<volatile int*>(&sm.last[t]) != 0) {
+        if (!dead && *reinterpret_cast<volatile int*>(&sm.last[t]) != 0) {
           __threadfence();
           float mm = -INFINITY, ll = 0.f;
           for (int s = 0; s < p.splits && live; ++s) mm = fmaxf(mm, __ldcg(g.stat + slot_of(s) * kRows + at).x);
@@ -1140,11 +1231,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       tc::fence_before_sync();  // O has been read: the next piece's first PV may overwrite it
     }
-    if (lane == 0) tma_store_done();
+    if (lane == 0) {
+      tma_store_done();
+      if (dead) sm.left[warp] = k - 1;  // (the one it was at when it stopped, or the last before)
+    }
   }
   tc::fence_before_sync();
   __syncthreads();
-  if (threadIdx.x == 0 && sm.err) report(a.status, MKB_SERVE_TIMEOUT);
+  if (sm.err) {
+    if (threadIdx.x == 0) report(a.status, MKB_SERVE_TIMEOUT);
+    for (int i = 0; i < 100; ++i) __nanosleep(100000);  // (products still in flight)
+    if (warp == 11) clean_up<T, D, kPaged>(g, sm);
+    __syncthreads();
+  }
   if (warp == 8) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tbase, 512);
@@ -1223,6 +1322,7 @@ static cudaError_t tc_launch(const mkb_attn_args& a, cudaStream_t stream) {
   g.group_mul = 65536 / g.group + 1;
   g.k_head = a.k_stride[1] != 0;
   g.v_head = a.v_stride[1] != 0;
+  g.withheld = withheld();
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   if (ws == nullptr) return cudaErrorInvalidValue;
   g.tile_mul = g.tile_tokens > 1 ? static_cast<unsigned>((1ull << 32) / g.tile_tokens + 1) : 0;

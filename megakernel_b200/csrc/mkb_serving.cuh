@@ -161,6 +161,14 @@ cudaError_t launch_early(void (*kernel)(P...), int grid, int threads, size_t sme
   return cudaLaunchKernelEx(&c, kernel, std::forward<A>(args)...);
 }
 
+// ---- testing -----------------------------------------------------------------------------
+// CTA `cta` (-1: none, -2: each) loads its first `from` pieces and no more.
+struct Withheld {
+  int cta, from;
+  __device__ __forceinline__ bool here() const { return cta != -1 && (cta == -2 || cta == static_cast<int>(blockIdx.x)); }
+};
+Withheld withheld();  // of a launch: mkb_attn.cu
+
 // ---- host: what the entry points check ---------------------------------------------------
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool strides_ok(const int64_t* s, int n) {  // (whole 16 bytes of the 16-bit types)

@@ -189,3 +189,49 @@ def test_output_in_place_of_q(new, kv):
     got = mk.paged_attention(q, c.kc, c.vc, c.table, c.lens, cu, out=q)
     assert got.data_ptr() == q.data_ptr()
     assert torch.equal(got.nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
+
+
+# ---- a wait that runs out ------------------------------------------------------------------
+
+@pytest.fixture
+def withhold():
+    """Makes a CTA of the calls that follow stop loading, so that its waits run out."""
+    from megakernel_b200 import _lib
+    lib = _lib.load()
+    yield lib.mkb_attn_withhold
+    lib.mkb_attn_withhold(-1, 0)
+    mk.serving_status()
+
+
+def calls_to_stop():
+    lens = [900, 45, 1300, 1]
+    q, k, v = prompts(lens, 16, 8, 128, seed=4)
+    many = prompts([33] * 300, 8, 4, 64, seed=5)
+    c = Cache([30000, 50, 7000, 1], 2, 128, 16, seed=6)
+    few, cu = rand(seeded(11), 33, 16, 128), cu_of([1, 30, 1, 1])
+    long = Cache([1500] * 60, 8, 128, 16, seed=7)
+    one = rand(seeded(12), 60, 16, 128)
+    return {"prompts": (mk.prompt_attention, (q, k, v, cu_of(lens))),
+            "many prompts": (mk.prompt_attention, (*many, cu_of([33] * 300))),
+            "split rows": (mk.paged_attention, (few, c.kc, c.vc, c.table, c.lens, cu)),
+            "decode": (mk.paged_attention, (one, long.kc, long.vc, long.table, long.lens))}
+
+
+@pytest.mark.parametrize("name,cta,start", [(name, cta, 0) for cta in (3, -2) for name in
+                                            ("prompts", "many prompts", "split rows", "decode")] +
+                         [("prompts", -2, 1), ("many prompts", 0, 1), ("many prompts", -2, 1), ("many prompts", -2, 3)])
+def test_a_wait_that_runs_out_leaves_rows_right_or_nan_and_the_next_call_right(name, cta, start, withhold):
+    """With a CTA that loads nothing, or nothing after its first piece of work, and with all of them."""
+    call, args = calls_to_stop()[name]
+    want = call(*args)
+    assert mk.serving_status() == (0, "ok") and not want.isnan().any()
+    out = torch.full_like(want, 7.0)
+    withhold(cta, start)
+    call(*args, out=out)
+    withhold(-1, 0)
+    after = call(*args)  # on the same workspace
+    lost = out.isnan()
+    assert torch.equal(out[~lost], want[~lost])
+    assert torch.equal(after, want)
+    assert lost.all() if cta == -2 and start == 0 else lost.any() and (cta == -2 or not lost.all())
+    assert mk.serving_status()[0] == 4 and mk.serving_status()[0] == 0
