@@ -332,6 +332,8 @@ pybind11::object paged_append(const Tensor& qkv, const Tensor& k_cache, const Te
   const int64_t d = qkv.dim(), dim = qkv.size(d - 1);
   TORCH_CHECK_VALUE(dim == 64 || dim == 128, "the head dimension must be 64 or 128, got ", dim);
   const Paging p = paging_of(k_cache, v_cache, block_table, kv_lens, dim, dev);
+  check_apart(k_cache, "k_cache", 1);  // (attention may read one head for all; here each is written)
+  check_apart(v_cache, "v_cache", 1);
   a.dtype = type_code(k_cache, "k_cache");
   const Batch b = batch_of(qkv, "qkv", cu_q, kv_lens.size(0), dev);
   const int64_t heads = qkv.size(d - 2) - 2 * static_cast<int64_t>(p.kv_heads);

@@ -202,5 +202,7 @@ extern "C" cudaError_t mkb_paged_append(const mkb_append_args* a, cudaStream_t s
       !aligned16(a->v_cache) || !strides_ok(a->qkv_stride, 2) || !strides_ok(a->k_stride, 3) ||
       !strides_ok(a->v_stride, 3))
     return cudaErrorMisalignedAddress;
+  for (const int64_t* s : {a->k_stride, a->v_stride})  // every row is written at a place of its own
+    if ((a->pages > 1 && !s[0]) || (a->kv_heads > 1 && !s[1]) || !s[2]) return cudaErrorInvalidValue;
   return a->dtype == MKB_BF16 ? append_source<__nv_bfloat16>(*a, stream) : append_source<__half>(*a, stream);
 }

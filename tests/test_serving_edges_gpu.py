@@ -235,3 +235,15 @@ def test_a_wait_that_runs_out_leaves_rows_right_or_nan_and_the_next_call_right(n
     assert torch.equal(after, want)
     assert lost.all() if cta == -2 and start == 0 else lost.any() and (cta == -2 or not lost.all())
     assert mk.serving_status()[0] == 4 and mk.serving_status()[0] == 0
+
+
+# ---- calls ----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("which", ["k_cache", "v_cache"])
+def test_append_refuses_a_cache_whose_heads_are_one(which):
+    c = Cache([20, 30], 2, 128, 16)
+    cos, sin = mk.rope_tables(64, DEV)
+    caches = {"k_cache": c.kc, "v_cache": c.vc}
+    caches[which] = caches[which][:, :1].expand(-1, 2, -1, -1)
+    with pytest.raises(ValueError, match=which):
+        mk.paged_append(rand(seeded(0), 2, 8, 128), **caches, block_table=c.table, kv_lens=c.lens, cos=cos, sin=sin)
