@@ -106,7 +106,7 @@ __device__ __forceinline__ void mma16816(float c[4], const uint32_t a[4], uint32
 
 // Tiles of a request (one for a request without keys: its zeros have to be written).
 __device__ __forceinline__ int dec_tiles(const DecArgs& g, int b, int* len_out, bool* bad_out) {
-  const int len = max(__ldg(g.a.kv_lens + b), 0);
+  const int len = max(g.a.kv_lens[b], 0);
   const bool bad = static_cast<int64_t>(len) > static_cast<int64_t>(g.a.table_width) * g.a.page_size;
   *len_out = len;
   *bad_out = bad;
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
         pages_b = ahead.b;
         pages_at = ahead.t;
         const int key = (ahead.t + lane) * kTileKeys;  // 16 keys lie in one page
-        pages = key < ahead.len ? __ldg(a.block_table + ahead.b * a.table_stride + key / a.page_size) : 0;
+        pages = key < ahead.len ? a.block_table[ahead.b * a.table_stride + key / a.page_size] : 0;
         if (pages < 0 || pages >= a.pages) {
           report(a.status, MKB_SERVE_BAD_PAGE);
           pages = -1;
@@ -300,8 +300,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
                                                           h * a.q_stride[1]);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
-      qf[kk][0] = live ? __ldg(q + 8 * kk + lane % 4) : 0;
-      qf[kk][1] = live ? __ldg(q + 8 * kk + 4 + lane % 4) : 0;
+      qf[kk][0] = live ? q[8 * kk + lane % 4] : 0;
+      qf[kk][1] = live ? q[8 * kk + 4 + lane % 4] : 0;
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {

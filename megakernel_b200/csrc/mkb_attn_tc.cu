@@ -315,7 +315,7 @@ __device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
   Load l;
   l.first = rq.first;
   l.q = rq.n;
-  l.len = kPaged ? max(__ldg(g.a.kv_lens + b), 0) : rq.n;
+  l.len = kPaged ? max(g.a.kv_lens[b], 0) : rq.n;
   l.bad = kPaged && static_cast<int64_t>(l.len) > static_cast<int64_t>(g.a.table_width) * g.a.page_size;
   l.ctx = l.len - l.q;
   l.tiles = l.bad || l.q == 0 ? 0 : static_cast<int>((static_cast<unsigned>(l.len) + kKeys - 1) / kKeys);
@@ -682,7 +682,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int at = pages_at + lane * box;
             pages = -2;  // past the last key: outside the pool, which reads as zeros
             if (at < p.len) {
-              pages = __ldg(a.block_table + p.b * a.table_stride + (at >> 31 - __clz(a.page_size)));
+              pages = a.block_table[p.b * a.table_stride + (at >> 31 - __clz(a.page_size))];
               if (pages < 0 || pages >= a.pages) pages = -1;
             }
           }

@@ -63,13 +63,13 @@ __device__ __forceinline__ uint4 pack8(const float v[8]) {
 // The request of packed token `t` (every lane of a warp calls it, all with the same
 // t): how many of cu[1 .. batch] are <= t. 32 probes at a time: one load deep up to
 // 32 requests, two up to 1,024.
-__device__ __forceinline__ int request_of(const int* __restrict__ cu, int batch, int t) {
+__device__ __forceinline__ int request_of(const int* cu, int batch, int t) {
   const int lane = threadIdx.x & 31;
   int lo = 0, n = batch;  // the answer lies in [lo, lo + n], cu[lo] <= t
   while (n > 0) {
     const int step = (n + 31) / 32;
     const int at = lo + (lane + 1) * step;  // probes cu[at], the last of its stretch
-    const bool below = at <= lo + n && __ldg(cu + at) <= t;
+    const bool below = at <= lo + n && cu[at] <= t;
     const int full = __popc(__ballot_sync(0xffffffffu, below));
     lo += full * step;
     n = step == 1 ? 0 : min(step - 1, n - full * step);
@@ -82,12 +82,12 @@ __device__ __forceinline__ int request_of(const int* __restrict__ cu, int batch,
 struct Request {
   int b, first, n;
 };
-__device__ __forceinline__ Request request_rows(const int* __restrict__ cu, int b, int q_len, int tokens) {
+__device__ __forceinline__ Request request_rows(const int* cu, int b, int q_len, int tokens) {
   if (cu == nullptr) return {b, b * q_len, q_len};
-  const int first = min(max(__ldg(cu + b), 0), tokens);
-  return {b, first, max(min(__ldg(cu + b + 1), tokens) - first, 0)};
+  const int first = min(max(cu[b], 0), tokens);
+  return {b, first, max(min(cu[b + 1], tokens) - first, 0)};
 }
-__device__ __forceinline__ Request request_at(const int* __restrict__ cu, int batch, int q_len, int tokens, int t) {
+__device__ __forceinline__ Request request_at(const int* cu, int batch, int q_len, int tokens, int t) {
   return request_rows(cu, cu == nullptr ? t / q_len : request_of(cu, batch, t), q_len, tokens);
 }
 
@@ -142,7 +142,9 @@ __device__ __noinline__ void sum_odd(const mkb_attn_args& a, int b, int first, i
 // ---- early launch ----------------------------------------------------------------------
 // A kernel of this family may be brought in while the one before it in the stream is
 // still running its last blocks: it sets itself up, and waits (depend_wait) before it
-// touches memory until all that came before has completed.
+// touches memory until all that came before has completed. What it reads may be written
+// during its life, so its loads are plain ones: no path for read-only data, no pointer
+// declared free of aliases, which would let the compiler take that path or move a load.
 __device__ __forceinline__ void depend_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void depend_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

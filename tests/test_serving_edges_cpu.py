@@ -1,7 +1,10 @@
-"""More that the C entry points of the serving operators refuse before anything is launched."""
+"""The serving operators without a GPU: more that the C entry points refuse before anything is
+launched, and what their sources must not hold."""
+import os
+
 import pytest
 
-from megakernel_b200 import _lib
+from megakernel_b200 import _lib, build
 from test_serving_cpu import INVALID, append
 
 
@@ -10,3 +13,13 @@ from test_serving_cpu import INVALID, append
 def test_append_refuses_rows_at_one_place(kw):
     """Strides of 0 between KV heads, pages or slots: several rows would be written to the same memory."""
     assert _lib.load().mkb_paged_append(append(**kw), None) == INVALID
+
+
+@pytest.mark.parametrize("source", ["mkb_append.cu", "mkb_attn_tc.cu", "mkb_attn_decode.cu", "mkb_serving.cuh"])
+def test_kernels_that_start_early_use_coherent_loads(source):
+    """These kernels are brought in while the one before them in the stream still runs. A load of
+    data that has to be read-only for the kernel's whole life (ld.global.nc) would be of memory
+    that the one before may be writing, as the append writes a decode step's q."""
+    with open(os.path.join(build.CSRC, source)) as f:
+        text = f.read()
+    assert "__ldg(" not in text and "__restrict__" not in text and ".nc" not in text
