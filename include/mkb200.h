@@ -339,9 +339,9 @@ typedef struct mkb_attn_args {
   int64_t table_stride;
   int table_width, pages, page_size; /* page_size a power of two, 16 or more */
   float scale;                 /* scores are scale * q.k */
-  void* workspace;             /* device, mkb_attn_workspace_bytes(); zeroed once with
-                                  mkb_attn_workspace_reset and left ready for the next call
-                                  of any shape that fits.
+  void* workspace;             /* device, mkb_attn_workspace_bytes(); made ready once with
+                                  mkb_attn_workspace_reset (which clears its counters) and
+                                  left ready for the next call of any shape that fits.
                                   Calls that share one must not overlap in time. */
   uint32_t* status;            /* device uint32 or NULL */
 } mkb_attn_args;

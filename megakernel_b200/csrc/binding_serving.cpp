@@ -5,8 +5,9 @@
 // numbers live on the device and are checked there (see serving_status). A call
 // launches on the caller's current stream, synchronises nothing and can be captured
 // into a CUDA graph. The attention's workspace is kept per device and stream, so
-// that calls on different streams never share one; a capture gets its own, zeroed
-// by the graph.
+// that calls on different streams never share one; a captured call gets its own, whose
+// counters (5 KB) the graph clears. (A replayed decode call over one request of 33 keys takes
+// 7.9 us, over 48 of 1-4,096 58.4; 27.9 and 87.2 where all of its 79 MB are cleared.)
 
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -110,13 +111,17 @@ Tensor workspace_of(c10::Device dev, cudaStream_t stream, size_t bytes) {
   const auto options = torch::TensorOptions().dtype(torch::kByte).device(dev);
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   C10_CUDA_CHECK(cudaStreamIsCapturing(stream, &cap));
-  if (cap != cudaStreamCaptureStatusNone) return torch::zeros({static_cast<int64_t>(bytes)}, options);
+  auto fresh = [&] {
+    const Tensor t = torch::empty({static_cast<int64_t>(bytes)}, options);
+    C10_CUDA_CHECK(mkb_attn_workspace_reset(t.data_ptr(), bytes, stream));
+    return t;
+  };
+  if (cap != cudaStreamCaptureStatusNone) return fresh();
   unsigned long long id = 0;
   C10_CUDA_CHECK(cudaStreamGetId(stream, &id));
   std::lock_guard<std::mutex> lk(kept().mu);
   Tensor& t = kept().workspace[{dev.index(), id}];
-  if (!t.defined() || static_cast<size_t>(t.numel()) < bytes)
-    t = torch::zeros({static_cast<int64_t>(bytes + bytes / 4)}, options);  // the old one is freed in stream order
+  if (!t.defined() || static_cast<size_t>(t.numel()) < bytes) t = fresh();  // the old one is freed in stream order
   return t;
 }
 

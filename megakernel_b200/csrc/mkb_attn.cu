@@ -13,6 +13,7 @@ size_t tc_workspace(const mkb_attn_args& a);
 cudaError_t attn_decode(const mkb_attn_args& a, cudaStream_t stream);  // mkb_attn_decode.cu
 size_t decode_workspace(const mkb_attn_args& a);
 bool decode_fits(const mkb_attn_args& a);
+size_t counter_bytes();  // at the start of either's workspace
 
 static std::atomic<Withheld> g_withheld{Withheld{-1, 0}};
 Withheld withheld() { return g_withheld.load(std::memory_order_relaxed); }
@@ -65,7 +66,9 @@ size_t mkb_attn_workspace_bytes(const mkb_attn_args* a) {
 }
 
 cudaError_t mkb_attn_workspace_reset(void* workspace, size_t bytes, cudaStream_t stream) {
-  return cudaMemsetAsync(workspace, 0, bytes, stream);
+  // the counters: partial results are written before they are read
+  const size_t counters = mkb::sv::counter_bytes();
+  return cudaMemsetAsync(workspace, 0, bytes < counters ? bytes : counters, stream);
 }
 
 void mkb_attn_withhold(int cta, int from) { mkb::sv::g_withheld.store({cta, from}); }
