@@ -296,7 +296,7 @@ void mkb_engine_destroy(mkb_engine* e);
  * q_len tokens each (tokens == batch * q_len). Query head h reads KV head
  * h / (heads / kv_heads). Strides are in elements; the last dimension (head_dim,
  * 64 or 128) is contiguous; every base is 16-byte aligned and every other stride
- * a multiple of 8 elements.
+ * a multiple of 16 bytes.
  *
  * The paged cache is two pools of pages, addressed as page * stride[0] + KV head *
  * stride[1] + slot * stride[2]. Key j of request b lies in page block_table[b,

@@ -199,7 +199,7 @@ extern "C" cudaError_t mkb_paged_append(const mkb_append_args* a, cudaStream_t s
     return cudaErrorInvalidValue;
   if (!aligned16(a->qkv) || !aligned16(a->q_norm) || !aligned16(a->k_norm) || !aligned16(a->cos_table) ||
       !aligned16(a->sin_table) || !aligned16(a->q_out) || !aligned16(a->k_out) || !aligned16(a->k_cache) ||
-      !aligned16(a->v_cache) || !strides_ok(a->qkv_stride, 2) || !strides_ok(a->k_stride, 3) ||
+      !aligned16(a->v_cache) || !strides_ok(a->qkv_stride, 2, a->source_dtype == MKB_FP32 ? 4 : 8) || !strides_ok(a->k_stride, 3) ||
       !strides_ok(a->v_stride, 3))
     return cudaErrorMisalignedAddress;
   for (const int64_t* s : {a->k_stride, a->v_stride})  // every row is written at a place of its own

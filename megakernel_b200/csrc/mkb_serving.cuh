@@ -173,9 +173,9 @@ Withheld withheld();  // of a launch: mkb_attn.cu
 
 // ---- host: what the entry points check ---------------------------------------------------
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-inline bool strides_ok(const int64_t* s, int n) {  // (whole 16 bytes of the 16-bit types)
+inline bool strides_ok(const int64_t* s, int n, int unit = 8) {  // whole 16 bytes: 8 values of the 16-bit types
   for (int i = 0; i < n; ++i)
-    if (s[i] < 0 || s[i] % 8) return false;
+    if (s[i] < 0 || s[i] % unit) return false;
   return true;
 }
 

@@ -274,3 +274,15 @@ def test_a_captured_call_clears_no_more_than_its_counters():
     direct, replayed = elapsed(layers), elapsed(graph.replay)
     assert all(torch.equal(x, want) for x in out)
     assert replayed < direct + n * 6e-3, (direct, replayed)  # ms: 6 us a call
+
+
+def test_append_from_fp32_with_strides_of_four_elements():
+    """16 bytes are four FP32 values: strides need be no more."""
+    c = Cache([20, 30], 2, 128, 16)
+    cos, sin = mk.rope_tables(64, DEV)
+    wide = rand(seeded(3), 2, 9, 132, dtype=torch.float32)
+    qkv = wide[:, 1:, 4:]
+    assert qkv.stride(0) % 8 and qkv.stride(1) % 8
+    q = mk.paged_append(qkv, c.kc, c.vc, c.table, c.lens, cos, sin)
+    want = mk.paged_append(qkv.contiguous(), c.kc, c.vc, c.table, c.lens, cos, sin)
+    assert torch.equal(q, want)
