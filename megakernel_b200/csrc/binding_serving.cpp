@@ -195,10 +195,14 @@ void set_query(mkb_attn_args& a, const Tensor& q, const Tensor& out, const Batch
   a.scale = static_cast<float>(s);
 }
 
-void check_heads(int heads, int64_t kv_heads) {
+void check_heads(int heads, int64_t kv_heads, const Batch& b) {
   TORCH_CHECK_VALUE(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, heads, " query heads are no multiple of ",
                     kv_heads, " KV heads");
   TORCH_CHECK_VALUE(heads / kv_heads <= 128, "at most 128 query heads may share a KV head, got ", heads / kv_heads);
+  // (rows and their blocks, over all heads, are counted in 32 bits)
+  TORCH_CHECK_VALUE(static_cast<int64_t>(b.tokens) + b.batch <= (int64_t{1} << 30) / heads, b.tokens, " tokens and ",
+                    b.batch, " requests of ", heads, " heads are more than can be counted: at most ",
+                    (int64_t{1} << 30) / heads);
 }
 
 struct Paging {
@@ -268,7 +272,7 @@ Tensor prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   const Tensor out = output_for(out_, q, dev);
   set_query(a, q, out, b, scale);
   a.kv_heads = as_int(k.size(1), "kv_heads");
-  check_heads(a.heads, a.kv_heads);
+  check_heads(a.heads, a.kv_heads, b);
   if (a.tokens == 0) return out;
   a.k = k.data_ptr();
   a.v = v.data_ptr();
@@ -301,7 +305,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_c
   const Tensor out = output_for(out_, q, dev);
   set_query(a, q, out, b, scale);
   a.kv_heads = p.kv_heads;
-  check_heads(a.heads, a.kv_heads);
+  check_heads(a.heads, a.kv_heads, b);
   if (a.tokens == 0) return out;
   a.k = k_cache.data_ptr();
   a.v = v_cache.data_ptr();

@@ -16,7 +16,8 @@ Without ``cu_q`` every request brings one token (``[batch, heads, dim]``) or ``n
 dim]`` (any strides of whole 16 bytes, so another order of the dimensions is a
 permuted view), ``block_table[b]`` lists request ``b``'s pages and ``kv_lens[b]``
 counts its keys, the new tokens included. BF16 or FP16, heads of 64 or 128, up
-to 128 query heads per KV head, pages of a power of two of 16 keys or more.
+to 128 query heads per KV head, pages of a power of two of 16 keys or more; tokens and
+requests together, times the query heads, up to 2^30.
 
 A token sees the keys up to its own position; one that sees none gets zeros. What a
 page holds past a request's last key reaches no output. Calls run on the current

@@ -286,3 +286,11 @@ def test_append_from_fp32_with_strides_of_four_elements():
     q = mk.paged_append(qkv, c.kc, c.vc, c.table, c.lens, cos, sin)
     want = mk.paged_append(qkv.contiguous(), c.kc, c.vc, c.table, c.lens, cos, sin)
     assert torch.equal(q, want)
+
+
+def test_more_tokens_and_requests_than_can_be_counted_are_refused():
+    n = 2 ** 20
+    pool = torch.zeros((1, 8, 16, 64), dtype=BF, device=DEV)
+    table, lens, cu = (torch.zeros(s, dtype=torch.int32, device=DEV) for s in ((n, 1), (n,), (n + 1,)))
+    with pytest.raises(ValueError, match="tokens"):
+        mk.paged_attention(torch.zeros((1, 1024, 64), dtype=BF, device=DEV), pool, pool, table, lens, cu)
