@@ -13,6 +13,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime.h>
 
@@ -98,11 +99,17 @@ Tensor status_of(c10::Device dev) {
   std::lock_guard<std::mutex> lk(kept().mu);
   Tensor& t = kept().status[dev.index()];
   if (!t.defined()) {
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    C10_CUDA_CHECK(cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream().stream(), &cap));
-    if (cap != cudaStreamCaptureStatusNone) return Tensor();  // not from a graph's memory: the word outlives it
-    t = torch::zeros({1}, torch::TensorOptions().dtype(torch::kInt).device(dev));
-    C10_CUDA_CHECK(cudaStreamSynchronize(at::cuda::getCurrentCUDAStream().stream()));  // once per device
+    // once per device, in memory of its own and cleared on a stream of its own: the first call
+    // may be one that is captured, and the word outlives the graph
+    const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+    void* word = nullptr;
+    cudaStream_t side = nullptr;
+    C10_CUDA_CHECK(cudaMalloc(&word, sizeof(int)));
+    C10_CUDA_CHECK(cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking));
+    C10_CUDA_CHECK(cudaMemsetAsync(word, 0, sizeof(int), side));
+    C10_CUDA_CHECK(cudaStreamSynchronize(side));
+    C10_CUDA_CHECK(cudaStreamDestroy(side));
+    t = torch::from_blob(word, {1}, torch::TensorOptions().dtype(torch::kInt).device(dev));
   }
   return t;
 }
@@ -283,7 +290,7 @@ Tensor prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
   const Tensor ws = workspace_of(dev, stream, mkb_attn_workspace_bytes(&a)), st = status_of(dev);
   a.workspace = ws.data_ptr();
-  a.status = st.defined() ? reinterpret_cast<uint32_t*>(st.data_ptr()) : nullptr;
+  a.status = reinterpret_cast<uint32_t*>(st.data_ptr());
   C10_CUDA_CHECK(mkb_prompt_attention(&a, stream));
   return out;
 }
@@ -322,7 +329,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_c
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
   const Tensor ws = workspace_of(dev, stream, mkb_attn_workspace_bytes(&a)), st = status_of(dev);
   a.workspace = ws.data_ptr();
-  a.status = st.defined() ? reinterpret_cast<uint32_t*>(st.data_ptr()) : nullptr;
+  a.status = reinterpret_cast<uint32_t*>(st.data_ptr());
   C10_CUDA_CHECK(mkb_paged_attention(&a, stream));
   return out;
 }
@@ -409,7 +416,7 @@ pybind11::object paged_append(const Tensor& qkv, const Tensor& k_cache, const Te
     a.pages = p.pages;
     a.page_size = p.page_size;
     const Tensor st = status_of(dev);
-    a.status = st.defined() ? reinterpret_cast<uint32_t*>(st.data_ptr()) : nullptr;
+    a.status = reinterpret_cast<uint32_t*>(st.data_ptr());
     C10_CUDA_CHECK(mkb_paged_append(&a, at::cuda::getCurrentCUDAStream().stream()));
   }
   if (!return_k) return pybind11::cast(q);

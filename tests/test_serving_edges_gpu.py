@@ -294,3 +294,31 @@ def test_more_tokens_and_requests_than_can_be_counted_are_refused():
     table, lens, cu = (torch.zeros(s, dtype=torch.int32, device=DEV) for s in ((n, 1), (n,), (n + 1,)))
     with pytest.raises(ValueError, match="tokens"):
         mk.paged_attention(torch.zeros((1, 1024, 64), dtype=BF, device=DEV), pool, pool, table, lens, cu)
+
+
+def test_errors_are_kept_where_the_first_call_of_a_process_is_captured():
+    import os
+    import subprocess
+    import sys
+    code = """if True:
+        import torch
+        import megakernel_b200 as mk
+        pool = torch.zeros((3, 2, 16, 128), dtype=torch.bfloat16, device="cuda")
+        table, lens = (torch.full(s, 7, dtype=torch.int32, device="cuda") for s in ((2, 1), (2,)))
+        q = torch.zeros((2, 4, 128), dtype=torch.bfloat16, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = mk.paged_attention(q, pool, pool, table, lens)
+        assert mk.serving_status() == (0, "ok")
+        graph.replay()
+        assert out.isnan().all()
+        code = mk.serving_status()[0]
+        assert code == 1, code
+        lens.fill_(0)
+        graph.replay()
+        assert bool((out == 0).all()) and mk.serving_status()[0] == 0
+        print("kept")
+    """
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "kept" in r.stdout, r.stderr[-2000:]
