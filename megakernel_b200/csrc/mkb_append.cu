@@ -194,8 +194,10 @@ extern "C" cudaError_t mkb_paged_append(const mkb_append_args* a, cudaStream_t s
   if ((a->head_dim != 64 && a->head_dim != 128) || a->heads < 1 || a->kv_heads < 1) return cudaErrorInvalidValue;
   if (a->cu_q == nullptr && (a->q_len < 1 || (int64_t)a->q_len * a->batch != a->tokens)) return cudaErrorInvalidValue;
   if (a->page_size < 16 || (a->page_size & (a->page_size - 1)) || a->pages < 0 || a->table_width < 0 || a->rope_rows < 0) return cudaErrorInvalidValue;
-  if (!a->qkv || !a->q_out || !a->k_cache || !a->v_cache || !a->kv_lens || !a->block_table || !a->cos_table ||
-      !a->sin_table)
+  if (!a->qkv || !a->q_out || !a->kv_lens) return cudaErrorInvalidValue;
+  // (no pages, entries or positions: no memory of them either)
+  if ((a->pages > 0 && (!a->k_cache || !a->v_cache)) || (a->table_width > 0 && !a->block_table) ||
+      (a->rope_rows > 0 && (!a->cos_table || !a->sin_table)))
     return cudaErrorInvalidValue;
   if (!aligned16(a->qkv) || !aligned16(a->q_norm) || !aligned16(a->k_norm) || !aligned16(a->cos_table) ||
       !aligned16(a->sin_table) || !aligned16(a->q_out) || !aligned16(a->k_out) || !aligned16(a->k_cache) ||
@@ -203,6 +205,6 @@ extern "C" cudaError_t mkb_paged_append(const mkb_append_args* a, cudaStream_t s
       !strides_ok(a->v_stride, 3))
     return cudaErrorMisalignedAddress;
   for (const int64_t* s : {a->k_stride, a->v_stride})  // every row is written at a place of its own
-    if ((a->pages > 1 && !s[0]) || (a->kv_heads > 1 && !s[1]) || !s[2]) return cudaErrorInvalidValue;
+    if (a->pages > 0 && ((a->pages > 1 && !s[0]) || (a->kv_heads > 1 && !s[1]) || !s[2])) return cudaErrorInvalidValue;
   return a->dtype == MKB_BF16 ? append_source<__nv_bfloat16>(*a, stream) : append_source<__half>(*a, stream);
 }

@@ -322,3 +322,19 @@ def test_errors_are_kept_where_the_first_call_of_a_process_is_captured():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "kept" in r.stdout, r.stderr[-2000:]
+
+
+def test_append_to_a_pool_without_pages_or_a_table_without_entries():
+    """Nothing can be stored: what needs a page is reported, what needs none is not."""
+    cos, sin = mk.rope_tables(64, DEV)
+    qkv = rand(seeded(4), 2, 8, 128)
+    pool = torch.empty((0, 2, 16, 128), dtype=BF, device=DEV)
+    some = torch.zeros((3, 2, 16, 128), dtype=BF, device=DEV)
+    table = torch.zeros((2, 4), dtype=torch.int32, device=DEV)
+    lens = torch.tensor([0, 5], dtype=torch.int32, device=DEV)
+    for caches, entries, code in ((pool, table, 1), (some, table[:, :0], 2)):
+        q = mk.paged_append(qkv, caches, caches.clone(), entries, lens, cos, sin)
+        assert bool((q[0] == 0).all()) and q[1].isnan().all()
+        assert mk.serving_status()[0] == code
+    q = mk.paged_append(qkv, some, some.clone(), table, lens, cos[:0], sin[:0])
+    assert bool((q[0] == 0).all()) and q[1].isnan().all() and mk.serving_status()[0] == 3
