@@ -111,10 +111,9 @@ __global__ void __launch_bounds__(kAppendThreads, 6) append_kernel(const mkb_app
       load8(s + d0, sn);
       load8(s + d1, sn + 8);
     }
-  } else {  // no such position: q reads as zeros, or as NaN where that is an error
-#pragma unroll
-    for (int i = 0; i < 16; ++i) cs[i] = sn[i] = bad != 0 ? __int_as_float(0x7fffffff) : 0.f;
   }
+  // no such position: zeros, or NaN where that is an error, whatever the token holds
+  const uint32_t none = bad != 0 ? 0x7fff7fffu : 0u;
 
   for (int r0 = 0; r0 < rows; r0 += kRows) {
     const int row = r0 + row0;
@@ -149,7 +148,8 @@ __global__ void __launch_bounds__(kAppendThreads, 6) append_kernel(const mkb_app
         x[i + 8] = hi * cs[i + 8] + lo * sn[i + 8];
       }
     }
-    const uint4 u0 = pack8<T>(x), u1 = pack8<T>(x + 8);
+    uint4 u0 = pack8<T>(x), u1 = pack8<T>(x + 8);
+    if (!store) u0 = u1 = make_uint4(none, none, none, none);
     T* dst = nullptr;
     if (row < a.heads) {
       dst = static_cast<T*>(a.q_out) + ((size_t)t * a.heads + row) * D;

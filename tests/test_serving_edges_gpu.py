@@ -338,3 +338,15 @@ def test_append_to_a_pool_without_pages_or_a_table_without_entries():
         assert mk.serving_status()[0] == code
     q = mk.paged_append(qkv, some, some.clone(), table, lens, cos[:0], sin[:0])
     assert bool((q[0] == 0).all()) and q[1].isnan().all() and mk.serving_status()[0] == 3
+
+
+@pytest.mark.parametrize("bad", [NAN, INF])
+def test_append_before_position_0_gives_zeros_whatever_the_token_holds(bad):
+    c = Cache([0, 30], 2, 128, 16)
+    cos, sin = mk.rope_tables(64, DEV)
+    w = rand(seeded(6), 128)
+    for norm in (dict(), dict(q_norm=w, k_norm=w)):
+        qkv = rand(seeded(5), 2, 8, 128)
+        qkv[0, 0, 3] = qkv[0, 5, 100] = bad
+        q, k = mk.paged_append(qkv, c.kc, c.vc, c.table, c.lens, cos, sin, return_k=True, **norm)
+        assert bool((q[0] == 0).all()) and bool((k[0] == 0).all()) and q[1].isfinite().all()
