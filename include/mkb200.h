@@ -316,7 +316,7 @@ void mkb_engine_destroy(mkb_engine* e);
 enum { MKB_BF16 = 0, MKB_FP16 = 1, MKB_FP32 = 2 };
 enum {
   MKB_SERVE_BAD_PAGE = 1,      /* block_table names a page outside the pool */
-  MKB_SERVE_BAD_LENGTH = 2,    /* kv_lens[b] exceeds the table's width in keys */
+  MKB_SERVE_BAD_LENGTH = 2,    /* kv_lens[b] exceeds the table's width in keys, or 2^30 */
   MKB_SERVE_BAD_POSITION = 3,  /* a position past the RoPE tables (append) */
   MKB_SERVE_TIMEOUT = 4        /* a bounded wait inside the kernel expired */
 };

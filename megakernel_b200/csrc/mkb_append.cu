@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kAppendThreads, 6) append_kernel(const mkb_app
   fetch(row0);
   const Request rq = request_at(a.cu_q, a.batch, a.q_len, a.tokens, t);
   const int b = rq.b, at = t - rq.first;
-  const int pos = at >= 0 && at < rq.n ? a.kv_lens[b] - rq.n + at : -1;
+  const int pos = at >= 0 && at < rq.n ? max(a.kv_lens[b], 0) - rq.n + at : -1;
   int64_t page = -1;
   uint32_t bad = 0;
   if (pos >= 0) {

@@ -107,7 +107,7 @@ __device__ __forceinline__ void mma16816(float c[4], const uint32_t a[4], uint32
 // Tiles of a request (one for a request without keys: its zeros have to be written).
 __device__ __forceinline__ int dec_tiles(const DecArgs& g, int b, int* len_out, bool* bad_out) {
   const int len = max(g.a.kv_lens[b], 0);
-  const bool bad = static_cast<int64_t>(len) > static_cast<int64_t>(g.a.table_width) * g.a.page_size;
+  const bool bad = len > kMaxKeys || static_cast<int64_t>(len) > static_cast<int64_t>(g.a.table_width) * g.a.page_size;
   *len_out = len;
   *bad_out = bad;
   return bad ? 1 : max((len + kTileKeys - 1) / kTileKeys, 1);
@@ -201,8 +201,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
       ahead.len = __shfl_sync(0xffffffffu, ln, src);
       ahead.bad = __shfl_sync(0xffffffffu, static_cast<int>(bd), src) != 0;
       ahead.pos += __shfl_sync(0xffffffffu, inc - own, src);
-      const unsigned at = static_cast<unsigned>(from - ahead.pos);  // (under 2^31: tiles of one request, all heads)
-      ahead.hk = static_cast<int>(at / static_cast<unsigned>(ahead.n + 1));
+      ahead.hk = static_cast<int>((from - ahead.pos) / (ahead.n + 1));
       ahead.pos += static_cast<int64_t>(ahead.n + 1) * ahead.hk;
       break;
     }

@@ -316,7 +316,7 @@ __device__ __forceinline__ Load load_of(const TcArgs& g, int b) {
   l.first = rq.first;
   l.q = rq.n;
   l.len = kPaged ? max(g.a.kv_lens[b], 0) : rq.n;
-  l.bad = kPaged && static_cast<int64_t>(l.len) > static_cast<int64_t>(g.a.table_width) * g.a.page_size;
+  l.bad = kPaged && (l.len > kMaxKeys || static_cast<int64_t>(l.len) > static_cast<int64_t>(g.a.table_width) * g.a.page_size);
   l.ctx = l.len - l.q;
   l.tiles = l.bad || l.q == 0 ? 0 : static_cast<int>((static_cast<unsigned>(l.len) + kKeys - 1) / kKeys);
   return l;

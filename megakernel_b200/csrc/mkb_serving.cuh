@@ -77,6 +77,9 @@ __device__ __forceinline__ int request_of(const int* cu, int batch, int t) {
   return min(lo, batch - 1);
 }
 
+// Keys of a request at most: they are counted in 32 bits, with room for the tiles past the last.
+constexpr int kMaxKeys = 1 << 30;
+
 // Where packed token `t`'s request lies: its rows first .. first + n - 1, clamped to
 // the batch so that no offsets of the caller's lead out of it.
 struct Request {

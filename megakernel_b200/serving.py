@@ -34,7 +34,7 @@ import torch
 STATUS_NAMES = {
     0: "ok",
     1: "block_table names a page outside the pool",
-    2: "kv_lens counts more keys than block_table has pages for",
+    2: "kv_lens counts more keys than block_table has pages for, or than 2^30",
     3: "a position past the RoPE tables",
     4: "timeout of a wait inside a kernel",
 }

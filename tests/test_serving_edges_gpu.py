@@ -350,3 +350,23 @@ def test_append_before_position_0_gives_zeros_whatever_the_token_holds(bad):
         qkv[0, 0, 3] = qkv[0, 5, 100] = bad
         q, k = mk.paged_append(qkv, c.kc, c.vc, c.table, c.lens, cos, sin, return_k=True, **norm)
         assert bool((q[0] == 0).all()) and bool((k[0] == 0).all()) and q[1].isfinite().all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_lengths_past_two_to_the_thirty_are_reported(new):
+    """A table may list a page many times; keys are counted in 32 bits, with room for a tile."""
+    pool = torch.zeros((1, 1, 2 ** 16, 64), dtype=BF, device=DEV)
+    table = torch.zeros((2, 2 ** 15), dtype=torch.int32, device=DEV)
+    q = torch.zeros((2 * new, 1, 64), dtype=BF, device=DEV)
+    cu = None if new == 1 else cu_of([new, new])
+    for n in (2 ** 31 - 1, 2 ** 30 + 1):
+        lens = torch.tensor([50, n], dtype=torch.int32, device=DEV)
+        got = mk.paged_attention(q, pool, pool, table, lens, cu)
+        assert bool((got[:new] == 0).all()) and got[new:].isnan().all()
+        assert mk.serving_status()[0] == 2
+    lens = torch.tensor([50, -2 ** 31], dtype=torch.int32, device=DEV)  # no keys: tokens before position 0
+    assert bool((mk.paged_attention(q, pool, pool, table, lens, cu) == 0).all())
+    cos = torch.ones((64, 64), device=DEV)
+    qkv = torch.ones((2 * new, 3, 64), dtype=BF, device=DEV)
+    got = mk.paged_append(qkv, pool, pool.clone(), table, lens, cos, cos, cu)
+    assert bool((got[new:] == 0).all()) and mk.serving_status() == (0, "ok")
