@@ -669,17 +669,22 @@ static cudaError_t decode_launch(const mkb_attn_args& a, cudaStream_t stream) {
 
 // Rows (new tokens x query heads of a KV head) known from the shapes alone, and few: up to 4;
 // up to 8 where there are few requests and KV heads, whose keys have to be shared out over the
-// SMs. This kernel against the tensor-core tiles, heads 16 over 8 of 128 unless named:
-//   2 rows: 48 requests of 1-4,096 keys 58 and 66 us, 9,001-60,000 keys 78 and 95, 33 keys 7.3 and 9.2
-//   8 rows: 48 requests 71 and 66, four of 300-1,000 keys 26 and 17 (heads 16 over 2: 36 and 32 for
-//           the 48); 9,001-60,000 keys 89 and 90, one of 33 keys 8.6 and 9.3, heads 16 over 2 and
-//           500-30,000 keys 42 and 54
+// SMs, and the table has room for long ones (how long they are only the device knows). This
+// kernel against the tensor-core tiles, heads 16 over 8 of 128 unless named, us:
+//   2 rows: 48 requests of 1-4,096 keys 58 and 66, 9,001-60,000 keys 78 and 95, 33 keys 7.3 and 9.2
+//   8 rows: 48 requests 71 and 66; three of 500-1,000 keys 26.9 and 17.6, of 4,000-8,000 37.7 and
+//           36.0, of 16,000-32,000 69.7 and 72.6; one of 700 keys 15.0 and 15.2, of 8,000 34.4 and
+//           33.8, of 16,000 40.8 and 44.3
+//   8 rows, heads 16 over 2: four of 300-1,000 keys 23.5 and 16.9, 12 of 300-1,000 27.2 and 17.2, of
+//           666-8,000 35.5 and 34.1, of 1,333-16,000 43.9 and 45.2, of 2,666-32,000 58.7 and 64.5
 //   16 rows, by two columns of products: 48 requests 100 and 71
+constexpr int kLongTable = 16384;
 bool decode_fits(const mkb_attn_args& a) {
   if (a.cu_q != nullptr) return false;
   const int64_t rows = static_cast<int64_t>(a.q_len) * (a.heads / a.kv_heads);
-  const int64_t most = static_cast<int64_t>(a.batch) * a.kv_heads * 6 <= sm_count() ? kDecRows : kDecRows / 2;
-  return rows <= most;
+  const bool few = static_cast<int64_t>(a.batch) * a.kv_heads * 6 <= sm_count();
+  const bool longer = static_cast<int64_t>(a.table_width) * a.page_size >= kLongTable;
+  return rows <= (few && longer ? kDecRows : kDecRows / 2);
 }
 
 template <typename T>

@@ -97,6 +97,33 @@ def test_decode_of_several_tokens_with_values_that_some_do_not_see(n):
     check_any(got.flatten(0, 1), *want_of(c, q.flatten(0, 1), [n] * len(kv)), BF)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("hq,hk,d,n", [(14, 2, 128, 1), (16, 2, 64, 1), (5, 1, 128, 1), (6, 2, 128, 2), (2, 1, 64, 4)])
+def test_five_to_eight_rows_over_a_table_for_long_requests(n, hq, hk, d, dtype):
+    """Room for 16,384 keys or more, of which the requests use any part."""
+    kv = [n, 40, 16384, 700]
+    c = Cache(kv, hk, d, 16, dtype, seed=n, width=1100)
+    for b, m in enumerate(kv):
+        plant(c, b, m - 1, 0, 3, INF)
+        plant(c, b, m // 2, hk - 1, 4, (NAN, -INF)[b % 2])
+    q = rand(seeded(25), 4, n, hq, d, dtype=dtype, scale=0.25)
+    got = mk.paged_attention(q, c.kc, c.vc, c.table, c.lens)
+    check_any(got.flatten(0, 1), *want_of(c, q.flatten(0, 1), [n] * 4), dtype)
+
+
+def test_few_short_requests_of_eight_rows_take_no_longer_than_with_offsets():
+    """With offsets the tensor-core tiles run: where they are faster they run without, too."""
+    c = Cache([500, 700, 1000], 8, 128, 16)
+    q, cu = rand(seeded(26), 12, 16, 128), cu_of([4, 4, 4])
+
+    def times(call):
+        graph, _ = captured(call, 20)
+        return elapsed(graph.replay, 5)
+
+    direct = times(lambda: mk.paged_attention(q.view(3, 4, 16, 128), c.kc, c.vc, c.table, c.lens))
+    assert direct < 1.2 * times(lambda: mk.paged_attention(q, c.kc, c.vc, c.table, c.lens, cu))
+
+
 def spoil(v, at):
     """Values at (key, head, dim) of v, in place."""
     for key, head, dim, value in at:
