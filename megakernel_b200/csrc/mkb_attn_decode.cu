@@ -13,7 +13,7 @@
 // are: S^T's accumulators, transposed by movmatrix, are the B operand of
 // O^T += V^T P^T, and V^T comes from V by ldmatrix.trans. P enters as a 16-bit high part
 // and the remainder: memory leaves time for the second product, and P then costs no
-// precision. The products take finite values of V only: a remainder of 0, or a row that
+// precision (in FP16, which ends at 2^-24, P is 2^15 times larger). The products take finite values of V only: a remainder of 0, or a row that
 // does not see the key, would make NaN of an infinity. A tile is looked over for the others
 // first (48 requests of 1-4,096 keys 57.9 us, 57.7 without; three of 9,001-60,000 78.7 and
 // 78.1); they are added to the rows that see them, as they are, and cleared.
@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
                        const __grid_constant__ DecArgs g) {
   constexpr int kBytes = kStageBytes<D>, kHalf = kTileKeys * 128;  // (64 values of 16 keys)
   constexpr int kRing = kStages<D>;
+  constexpr float kLift = Pair<T>::kDtype == MKB_FP16 ? 15.f : 0.f;  // P and its sum times 2^kLift
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[kDecWarps][kRing];
@@ -367,8 +368,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
         const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: weights of 0
         const float sc = ex2_approx(m[e] - ref);
         m[e] = mn;
-        p[e] = ex2_approx(x0 - ref);
-        p[2 + e] = ex2_approx(x1 - ref);
+        p[e] = ex2_approx(x0 - (ref - kLift));
+        p[2 + e] = ex2_approx(x1 - (ref - kLift));
         l[e] = l[e] * sc + (p[e] + p[2 + e]);  // of this lane's keys: added up at the end
         if (__any_sync(0xffffffffu, sc != 1.f)) {
 #pragma unroll

@@ -33,8 +33,10 @@
 //
 // The running maximum that P is relative to moves only when a row's grows by more than 8
 // (a factor 256): O, in tensor memory, is then rescaled by the softmax warps; between
-// moves P stays below 2^8, which FP32 sums and 16-bit P hold without loss. P is rounded
-// to the operands' 16-bit type, as the output is: the same relative error.
+// moves P stays below 2^8, which FP32 sums and BF16 hold without loss. P is rounded to the
+// operands' 16-bit type, as the output is: the same relative error. FP16 has no relative
+// error below 2^-14, and nothing below 2^-25: there P is 2^7 times larger (2^15 at most), so
+// that a weight is rounded by 2^-32 of the row's largest at most.
 //
 // Work: a piece is (request, KV head, one or two tiles of rows, a range of key tiles).
 // Every CTA works the list out for itself from the lengths, the longest pieces first, and
@@ -918,6 +920,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t t_s = tbase + lanes + 128 * t, t_o = tbase + lanes + Shape::kO + D * t;
     const float sl2 = g.sl2;
+    constexpr float kLift = Pair<T>::kDtype == MKB_FP16 ? 7.f : 0.f;  // P and its sum times 2^kLift
     uint32_t s_ph = 0, o_ph = 0;
     const int tok_in = row_in * g.group_mul >> 16;
     uint32_t t_ph = 0, pair_ph = 0;
@@ -992,7 +995,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           m = mn;
         }
         // an infinite maximum leaves no weights (inf - inf); none at all, weights of 0
-        const float ref = m == -INFINITY ? 0.f : -m;
+        const float ref = m == -INFINITY ? 0.f : kLift - m;
         const uint64_t ref2 = pack2(ref, ref), sl22 = pack2(sl2, sl2);
         uint64_t la = 0, lb = 0;
         auto arrive = [&](uint64_t* bar) {

@@ -218,6 +218,50 @@ def test_output_in_place_of_q(new, kv):
     assert torch.equal(got.nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0))
 
 
+# ---- small weights ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("gap", [12, 20, 25.3, 27])
+@pytest.mark.parametrize("n", [1, 3])
+def test_many_small_weights_beside_a_large_one(n, gap, dtype):
+    """One key far ahead (by ``gap`` powers of two) of 40,000 that together still count. A 16-bit
+    weight holds 2^-32 of the largest at least (FP16: its smallest value 2^-24, half of that in
+    rounding, and 2^7 of headroom), so the error may be that of every value on top."""
+    m, d = 40000, 64
+    c = Cache([m], 1, d, 16, dtype)
+    lead = gap * math.log(2) * d ** 0.5
+    k, v = torch.zeros((m, 1, d), device=DEV), rand(seeded(31), m, 1, d).float().abs()
+    k[0, 0, 0] = 1
+    v[0] = 0
+    c.k[0], c.v[0] = k.to(dtype), v.to(dtype)
+    ids = c.table[0].long()
+    c.kc[ids, 0], c.vc[ids, 0] = (x.view(-1, 16, d) for x in (c.k[0][:, 0], c.v[0][:, 0]))
+    q = torch.zeros((n, 2, d), dtype=dtype, device=DEV)
+    q[:, :, 0] = lead
+    want, size = attend(q, c.k[0], c.v[0])
+    for cu in (None, cu_of([n])):
+        got = mk.paged_attention(q[None] if cu is None else q, c.kc, c.vc, c.table, c.lens, cu).view(n, 2, d)
+        low = 2.0 ** -32 * c.v[0].double().abs().sum(0) if dtype == FP else 0
+        off = (got.double() - want).abs() - U[dtype] * (want.abs() + size) - low
+        assert float(off.max()) <= 0, (cu is None, float(off.max()))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("gap", [12, 20, 25.3, 27])
+def test_many_small_weights_beside_a_large_one_in_a_long_prompt(gap, dtype):
+    m, d = 16000, 64
+    k, v = torch.zeros((m, 8, d), dtype=dtype, device=DEV), rand(seeded(32), m, 8, d).abs().to(dtype)
+    k[0, :, 0] = 1
+    v[0] = 0
+    q = torch.zeros((m, 16, d), dtype=dtype, device=DEV)
+    q[:, :, 0] = gap * math.log(2) * d ** 0.5
+    got = mk.prompt_attention(q, k, v, cu_of([m]))[-64:]
+    want, size = attend(q[-64:], k, v)
+    low = 2.0 ** -32 * v.double().abs().sum(0).repeat_interleave(2, 0) if dtype == FP else 0
+    off = (got.double() - want).abs() - U[dtype] * (want.abs() + size) - low
+    assert float(off.max()) <= 0, float(off.max())
+
+
 # ---- a wait that runs out ------------------------------------------------------------------
 
 @pytest.fixture
