@@ -306,7 +306,9 @@ void mkb_engine_destroy(mkb_engine* e);
  *
  * A token sees the keys at its own position and before it. One that sees none (a
  * negative position) gets zeros. What lies in the cache past a request's last key
- * (uninitialised memory, NaN) reaches no output.
+ * (uninitialised memory, NaN) reaches no output. Rows of no request (before cu_q[0],
+ * from cu_q[batch] on) are not written by the attention; the append gives zeros.
+ * `out` may be `q`.
  *
  * Lengths live on the device, so they are checked there: a page outside the pool,
  * more keys than the table has room for, or a position past the RoPE tables makes

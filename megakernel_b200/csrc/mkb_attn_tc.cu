@@ -20,11 +20,14 @@
 //   warps 4-7   maximum and sum in FP32 registers, P into tensor memory; tile B
 //
 // While one tile's softmax runs, the tensor core works on the other's products. Tensor core
-// (4 D cycles a 128 x 128 tile: 1,024 at D = 128) and exponentials (1,024: 16 a cycle and SM)
-// bound a pair of tiles at 2,048 cycles each; the chain of one tile (load 215, maximum 450,
-// weights 1,450, the rest of PV and the next S 1,100) makes it 3,250. 15,999 tokens, 16 heads
-// over 8 of 128: 820 us, 1,280 TFLOP/s (of 1,640 that a library GEMM reaches), both units 63 %
-// busy; 980 us once the power limit holds the clock (1,070 of 1,370 TFLOP/s).
+// (8 D cycles for the two products of a 128 x 128 tile: 1,024 at D = 128) and exponentials
+// (1,024: 16 a cycle and SM) bound a pair of tiles at 2,048 cycles each; the chain of one tile
+// (load 215, maximum 450, weights 1,450, the rest of PV and the next S 1,100) makes it 3,250.
+// That is for two tiles of rows; where there is one and the tiles take turns with the keys, the
+// products have no order and a pair takes about 5,000 (four chunks of 512: 24 tiles of keys an
+// SM, tensor core 31 % busy). 15,999 tokens, 16 heads over 8 of 128: 820-850 us, 1,280 TFLOP/s
+// (of 1,640 that a library GEMM reaches), both units 63 % busy; 955 us once the power limit
+// holds the clock (1,100 of 1,370 TFLOP/s).
 // What did not shorten the chain: P in columns of its own, so that the next S need not wait
 // for it (80 keys a tile at D = 128: 2,330 cycles a pair; both tiles' softmax then run at
 // once); the next S in halves, the upper one while the weights are worked out (3-10 % slower:
@@ -52,8 +55,8 @@
 // product looks those over while it waits for P, and where it finds such a value clears it;
 // the softmax warps then add it to the rows that see it, as it is. What every row of the
 // piece sees goes through the product: a weight that rounds to 0 makes NaN of an infinity.
-// (Looking over takes instructions from the softmax warps: 12 prompts of 1-1,411 tokens 36.3 us,
-// 34.7 without; 2,049, 1,000 and 4,097 tokens of 64-wide FP16 118.8, 117.1; two of 4,096 125.3,
+// (Looking over takes instructions from the softmax warps, which the comparisons below do not
+// have in them yet: 12 prompts of 1-1,411 tokens 36.3 us, 34.7 without; 2,049, 1,000 and 4,097 tokens of 64-wide FP16 118.8, 117.1; two of 4,096 125.3,
 // 123.0. 15,999 tokens 802 us; with NaN in all of the first key 834, all of V infinite 1,381.)
 
 #include <cmath>

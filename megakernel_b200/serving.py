@@ -19,11 +19,15 @@ counts its keys, the new tokens included. BF16 or FP16, heads of 64 or 128, up
 to 128 query heads per KV head, pages of a power of two of 16 keys or more; tokens and
 requests together, times the query heads, up to 2^30.
 
-A token sees the keys up to its own position; one that sees none gets zeros. What a
-page holds past a request's last key reaches no output. Calls run on the current
-stream, do not synchronise, and can be captured into a CUDA graph. Host-side misuse
-raises ``ValueError``; lengths and page numbers are read on the device, where a wrong
-one makes its request's new rows NaN, some or all, and is kept for :func:`serving_status`.
+A token sees the keys up to its own position; one that sees none gets zeros, one whose
+scores are all ``-inf`` NaN. What a page holds past a request's last key reaches no
+output, and values that are not finite reach the rows that see them and no others. Rows
+of no request (before ``cu_q[0]``, from ``cu_q[-1]`` on) are not written by the
+attention; the append gives zeros. Calls run on the current stream, do not synchronise,
+and can be captured into a CUDA graph. Host-side misuse raises ``ValueError``; lengths
+and page numbers are read on the device, where a wrong one makes its request's new rows
+NaN, some or all, and is kept for :func:`serving_status`. These are operators of an
+inference framework: results carry no gradients, whatever the inputs do.
 
 There is no CPU or PyTorch fallback.
 """
@@ -53,13 +57,14 @@ def _extension():
 def prompt_attention(q, k, v, cu_seqlens, *, scale=None, out=None):
     """Causal attention of packed prompts: ``q`` [tokens, heads, dim], ``k`` and ``v``
     [tokens, kv_heads, dim], ``cu_seqlens`` int32 [prompts + 1] on the device. ``scale``
-    defaults to ``dim ** -0.5``. Returns [tokens, heads, dim]."""
+    defaults to ``dim ** -0.5``. Returns [tokens, heads, dim], in ``out`` if given, which may
+    be ``q``."""
     return (_ops or _extension()).prompt_attention(q, k, v, cu_seqlens, scale, out)
 
 
 def paged_attention(q, k_cache, v_cache, block_table, kv_lens, cu_q=None, *, scale=None, out=None):
     """Attention of new tokens over the paged cache (their own K/V rows already in it).
-    Returns ``q``'s shape."""
+    Returns ``q``'s shape, in ``out`` if given, which may be ``q``."""
     return (_ops or _extension()).paged_attention(q, k_cache, v_cache, block_table, kv_lens, cu_q, scale, out)
 
 
@@ -75,7 +80,7 @@ def paged_append(qkv, k_cache, v_cache, block_table, kv_lens, cos, sin, cu_q=Non
 
 def serving_status(device=None):
     """(code, name) of the first error that these operators met on ``device`` since the
-    last call; (0, "ok") if none. Waits for the device."""
+    last call, replays of graphs included; (0, "ok") if none. Waits for the device."""
     d = torch.device("cuda" if device is None else device)
     code = int(_extension().serving_status(d.index if d.index is not None else torch.cuda.current_device()))
     return code, STATUS_NAMES.get(code, "unknown")
